@@ -22,6 +22,14 @@ class Stats(C.Structure):
                 ("loop_launches", C.c_int32), ("resident_group", C.c_int32)]
 
 
+class Operand(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("stride", C.c_int64), ("type", C.c_int32), ("reserved", C.c_int32)]
+
+
+_OP = C.POINTER(Operand)
+# workspace, its bytes, stream, error buffer and its length: how the operators' calls end
+_TAIL = [C.c_void_p, C.c_int64, C.c_void_p, C.c_char_p, C.c_int]
+
 # every entry point include/spdnn_b200.h declares
 SYMBOLS = {
     "spdnn_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int, C.c_float, C.c_float]),
@@ -49,6 +57,21 @@ SYMBOLS = {
     "spdnn_layer_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                      C.c_float, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p,
                                      C.c_int]),
+    "spdnn_topology_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_char_p,
+                                        C.c_int]),
+    "spdnn_topology_destroy": (None, [C.c_void_p]),
+    "spdnn_topology_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int),
+                                      C.POINTER(C.c_int64)]),
+    "spdnn_topology_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64]),
+    "spdnn_layer_workspace": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int64)]),
+    "spdnn_linear": (C.c_int, [C.c_void_p, C.c_int, _OP, _OP, C.c_void_p, C.c_int, C.c_float, _OP, _OP, *_TAIL]),
+    "spdnn_gated": (C.c_int, [C.c_void_p, C.c_int, _OP, _OP, _OP, C.c_void_p, C.c_void_p, C.c_int, C.c_float, _OP, _OP, _OP, *_TAIL]),
+    "spdnn_linear_backward": (C.c_int, [C.c_void_p, C.c_int, _OP, _OP, _OP, _OP, C.c_int, C.c_float, _OP, C.c_void_p, C.c_void_p,
+                                        *_TAIL]),
+    "spdnn_gated_backward": (C.c_int, [C.c_void_p, C.c_int, _OP, _OP, _OP, _OP, _OP, _OP, C.c_int, C.c_float, _OP, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, *_TAIL]),
+    "spdnn_mx4_quantize": (C.c_int, [_OP, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_int]),
+    "spdnn_mx4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, _OP, C.c_void_p, C.c_char_p, C.c_int]),
     "spdnn_last_error": (C.c_char_p, [C.c_void_p]),
     "spdnn_destroy": (None, [C.c_void_p]),
     "spdnn_version": (C.c_char_p, []),

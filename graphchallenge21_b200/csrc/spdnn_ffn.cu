@@ -1,0 +1,594 @@
+// C ABI of the feed-forward operators: topologies, sparse layers on row-major activations (plain and gated, forward and
+// backward) and microscaled 4-bit matrices.  Kernels: spdnn_ffn.cuh, spdnn_mx4.cuh; host analysis: topology.h.
+//
+// A topology is immutable once created, and every call works on buffers of its caller (operands and workspace) on the caller's
+// stream, so calls on one topology may overlap, from several threads too.
+#include "../../include/spdnn_b200.h"
+
+#include <cstdio>
+#include <new>
+#include <string>
+#include <tuple>
+
+#include "spdnn_ffn.cuh"
+#include "spdnn_mx4.cuh"
+#include "topology.h"
+
+using namespace spdnn_impl;
+using namespace spdnn_impl::ffn;
+
+static_assert((int)SPDNN_F32 == F32 && (int)SPDNN_F16 == F16 && (int)SPDNN_BF16 == BF16 && (int)SPDNN_MX4 == MX4, "types of the header");
+static_assert((int)SPDNN_ACT_NONE == NONE && (int)SPDNN_ACT_RELU == RELU && (int)SPDNN_ACT_CLIP == CLIP && (int)SPDNN_ACT_SILU == SILU &&
+                  (int)SPDNN_ACT_GELU == GELU && (int)SPDNN_ACT_GELU_TANH == GELU_TANH, "activations of the header");
+
+namespace {
+
+struct DeviceTable {
+    uint32_t *slice_ptr = nullptr, *idx = nullptr, *src = nullptr;
+    uint16_t *idx16 = nullptr;      // where every row fits: what the kernels read from an image in shared memory
+    int64_t entries = 0;
+    int outs = 0, rows = 0;
+};
+
+}  // namespace
+
+struct spdnn_topology {
+    Topology host;
+    int device = -1;                // -1: analysis only
+    int sm_count = 0;
+    DeviceTable forward, backward;
+    int32_t *rows = nullptr;
+};
+
+namespace {
+
+int fail(char *err, int err_len, int code, const char *msg) {
+    if (err && err_len > 0) snprintf(err, (size_t)err_len, "%s", msg);
+    return code;
+}
+int fail(char *err, int err_len, int code, const std::string &msg) { return fail(err, err_len, code, msg.c_str()); }
+
+// A failed runtime call: its message, and nothing left for the next caller of cudaGetLastError to find.
+int fail_cuda(char *err, int err_len, cudaError_t e) {
+    cudaGetLastError();
+    return fail(err, err_len, e == cudaErrorMemoryAllocation ? SPDNN_ERR_MEMORY : SPDNN_ERR_CUDA, cudaGetErrorString(e));
+}
+
+// A launch whose status is its own (cudaGetLastError would also return what an earlier call of someone else left behind).
+template <class... P, class... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, const A &...args) {
+    std::tuple<P...> values(args...);
+    return std::apply([&](P &...v) {
+        void *ptrs[] = {(void *)&v...};
+        return cudaLaunchKernel((const void *)kernel, dim3(grid), dim3(block), ptrs, 0, stream);
+    }, values);
+}
+
+// The device of the topology for the length of a call.
+struct OnDevice {
+    int before = -1;
+    cudaError_t status;
+    explicit OnDevice(int device) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
+        if (before == device) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+template <class T>
+cudaError_t upload(T **to, const std::vector<T> &from) {
+    cudaError_t e = cudaMalloc((void **)to, std::max<size_t>(from.size(), 1) * sizeof(T));
+    if (e != cudaSuccess) return e;
+    return cudaMemcpy(*to, from.data(), from.size() * sizeof(T), cudaMemcpyHostToDevice);
+}
+
+cudaError_t upload(DeviceTable &d, const GatherTable &t) {
+    d.outs = t.outs; d.rows = t.rows; d.entries = (int64_t)t.idx.size();
+    cudaError_t e = upload(&d.slice_ptr, t.slice_ptr);
+    if (e == cudaSuccess) e = upload(&d.idx, t.idx);
+    if (e == cudaSuccess) e = upload(&d.src, t.src);
+    if (e == cudaSuccess && t.rows < 65536) e = upload(&d.idx16, std::vector<uint16_t>(t.idx.begin(), t.idx.end()));
+    return e;
+}
+
+void release(DeviceTable &d) {
+    cudaFree(d.slice_ptr); cudaFree(d.idx); cudaFree(d.src); cudaFree(d.idx16);
+    d = DeviceTable();
+}
+
+int type_size(int type) { return type == F32 ? 4 : 2; }
+bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
+int64_t aligned(int64_t n) { return (n + 255) & ~255ll; }
+
+// How a gather runs: the image's unit (v tokens) and units per neuron (p), and how many blocks share a tile.
+struct GatherPlan {
+    int v = 1, p = 1, splits = 1;
+    int64_t tiles = 0, image_bytes = 0;
+    bool global = false;
+};
+
+constexpr int64_t kSharedLimit = 227 * 1024;
+
+int64_t image_size(int rows, int sets, int v, int p, int size) {
+    return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
+}
+
+GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int tokens, int sets, int size) {
+    GatherPlan g;
+    const int full = 16 / size;
+    bool found = false;
+    for (int T = full * 8; T >= 1 && !found; T /= 2) {
+        const int v = T < full ? T : full, p = T / v;
+        if (T > 1 && T / 2 >= tokens) continue;
+        const int64_t bytes = image_size(t.rows, sets, v, p, size);
+        if (!t.idx16 || bytes > kSharedLimit) continue;
+        g.v = v; g.p = p; g.image_bytes = bytes;
+        found = true;
+    }
+    if (!found) {
+        g.global = true;
+        g.v = full; g.p = tokens > full ? 8 : 1;
+        g.image_bytes = image_size(t.rows, sets, g.v, g.p, size);
+    }
+    const int T = g.v * g.p;
+    g.tiles = (tokens + T - 1) / T;
+    const int64_t per_sm = g.global ? 4 : std::max<int64_t>(1, std::min<int64_t>(4, kSharedLimit / (g.image_bytes + 1024)));
+    const int64_t want = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * g.p;
+    g.splits = (int)std::max<int64_t>(1, std::min<int64_t>((want + g.tiles - 1) / g.tiles, (units + 15) / 16));
+    return g;
+}
+
+template <class E, class W, int S, int G>
+const void *gather_variant(const GatherPlan &g) {
+    constexpr int F = 16 / (int)sizeof(E);
+    if (g.global) return g.p == 8 ? (const void *)gather_kernel<E, W, F, 8, S, G, true> : (const void *)gather_kernel<E, W, F, 1, S, G, true>;
+    if (g.v == F) {
+        switch (g.p) {
+            case 8: return (const void *)gather_kernel<E, W, F, 8, S, G, false>;
+            case 4: return (const void *)gather_kernel<E, W, F, 4, S, G, false>;
+            case 2: return (const void *)gather_kernel<E, W, F, 2, S, G, false>;
+            default: return (const void *)gather_kernel<E, W, F, 1, S, G, false>;
+        }
+    }
+    if constexpr (F == 8) {
+        if (g.v == 4) return (const void *)gather_kernel<E, W, 4, 1, S, G, false>;
+    }
+    return g.v == 2 ? (const void *)gather_kernel<E, W, 2, 1, S, G, false> : (const void *)gather_kernel<E, W, 1, 1, S, G, false>;
+}
+
+template <class E, class W>
+const void *gather_variant(const GatherPlan &g, int s, int sets) {
+    if (s == 2) return gather_variant<E, W, 2, 1>(g);
+    return sets == 2 ? gather_variant<E, W, 1, 2>(g) : gather_variant<E, W, 1, 1>(g);
+}
+
+// image_type: E; weight_type: W.  s: values gathered per connection, sets: sums per neuron.
+cudaError_t launch_gather(const GatherPlan &g, GatherArgs a, int image_type, int weight_type, int s, int sets, cudaStream_t stream) {
+    const void *kernel = image_type == F32 ? gather_variant<float, float>(g, s, sets)
+                         : image_type == BF16 ? gather_variant<bf16, bf16>(g, s, sets)
+                         : weight_type == F16 ? gather_variant<__half, __half>(g, s, sets)
+                                              : gather_variant<__half, bf16>(g, s, sets);
+    a.splits = g.splits;
+    a.image_bytes = g.image_bytes;
+    const size_t shared = g.global ? 0 : (size_t)g.image_bytes;
+    if (shared > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (e != cudaSuccess) return e;
+    }
+    void *args[] = {&a};
+    return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(kGatherThreads), args, shared, stream);
+}
+
+cudaError_t launch_pack(const PackArgs &a, int image_type, int sets, bool gradient, cudaStream_t stream) {
+    const int64_t blocks = (int64_t)((a.rows + 63) / 64) * ((a.tokens + 63) / 64);
+    const unsigned grid = (unsigned)blocks;
+    const auto run = [&](auto e) {
+        using E = decltype(e);
+        if (!gradient) return launch(pack_kernel<E, 1, false>, grid, kPackThreads, stream, a);
+        return sets == 1 ? launch(pack_kernel<E, 1, true>, grid, kPackThreads, stream, a) : launch(pack_kernel<E, 2, true>, grid, kPackThreads, stream, a);
+    };
+    return image_type == F32 ? run(float()) : image_type == F16 ? run(__half()) : run(bf16());
+}
+
+cudaError_t launch_order(const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int sets, int weight_type, void *out,
+                         cudaStream_t stream) {
+    if (!t.entries) return cudaSuccess;
+    const unsigned grid = (unsigned)((t.entries + 255) / 256);
+    const auto run = [&](auto w) {
+        using W = decltype(w);
+        return sets == 2 ? launch(order_weights_kernel<W, 2>, grid, 256, stream, w0, w1, t.src, slots, t.entries, (W *)out)
+                         : launch(order_weights_kernel<W, 1>, grid, 256, stream, w0, w1, t.src, slots, t.entries, (W *)out);
+    };
+    return weight_type == F32 ? run(float()) : weight_type == F16 ? run(__half()) : run(bf16());
+}
+
+// The type activations have in an image, and weights in a gather table's order.  Microscaled values are exact in bf16 (two bits of
+// magnitude, the exponents of float32), not in fp16.
+int image_type(int x_type) { return x_type == MX4 ? BF16 : x_type; }
+int ordered_type(int x_type, int w_type) { return x_type == F32 ? F32 : w_type == MX4 ? BF16 : w_type; }
+
+const char *check_types(int x_type, int w_type, bool backward) {
+    if (!is_float(x_type) && x_type != MX4) return "unknown type of the activations";
+    if (!is_float(w_type) && w_type != MX4) return "unknown type of the weights";
+    if (backward && (x_type == MX4 || w_type == MX4)) return "microscaled operands have no backward pass";
+    if (w_type != MX4 && w_type != (x_type == MX4 ? BF16 : x_type))
+        return "the weights must be microscaled or have the activations' type (bf16 for microscaled activations)";
+    return nullptr;
+}
+
+struct Workspace {
+    int64_t weights = 0, image = 0, x_columns = 0, d_columns = 0, total = 0;
+};
+
+// Layout of a call's workspace.  The plan is a function of the topology, the device and the arguments.
+Workspace layout(const spdnn_topology &top, const GatherPlan &g, const DeviceTable &t, int tokens, int sets, int image, int weight, bool backward) {
+    Workspace w;
+    int64_t at = 0;
+    w.weights = at; at += aligned(t.entries * sets * type_size(weight));
+    w.image = at; at += aligned(g.tiles * g.image_bytes);
+    if (backward) {
+        const int64_t stride = (tokens + 63) / 64 * 64;
+        w.x_columns = at; at += aligned(stride * top.host.inputs * type_size(image));
+        w.d_columns = at; at += aligned(stride * top.host.outputs * sets * 4);
+    }
+    w.total = std::max<int64_t>(at, 256);
+    return w;
+}
+
+struct Call {            // what linear and gated share
+    const spdnn_topology *top;
+    int tokens, sets, act;
+    float clip;
+    const spdnn_operand_t *x, *w[2], *y, *z[2];
+    void *workspace;
+    int64_t workspace_bytes;
+    cudaStream_t stream;
+    char *err;
+    int err_len;
+};
+
+Matrix matrix(const spdnn_operand_t *o) {
+    Matrix m{nullptr, nullptr, 0, F32};
+    if (o) { m.data = o->data; m.scales = o->scales; m.stride = o->stride; m.type = o->type; }
+    return m;
+}
+
+// nullptr, or what is wrong with an operand of `rows` x `cols` values
+const char *check_operand(const spdnn_operand_t *o, int64_t rows, int64_t cols, bool may_be_mx4) {
+    if (!o) return "a required operand is null";
+    if (!is_float(o->type) && !(may_be_mx4 && o->type == MX4)) return "an operand has a type that it cannot have";
+    if (rows == 0) return nullptr;
+    if (!o->data) return "an operand has no data";
+    if (o->type == MX4 && !o->scales) return "a microscaled operand has no scales";
+    const int64_t least = o->type == MX4 ? (cols + 31) / 32 : cols;
+    if (o->stride < least) return "an operand's stride is less than its row";
+    if (o->stride > (1ll << 40)) return "an operand's stride is out of range";
+    if (o->type != MX4 && reinterpret_cast<uintptr_t>(o->data) % type_size(o->type)) return "an operand is not aligned to its type";
+    return nullptr;
+}
+
+int check_call(const Call &c, bool backward) {
+    if (!c.top) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "null topology");
+    if (c.tokens < 0 || c.tokens > SPDNN_MAX_TOKENS) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "tokens must be in [0, 2^26]");
+    if (c.act < SPDNN_ACT_NONE || c.act > SPDNN_ACT_GELU_TANH) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "unknown activation");
+    if (c.act == SPDNN_ACT_CLIP && !(c.clip > 0.0f)) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "clip must be positive");
+    const Topology &h = c.top->host;
+    const char *bad = check_operand(c.x, c.tokens, h.inputs, !backward);
+    for (int s = 0; s < c.sets && !bad; ++s) bad = check_operand(c.w[s], h.outputs, h.slots, !backward);
+    if (!bad && c.sets == 2 && c.w[0]->type != c.w[1]->type) bad = "both sets of weights must have one type";
+    if (!bad) bad = check_types(c.x->type, c.w[0]->type, backward);
+    if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
+    return SPDNN_OK;
+}
+
+int check_run(const Call &c, int64_t need) {
+    if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, "the topology was created for analysis only (device -1)");
+    if (!c.workspace || c.workspace_bytes < need)
+        return fail(c.err, c.err_len, SPDNN_ERR_ARG, "the workspace is smaller than spdnn_layer_workspace asks for: " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(c.workspace) % 256) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "the workspace must be aligned to 256 bytes");
+    return SPDNN_OK;
+}
+
+int check_blocks(const Call &c, const GatherPlan &g) {
+    const int64_t pack = (int64_t)((std::max(c.top->host.inputs, c.top->host.outputs) + 63) / 64) * ((c.tokens + 63) / 64);
+    if (pack > 0x7fffffffll || g.tiles * g.splits > 0x7fffffffll)
+        return fail(c.err, c.err_len, SPDNN_ERR_LIMIT, "tokens times neurons is too large for one call: split the tokens");
+    return SPDNN_OK;
+}
+
+int run_forward(const Call &c, const float *b0, const float *b1) {
+    int rc = check_call(c, false);
+    if (rc) return rc;
+    const Topology &h = c.top->host;
+    const char *bad = check_operand(c.y, c.tokens, h.outputs, false);
+    for (int s = 0; s < c.sets && !bad; ++s)
+        if (c.z[s]) {
+            bad = check_operand(c.z[s], c.tokens, h.outputs, false);
+            if (!bad && c.z[s]->type != F32) bad = "pre-activations are saved as fp32";
+        }
+    if (!bad && c.sets == 2 && !c.z[0] != !c.z[1]) bad = "save both pre-activations or none";
+    if (!bad && c.sets == 2 && c.z[0] && c.z[0]->stride != c.z[1]->stride) bad = "both pre-activations must have one stride";
+    if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
+    if (c.tokens == 0 && c.top->device >= 0) return SPDNN_OK;
+    const DeviceTable &t = c.top->forward;
+    const int it = image_type(c.x->type), wt = ordered_type(c.x->type, c.w[0]->type);
+    const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), 1, type_size(it));
+    const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, it, wt, false);
+    if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
+    OnDevice guard(c.top->device);
+    if (guard.status != cudaSuccess) return fail_cuda(c.err, c.err_len, guard.status);
+    char *base = (char *)c.workspace;
+    cudaError_t e = launch_order(matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, wt, base + ws.weights, c.stream);
+    if (e == cudaSuccess) {
+        PackArgs p{};
+        p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
+        p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p;
+        e = launch_pack(p, it, 1, false, c.stream);
+    }
+    if (e == cudaSuccess) {
+        GatherArgs a{};
+        a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.idx = g.global ? (const void *)t.idx : t.idx16;
+        a.weights = base + ws.weights; a.outs = t.outs; a.rows = t.rows; a.tokens = c.tokens;
+        a.bias0 = b0; a.bias1 = b1; a.act = c.act; a.clip = c.clip;
+        a.y = const_cast<void *>(c.y->data); a.y_stride = c.y->stride; a.y_type = c.y->type;
+        if (c.z[0]) { a.z0 = (float *)const_cast<void *>(c.z[0]->data); a.z_stride = c.z[0]->stride; }
+        if (c.z[1]) a.z1 = (float *)const_cast<void *>(c.z[1]->data);
+        e = launch_gather(g, a, it, wt, 1, c.sets, c.stream);
+    }
+    if (e != cudaSuccess) return fail_cuda(c.err, c.err_len, e);
+    return SPDNN_OK;
+}
+
+struct Gradients {
+    const spdnn_operand_t *dy, *dx;
+    float *dw[2], *db[2];
+};
+
+int run_backward(const Call &c, const Gradients &d) {
+    int rc = check_call(c, true);
+    if (rc) return rc;
+    const Topology &h = c.top->host;
+    const int type = c.x->type;
+    const char *bad = check_operand(d.dy, c.tokens, h.outputs, false);
+    if (!bad && d.dy->type != type) bad = "dy must have the activations' type";
+    for (int s = 0; s < c.sets && !bad; ++s) {
+        if (c.sets == 1 && c.act == NONE) break;      // the slope is 1 everywhere: nothing saved is read
+        bad = check_operand(c.z[s], c.tokens, h.outputs, false);
+        if (!bad && c.z[s]->type != F32) bad = "pre-activations are saved as fp32";
+    }
+    if (!bad && c.sets == 2 && c.z[0]->stride != c.z[1]->stride) bad = "both pre-activations must have one stride";
+    if (!bad && d.dx) {
+        bad = check_operand(d.dx, c.tokens, h.inputs, false);
+        if (!bad && d.dx->type != type) bad = "dx must have the activations' type";
+    }
+    if (!bad && c.sets == 2 && !d.dw[0] != !d.dw[1]) bad = "ask for the gradients of both sets of weights or of none";
+    if (!bad && !d.dw[0] && (d.db[0] || d.db[1])) bad = "the gradients of the biases come with those of the weights";
+    if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
+    const DeviceTable &t = c.top->backward;
+    const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), c.sets, type_size(type));
+    const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, type, type, true);
+    if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
+    OnDevice guard(c.top->device);
+    cudaError_t e = guard.status;
+    char *base = (char *)c.workspace;
+    const int64_t stride = ((int64_t)c.tokens + 63) / 64 * 64;
+    if (c.tokens > 0 && e == cudaSuccess) {
+        PackArgs p{};
+        p.x = matrix(d.dy);
+        if (c.z[0]) { p.z0 = (const float *)c.z[0]->data; p.z_stride = c.z[0]->stride; }
+        if (c.z[1]) p.z1 = (const float *)c.z[1]->data;
+        p.rows = h.outputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.act = c.act; p.clip = c.clip;
+        p.image = d.dx ? base + ws.image : nullptr; p.image_bytes = g.image_bytes;
+        p.columns = d.dw[0] ? base + ws.d_columns : nullptr; p.token_stride = stride;
+        e = launch_pack(p, type, c.sets, true, c.stream);
+    }
+    if (c.tokens > 0 && d.dx && e == cudaSuccess) {
+        e = launch_order(matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, type, base + ws.weights, c.stream);
+        if (e == cudaSuccess) {
+            GatherArgs a{};
+            a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.idx = g.global ? (const void *)t.idx : t.idx16;
+            a.weights = base + ws.weights; a.outs = t.outs; a.rows = t.rows; a.tokens = c.tokens;
+            a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
+            e = launch_gather(g, a, type, type, c.sets, 1, c.stream);
+        }
+    }
+    if (d.dw[0] && e == cudaSuccess) {
+        if (c.tokens > 0) {
+            PackArgs p{};
+            p.x = matrix(c.x); p.rows = h.inputs; p.tokens = c.tokens; p.v = p.p = 1;
+            p.columns = base + ws.x_columns; p.token_stride = stride;
+            e = launch_pack(p, type, 1, false, c.stream);
+        }
+        if (e == cudaSuccess) {
+            DwArgs a{};
+            a.x = base + ws.x_columns; a.d = (const float *)(base + ws.d_columns); a.rows = c.top->rows; a.token_stride = stride;
+            a.outputs = h.outputs; a.slots = h.slots; a.chunks = (h.slots + kDwSlots - 1) / kDwSlots;
+            a.dw0 = d.dw[0]; a.dw1 = d.dw[1]; a.db0 = d.db[0]; a.db1 = d.db[1];
+            const int per_block = kDwThreads / 32;
+            const unsigned grid = (unsigned)(((int64_t)a.outputs * a.chunks + per_block - 1) / per_block);
+            const auto run = [&](auto v) {
+                using E = decltype(v);
+                return c.sets == 2 ? launch(dw_kernel<E, 2>, grid, kDwThreads, c.stream, a) : launch(dw_kernel<E, 1>, grid, kDwThreads, c.stream, a);
+            };
+            e = type == F32 ? run(float()) : type == F16 ? run(__half()) : run(bf16());
+        }
+    }
+    if (e != cudaSuccess) return fail_cuda(c.err, c.err_len, e);
+    return SPDNN_OK;
+}
+
+}  // namespace
+
+// ---- topologies ------------------------------------------------------------------------------------
+
+extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inputs, int outputs, const int32_t *col_ptr,
+                                     const int32_t *row_idx, char *err, int err_len) {
+    if (!out) return fail(err, err_len, SPDNN_ERR_ARG, "null handle pointer");
+    *out = nullptr;
+    spdnn_topology *t = nullptr;
+    try {
+        t = new spdnn_topology();
+        const std::string why = build_topology(inputs, outputs, col_ptr, row_idx, t->host);
+        if (!why.empty()) {
+            delete t;
+            return fail(err, err_len, SPDNN_ERR_ARG, why);
+        }
+        if (device < 0) {
+            *out = t;
+            return SPDNN_OK;
+        }
+        OnDevice guard(device);
+        cudaError_t e = guard.status;
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&t->sm_count, cudaDevAttrMultiProcessorCount, device);
+        if (e == cudaSuccess) e = upload(t->forward, t->host.forward);
+        if (e == cudaSuccess) e = upload(t->backward, t->host.backward);
+        if (e == cudaSuccess) e = upload(&t->rows, t->host.rows);
+        t->device = device;
+        if (e != cudaSuccess) {
+            spdnn_topology_destroy(t);
+            return fail_cuda(err, err_len, e);
+        }
+        // the tables are on the device: only the canonical rows are asked for again
+        t->host.forward = GatherTable();
+        t->host.backward = GatherTable();
+        *out = t;
+        return SPDNN_OK;
+    } catch (const std::bad_alloc &) {
+        spdnn_topology_destroy(t);
+        return fail(err, err_len, SPDNN_ERR_MEMORY, "host allocation failed");
+    } catch (...) {
+        spdnn_topology_destroy(t);
+        return fail(err, err_len, SPDNN_ERR_MEMORY, "topology analysis failed");
+    }
+}
+
+extern "C" void spdnn_topology_destroy(spdnn_topology_t *top) {
+    if (!top) return;
+    if (top->device >= 0) {
+        OnDevice guard(top->device);
+        release(top->forward);
+        release(top->backward);
+        cudaFree(top->rows);
+    }
+    delete top;
+}
+
+extern "C" int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int *outputs, int *slots, int *fan_out, int64_t *connections) {
+    if (!top) return SPDNN_ERR_ARG;
+    if (inputs) *inputs = top->host.inputs;
+    if (outputs) *outputs = top->host.outputs;
+    if (slots) *slots = top->host.slots;
+    if (fan_out) *fan_out = top->host.fan_out;
+    if (connections) *connections = top->host.connections;
+    return SPDNN_OK;
+}
+
+extern "C" int spdnn_topology_rows(const spdnn_topology_t *top, int32_t *rows, int64_t capacity) {
+    if (!top || !rows || capacity < (int64_t)top->host.rows.size()) return SPDNN_ERR_ARG;
+    std::copy(top->host.rows.begin(), top->host.rows.end(), rows);
+    return SPDNN_OK;
+}
+
+// ---- layers ------------------------------------------------------------------------------------------
+
+extern "C" int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, int sets, int x_type, int w_type, int backward, int64_t *bytes) {
+    if (!top || !bytes || tokens < 0 || tokens > SPDNN_MAX_TOKENS || (sets != 1 && sets != 2)) return SPDNN_ERR_ARG;
+    if (check_types(x_type, w_type, backward != 0)) return SPDNN_ERR_ARG;
+    if (top->device < 0) return SPDNN_ERR_STATE;
+    const int it = image_type(x_type), wt = ordered_type(x_type, w_type);
+    const DeviceTable &t = backward ? top->backward : top->forward;
+    const GatherPlan g = plan_gather(*top, t, std::max(tokens, 1), backward ? sets : 1, type_size(it));
+    *bytes = layout(*top, g, t, tokens, sets, it, wt, backward != 0).total;
+    return SPDNN_OK;
+}
+
+extern "C" int spdnn_linear(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w, const float *bias,
+                            int activation, float clip, const spdnn_operand_t *y, const spdnn_operand_t *z, void *workspace,
+                            int64_t workspace_bytes, void *cuda_stream, char *err, int err_len) {
+    const Call c{top, tokens, 1, activation, clip, x, {w, nullptr}, y, {z, nullptr}, workspace, workspace_bytes,
+                 static_cast<cudaStream_t>(cuda_stream), err, err_len};
+    return run_forward(c, bias, nullptr);
+}
+
+extern "C" int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w_gate,
+                           const spdnn_operand_t *w_up, const float *bias_gate, const float *bias_up, int activation, float clip,
+                           const spdnn_operand_t *y, const spdnn_operand_t *z_gate, const spdnn_operand_t *z_up, void *workspace,
+                           int64_t workspace_bytes, void *cuda_stream, char *err, int err_len) {
+    const Call c{top, tokens, 2, activation, clip, x, {w_gate, w_up}, y, {z_gate, z_up}, workspace, workspace_bytes,
+                 static_cast<cudaStream_t>(cuda_stream), err, err_len};
+    return run_forward(c, bias_gate, bias_up);
+}
+
+extern "C" int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
+                                     const spdnn_operand_t *w, const spdnn_operand_t *z, int activation, float clip, const spdnn_operand_t *dx,
+                                     float *dw, float *dbias, void *workspace, int64_t workspace_bytes, void *cuda_stream, char *err,
+                                     int err_len) {
+    const Call c{top, tokens, 1, activation, clip, x, {w, nullptr}, nullptr, {z, nullptr}, workspace, workspace_bytes,
+                 static_cast<cudaStream_t>(cuda_stream), err, err_len};
+    return run_backward(c, Gradients{dy, dx, {dw, nullptr}, {dbias, nullptr}});
+}
+
+extern "C" int spdnn_gated_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
+                                    const spdnn_operand_t *w_gate, const spdnn_operand_t *w_up, const spdnn_operand_t *z_gate,
+                                    const spdnn_operand_t *z_up, int activation, float clip, const spdnn_operand_t *dx, float *dw_gate,
+                                    float *dw_up, float *dbias_gate, float *dbias_up, void *workspace, int64_t workspace_bytes,
+                                    void *cuda_stream, char *err, int err_len) {
+    const Call c{top, tokens, 2, activation, clip, x, {w_gate, w_up}, nullptr, {z_gate, z_up}, workspace, workspace_bytes,
+                 static_cast<cudaStream_t>(cuda_stream), err, err_len};
+    return run_backward(c, Gradients{dy, dx, {dw_gate, dw_up}, {dbias_gate, dbias_up}});
+}
+
+// ---- microscaled matrices ------------------------------------------------------------------------------
+
+namespace {
+
+const char *check_mx4(const void *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *m) {
+    if (rows < 0 || cols <= 0 || cols > (1 << 30) || rows > (1ll << 40) / cols) return "a microscaled matrix has rows >= 0, cols in [1, 2^30], fewer than 2^40 values";
+    if (rows && (!codes || !scales)) return "null device pointer";
+    if (reinterpret_cast<uintptr_t>(codes) % 4) return "codes must be aligned to 4 bytes";
+    return check_operand(m, rows, cols, false);
+}
+
+unsigned mx4_grid(int64_t groups) { return (unsigned)std::min<int64_t>((groups + kMx4Threads - 1) / kMx4Threads, 1 << 20); }
+
+template <class E>
+cudaError_t quantize(const spdnn_operand_t *x, int64_t rows, int cols, uint8_t *codes, uint8_t *scales, cudaStream_t stream) {
+    const int blocks = (cols + 31) / 32;
+    const bool vector = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->stride * (int64_t)sizeof(E) % 16 == 0;
+    return launch(vector ? mx4_quantize_kernel<E, true> : mx4_quantize_kernel<E, false>, mx4_grid(rows * blocks * 4), kMx4Threads, stream,
+                  (const E *)x->data, x->stride, rows, cols, blocks, (uint32_t *)codes, scales);
+}
+
+template <class E>
+cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *y, cudaStream_t stream) {
+    const int blocks = (cols + 31) / 32;
+    return launch(mx4_dequantize_kernel<E>, mx4_grid(rows * blocks * 4), kMx4Threads, stream, (const uint32_t *)codes, scales, rows, cols, blocks,
+                  (E *)const_cast<void *>(y->data), y->stride);
+}
+
+}  // namespace
+
+extern "C" int spdnn_mx4_quantize(const spdnn_operand_t *x, int64_t rows, int cols, uint8_t *codes, uint8_t *scales, void *cuda_stream,
+                                  char *err, int err_len) {
+    const char *bad = check_mx4(codes, scales, rows, cols, x);
+    if (bad) return fail(err, err_len, SPDNN_ERR_ARG, bad);
+    if (!rows) return SPDNN_OK;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const cudaError_t e = x->type == F32   ? quantize<float>(x, rows, cols, codes, scales, stream)
+                          : x->type == F16 ? quantize<__half>(x, rows, cols, codes, scales, stream)
+                                         : quantize<bf16>(x, rows, cols, codes, scales, stream);
+    return e == cudaSuccess ? SPDNN_OK : fail_cuda(err, err_len, e);
+}
+
+extern "C" int spdnn_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *y,
+                                    void *cuda_stream, char *err, int err_len) {
+    const char *bad = check_mx4(codes, scales, rows, cols, y);
+    if (bad) return fail(err, err_len, SPDNN_ERR_ARG, bad);
+    if (!rows) return SPDNN_OK;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const cudaError_t e = y->type == F32   ? dequantize<float>(codes, scales, rows, cols, y, stream)
+                          : y->type == F16 ? dequantize<__half>(codes, scales, rows, cols, y, stream)
+                                         : dequantize<bf16>(codes, scales, rows, cols, y, stream);
+    return e == cudaSuccess ? SPDNN_OK : fail_cuda(err, err_len, e);
+}

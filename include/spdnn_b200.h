@@ -210,6 +210,97 @@ int spdnn_layer_static(const float *yin, float *yout, int neurons, int live_in, 
                        const int32_t *off, const float *vals, int k, float w, float bias, float clip,
                        int32_t *survivors, int32_t *survivor_count, void *cuda_stream, char *err, int err_len);
 
+/* ---- Feed-forward operators -------------------------------------------------------------------
+ *
+ * Sparse layers on row-major activations [tokens][neurons] in device memory of the caller, with trained weights: the plain
+ * layer y = act(x W + b) and the gated block y = act(x Wg + bg) * (x Wu + bu), forward and backward, in fp32, fp16 or
+ * bf16; and microscaled 4-bit matrices, which weights and activations of the forward calls may be.  They have no counterpart
+ * in the reference, whose layers carry one constant weight (src/inspector/matrix_block_container.h:218); like
+ * spdnn_layer_static they work on buffers the caller owns, enqueue on the caller's stream (a cudaStream_t as void*, NULL =
+ * default stream), allocate nothing, may be captured into a graph, and put the message of a failure into the optional host
+ * buffer err (err_len bytes).
+ *
+ * A TOPOLOGY says which inputs every output neuron is connected to; the weights are arguments of the calls.  It does not change
+ * once created: calls on one topology may overlap, on several streams and from several threads, each with a workspace of
+ * its own.  Destroy it when no call on it is in flight.
+ *
+ * A set of weights is a matrix [outputs][slots] in CANONICAL order: connection j of a neuron is its j-th smallest input
+ * (spdnn_topology_rows).  What a matrix holds where a neuron has no j-th connection is never read; gradients are zero there.
+ * Sums run in 32 bits, in no order that callers may rely on; results are rounded once. */
+typedef struct spdnn_topology spdnn_topology_t;
+
+enum { SPDNN_F32 = 0, SPDNN_F16 = 1, SPDNN_BF16 = 2, SPDNN_MX4 = 3 };
+
+/* NONE v, RELU max(v, 0), CLIP min(max(v, 0), clip), SILU v / (1 + e^-v), GELU v Phi(v), GELU_TANH its tanh approximation */
+enum {
+    SPDNN_ACT_NONE = 0, SPDNN_ACT_RELU = 1, SPDNN_ACT_CLIP = 2, SPDNN_ACT_SILU = 3, SPDNN_ACT_GELU = 4, SPDNN_ACT_GELU_TANH = 5
+};
+
+#define SPDNN_MAX_TOKENS (1 << 26)   /* of one call */
+
+/* A matrix in device memory.  F32, F16, BF16: row i begins at data + i * stride elements; any stride not less than a row, any
+ * alignment of the type.  MX4: data = codes [rows][stride][16], scales [rows][stride] (stride in blocks of 32 columns). */
+typedef struct spdnn_operand {
+    const void *data;         /* written where the call says so */
+    const uint8_t *scales;    /* MX4 only */
+    int64_t stride;
+    int32_t type;             /* SPDNN_F32 ... */
+    int32_t reserved;
+} spdnn_operand_t;
+
+/* Topology as CSC: output c is connected to inputs row_idx[col_ptr[c] .. col_ptr[c+1]), in any order (at most 4096; repeated
+ * entries stay separate connections).  Host arrays, borrowed for the call.  device -1: analysis only, for
+ * spdnn_topology_info and _rows, without a GPU.  Call it outside stream captures (it allocates). */
+int spdnn_topology_create(spdnn_topology_t **top, int device, int inputs, int outputs, const int32_t *col_ptr,
+                          const int32_t *row_idx, char *err, int err_len);
+void spdnn_topology_destroy(spdnn_topology_t *top);
+
+/* slots: connections of the output that has most, at least 1; fan_out: most outputs that one input feeds.  Pointers may be NULL. */
+int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int *outputs, int *slots, int *fan_out, int64_t *connections);
+
+/* The canonical order, to host memory: rows[outputs][slots] = inputs of every output ascending, -1 behind the last one. */
+int spdnn_topology_rows(const spdnn_topology_t *top, int32_t *rows, int64_t capacity);
+
+/* Bytes of device workspace (aligned to 256) that a call needs: sets 1 = spdnn_linear, 2 = spdnn_gated, or their backward calls.
+ * Its contents need not be kept between calls; calls that may overlap need one each. */
+int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, int sets, int x_type, int w_type, int backward, int64_t *bytes);
+
+/* y[tokens][outputs] = act(x W + bias).  x [tokens][inputs] and w [outputs][slots]: one float type, or w MX4 with any x, or x
+ * MX4 with w MX4 or BF16.  bias: fp32 [outputs] or NULL.  y: any float type, written.  z: x W + bias for the backward call, written in
+ * fp32, or NULL.  Outputs must not overlap inputs. */
+int spdnn_linear(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w, const float *bias,
+                 int activation, float clip, const spdnn_operand_t *y, const spdnn_operand_t *z, void *workspace,
+                 int64_t workspace_bytes, void *cuda_stream, char *err, int err_len);
+
+/* y = act(x w_gate + bias_gate) * (x w_up + bias_up), both projections over one topology in one pass; both z of one stride, or none. */
+int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w_gate,
+                const spdnn_operand_t *w_up, const float *bias_gate, const float *bias_up, int activation, float clip,
+                const spdnn_operand_t *y, const spdnn_operand_t *z_gate, const spdnn_operand_t *z_up, void *workspace,
+                int64_t workspace_bytes, void *cuda_stream, char *err, int err_len);
+
+/* Gradients from dy = dL/dy and what the forward call read and saved; dy, x, w and dx have one float type.  dx
+ * [tokens][inputs] or NULL; dw, dbias in fp32 ([outputs][slots] without gaps, [outputs]), overwritten, or NULL (dbias only with dw).
+ * z may be NULL for SPDNN_ACT_NONE (linear).  The slope of RELU at 0 is 0, of CLIP at 0 and clip too.  On its way to
+ * dx (not to dw and dbias) dL/dz is rounded to the operands' type.  Every sum has a fixed order: the same call gives the same bits. */
+int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
+                          const spdnn_operand_t *w, const spdnn_operand_t *z, int activation, float clip, const spdnn_operand_t *dx,
+                          float *dw, float *dbias, void *workspace, int64_t workspace_bytes, void *cuda_stream, char *err,
+                          int err_len);
+int spdnn_gated_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
+                         const spdnn_operand_t *w_gate, const spdnn_operand_t *w_up, const spdnn_operand_t *z_gate,
+                         const spdnn_operand_t *z_up, int activation, float clip, const spdnn_operand_t *dx, float *dw_gate,
+                         float *dw_up, float *dbias_gate, float *dbias_up, void *workspace, int64_t workspace_bytes,
+                         void *cuda_stream, char *err, int err_len);
+
+/* Microscaled 4-bit floats: rows in blocks of 32 columns, a block one power of two (E8M0) and 32 values of E2M1 (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 and their negatives).  Scale 2^(floor(log2 max) - 2), from 2^-127 on; values rounded half to even, above 6 to
+ * 6.  A block with a NaN or an infinity becomes NaN.  codes [rows][ceil(cols/32)][16] (even element in the low half of a byte;
+ * zeros behind the last column), scales [rows][ceil(cols/32)]; codes aligned to 4 bytes.  On the current device. */
+int spdnn_mx4_quantize(const spdnn_operand_t *x, int64_t rows, int cols, uint8_t *codes, uint8_t *scales, void *cuda_stream,
+                       char *err, int err_len);
+int spdnn_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *y,
+                         void *cuda_stream, char *err, int err_len);
+
 const char *spdnn_last_error(const spdnn_t *ctx);
 void spdnn_destroy(spdnn_t *ctx);
 
