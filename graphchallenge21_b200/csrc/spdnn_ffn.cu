@@ -25,7 +25,6 @@ namespace {
 
 struct DeviceTable {
     uint32_t *slice_ptr = nullptr, *idx = nullptr, *src = nullptr;
-    uint16_t *idx16 = nullptr;      // where every row fits: what the kernels read from an image in shared memory
     int64_t entries = 0;
     int outs = 0, rows = 0;
 };
@@ -88,12 +87,11 @@ cudaError_t upload(DeviceTable &d, const GatherTable &t) {
     cudaError_t e = upload(&d.slice_ptr, t.slice_ptr);
     if (e == cudaSuccess) e = upload(&d.idx, t.idx);
     if (e == cudaSuccess) e = upload(&d.src, t.src);
-    if (e == cudaSuccess && t.rows < 65536) e = upload(&d.idx16, std::vector<uint16_t>(t.idx.begin(), t.idx.end()));
     return e;
 }
 
 void release(DeviceTable &d) {
-    cudaFree(d.slice_ptr); cudaFree(d.idx); cudaFree(d.src); cudaFree(d.idx16);
+    cudaFree(d.slice_ptr); cudaFree(d.idx); cudaFree(d.src);
     d = DeviceTable();
 }
 
@@ -122,7 +120,7 @@ GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int toke
         const int v = T < full ? T : full, p = T / v;
         if (T > 1 && T / 2 >= tokens) continue;
         const int64_t bytes = image_size(t.rows, sets, v, p, size);
-        if (!t.idx16 || bytes > kSharedLimit) continue;
+        if (t.rows >= 65536 || bytes > kSharedLimit) continue;
         g.v = v; g.p = p; g.image_bytes = bytes;
         found = true;
     }
@@ -133,9 +131,17 @@ GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int toke
     }
     const int T = g.v * g.p;
     g.tiles = (tokens + T - 1) / T;
-    const int64_t per_sm = g.global ? 4 : std::max<int64_t>(1, std::min<int64_t>(4, kSharedLimit / (g.image_bytes + 1024)));
-    const int64_t want = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * g.p;
-    g.splits = (int)std::max<int64_t>(1, std::min<int64_t>((want + g.tiles - 1) / g.tiles, (units + 15) / 16));
+    const int64_t per_sm = g.global ? 2 : std::max<int64_t>(1, std::min<int64_t>(2, kSharedLimit / (g.image_bytes + 1024)));
+    const int64_t slots = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * g.p;
+    // Blocks of a tile: clocks of a wave of blocks are those of the image (about 40 bytes a clock) and of the block's units (a
+    // connection of 32 lanes about 8 clocks of the SM); the fewest in all waves.
+    const double per_unit = 8.0 * std::max<double>(1.0, (double)t.entries / 32.0 / std::max<int64_t>(1, (t.outs + 31) / 32)) / per_sm;
+    double best = 0.0;
+    for (int64_t s = 1; s <= 2 * slots && (s == 1 || s * 16 <= units); ++s) {
+        const int64_t waves = (g.tiles * s + slots - 1) / slots;
+        const double cost = waves * ((g.global ? 0.0 : g.image_bytes / 40.0) + 1000.0 + (double)((units + s - 1) / s) * per_unit);
+        if (s == 1 || cost < best) { best = cost; g.splits = (int)s; }
+    }
     return g;
 }
 
@@ -191,14 +197,18 @@ cudaError_t launch_pack(const PackArgs &a, int image_type, int sets, bool gradie
     return image_type == F32 ? run(float()) : image_type == F16 ? run(__half()) : run(bf16());
 }
 
-cudaError_t launch_order(const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int sets, int weight_type, void *out,
-                         cudaStream_t stream) {
+// weights, index: where the call's table goes
+cudaError_t launch_order(const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int values, int sets,
+                         int weight_type, int image_type, void *weights, void *index, cudaStream_t stream) {
     if (!t.entries) return cudaSuccess;
+    OrderArgs a{};
+    a.w0 = w0; a.w1 = w1; a.idx = t.idx; a.src = t.src; a.entries = t.entries; a.slots = slots; a.values = values; a.p = g.p;
+    a.swizzled = g.v * type_size(image_type) == 16; a.wide = g.global;
+    a.weights = weights; a.index = index;
     const unsigned grid = (unsigned)((t.entries + 255) / 256);
     const auto run = [&](auto w) {
         using W = decltype(w);
-        return sets == 2 ? launch(order_weights_kernel<W, 2>, grid, 256, stream, w0, w1, t.src, slots, t.entries, (W *)out)
-                         : launch(order_weights_kernel<W, 1>, grid, 256, stream, w0, w1, t.src, slots, t.entries, (W *)out);
+        return sets == 2 ? launch(order_kernel<W, 2>, grid, 256, stream, a) : launch(order_kernel<W, 1>, grid, 256, stream, a);
     };
     return weight_type == F32 ? run(float()) : weight_type == F16 ? run(__half()) : run(bf16());
 }
@@ -218,7 +228,7 @@ const char *check_types(int x_type, int w_type, bool backward) {
 }
 
 struct Workspace {
-    int64_t weights = 0, image = 0, x_columns = 0, d_columns = 0, total = 0;
+    int64_t weights = 0, index = 0, image = 0, x_columns = 0, d_columns = 0, total = 0;
 };
 
 // Layout of a call's workspace.  The plan is a function of the topology, the device and the arguments.
@@ -226,6 +236,7 @@ Workspace layout(const spdnn_topology &top, const GatherPlan &g, const DeviceTab
     Workspace w;
     int64_t at = 0;
     w.weights = at; at += aligned(t.entries * sets * type_size(weight));
+    w.index = at; at += aligned(t.entries * (g.global ? 4 : 2));
     w.image = at; at += aligned(g.tiles * g.image_bytes);
     if (backward) {
         const int64_t stride = (tokens + 63) / 64 * 64;
@@ -252,6 +263,11 @@ Matrix matrix(const spdnn_operand_t *o) {
     Matrix m{nullptr, nullptr, 0, F32};
     if (o) { m.data = o->data; m.scales = o->scales; m.stride = o->stride; m.type = o->type; }
     return m;
+}
+
+// Whether every row begins on 16 bytes (microscaled rows always do as far as the kernels load them).
+bool on_16_bytes(const spdnn_operand_t *o) {
+    return !o || o->type == MX4 || (reinterpret_cast<uintptr_t>(o->data) % 16 == 0 && o->stride * type_size(o->type) % 16 == 0);
 }
 
 // nullptr, or what is wrong with an operand of `rows` x `cols` values
@@ -319,17 +335,17 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     OnDevice guard(c.top->device);
     if (guard.status != cudaSuccess) return fail_cuda(c.err, c.err_len, guard.status);
     char *base = (char *)c.workspace;
-    cudaError_t e = launch_order(matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, wt, base + ws.weights, c.stream);
+    cudaError_t e = launch_order(g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, 1, c.sets, wt, it, base + ws.weights, base + ws.index, c.stream);
     if (e == cudaSuccess) {
         PackArgs p{};
         p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
-        p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p;
+        p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x);
         e = launch_pack(p, it, 1, false, c.stream);
     }
     if (e == cudaSuccess) {
         GatherArgs a{};
-        a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.idx = g.global ? (const void *)t.idx : t.idx16;
-        a.weights = base + ws.weights; a.outs = t.outs; a.rows = t.rows; a.tokens = c.tokens;
+        a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
+        a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
         a.bias0 = b0; a.bias1 = b1; a.act = c.act; a.clip = c.clip;
         a.y = const_cast<void *>(c.y->data); a.y_stride = c.y->stride; a.y_type = c.y->type;
         if (c.z[0]) { a.z0 = (float *)const_cast<void *>(c.z[0]->data); a.z_stride = c.z[0]->stride; }
@@ -378,17 +394,18 @@ int run_backward(const Call &c, const Gradients &d) {
         p.x = matrix(d.dy);
         if (c.z[0]) { p.z0 = (const float *)c.z[0]->data; p.z_stride = c.z[0]->stride; }
         if (c.z[1]) p.z1 = (const float *)c.z[1]->data;
+        p.vector = on_16_bytes(d.dy) && on_16_bytes(c.z[0]) && on_16_bytes(c.z[1]);
         p.rows = h.outputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.act = c.act; p.clip = c.clip;
         p.image = d.dx ? base + ws.image : nullptr; p.image_bytes = g.image_bytes;
         p.columns = d.dw[0] ? base + ws.d_columns : nullptr; p.token_stride = stride;
         e = launch_pack(p, type, c.sets, true, c.stream);
     }
     if (c.tokens > 0 && d.dx && e == cudaSuccess) {
-        e = launch_order(matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, type, base + ws.weights, c.stream);
+        e = launch_order(g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, c.sets, type, type, base + ws.weights, base + ws.index, c.stream);
         if (e == cudaSuccess) {
             GatherArgs a{};
-            a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.idx = g.global ? (const void *)t.idx : t.idx16;
-            a.weights = base + ws.weights; a.outs = t.outs; a.rows = t.rows; a.tokens = c.tokens;
+            a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
+            a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
             a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
             e = launch_gather(g, a, type, type, c.sets, 1, c.stream);
         }
@@ -396,7 +413,7 @@ int run_backward(const Call &c, const Gradients &d) {
     if (d.dw[0] && e == cudaSuccess) {
         if (c.tokens > 0) {
             PackArgs p{};
-            p.x = matrix(c.x); p.rows = h.inputs; p.tokens = c.tokens; p.v = p.p = 1;
+            p.x = matrix(c.x); p.rows = h.inputs; p.tokens = c.tokens; p.v = p.p = 1; p.vector = on_16_bytes(c.x);
             p.columns = base + ws.x_columns; p.token_stride = stride;
             e = launch_pack(p, type, 1, false, c.stream);
         }

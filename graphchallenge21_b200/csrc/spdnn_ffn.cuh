@@ -23,6 +23,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace spdnn_impl {
 namespace ffn {
 
@@ -78,29 +80,48 @@ constexpr float kInvSqrt2 = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluA = 0.79788456080286536f, kGeluB = 0.044715f;
 
+// v / (1 + e^-w), the shape of SILU (w = v) and of GELU_TANH (w = 2 a (v + b v^3): (1 + tanh(w / 2)) / 2 = 1 / (1 + e^-w)).  FAST:
+// the hardware's exponential and reciprocal, a few 2^-22 off: for results that are rounded to 16 bits, or made of 16-bit operands.
+template <bool FAST> __device__ __forceinline__ float sigmoid_times(float v, float w) {
+    return FAST ? __fdividef(v, 1.0f + __expf(-w)) : v / (1.0f + expf(-w));
+}
+
 // A NaN stays one (v < 0 is false for it).
-__device__ __forceinline__ float activate(float v, int act, float clip) {
+template <bool FAST> __device__ __forceinline__ float activate(float v, int act, float clip) {
     switch (act) {
         case RELU: return v < 0.0f ? 0.0f : v;
         case CLIP: return v < 0.0f ? 0.0f : v > clip ? clip : v;
-        case SILU: return v / (1.0f + expf(-v));
+        case SILU: return sigmoid_times<FAST>(v, v);
         case GELU: return 0.5f * v * (1.0f + erff(v * kInvSqrt2));
-        case GELU_TANH: return 0.5f * v * (1.0f + tanhf(kGeluA * (v + kGeluB * v * v * v)));
+        case GELU_TANH: return sigmoid_times<FAST>(v, 2.0f * kGeluA * (v + kGeluB * v * v * v));
         default: return v;
     }
 }
 
-__device__ __forceinline__ float activate_slope(float v, int act, float clip) {
+// act(v) and act'(v) for the backward pass
+__device__ __forceinline__ void activate_both(float v, int act, float clip, float &value, float &slope) {
     switch (act) {
-        case RELU: return v > 0.0f ? 1.0f : v != v ? v : 0.0f;
-        case CLIP: return v > 0.0f && v < clip ? 1.0f : v != v ? v : 0.0f;
-        case SILU: { const float s = 1.0f / (1.0f + expf(-v)); return s * (1.0f + v * (1.0f - s)); }
-        case GELU: return 0.5f * (1.0f + erff(v * kInvSqrt2)) + v * kInvSqrt2Pi * expf(-0.5f * v * v);
-        case GELU_TANH: {
-            const float t = tanhf(kGeluA * (v + kGeluB * v * v * v));
-            return 0.5f * (1.0f + t) + 0.5f * v * (1.0f - t * t) * kGeluA * (1.0f + 3.0f * kGeluB * v * v);
+        case RELU: value = v < 0.0f ? 0.0f : v; slope = v > 0.0f ? 1.0f : v != v ? v : 0.0f; return;
+        case CLIP:
+            value = v < 0.0f ? 0.0f : v > clip ? clip : v;
+            slope = v > 0.0f && v < clip ? 1.0f : v != v ? v : 0.0f;
+            return;
+        case SILU: {
+            const float s = 1.0f / (1.0f + expf(-v));
+            value = v * s; slope = s * (1.0f + v * (1.0f - s));
+            return;
         }
-        default: return 1.0f;
+        case GELU: {
+            const float h = 0.5f * (1.0f + erff(v * kInvSqrt2));
+            value = v * h; slope = h + v * kInvSqrt2Pi * expf(-0.5f * v * v);
+            return;
+        }
+        case GELU_TANH: {
+            const float s = 1.0f / (1.0f + expf(-2.0f * kGeluA * (v + kGeluB * v * v * v)));
+            value = v * s; slope = s + v * s * (1.0f - s) * 2.0f * kGeluA * (1.0f + 3.0f * kGeluB * v * v);
+            return;
+        }
+        default: value = v; slope = 1.0f;
     }
 }
 
@@ -162,13 +183,49 @@ template <class E, int V> struct Values {
     }
 };
 
+// V consecutive 16- or 32-bit values as they are in memory.
+template <class E, int V> struct Raw {
+    static constexpr int kBytes = V * (int)sizeof(E);
+    uint32_t w[(kBytes + 3) / 4];
+    __device__ __forceinline__ void load(const void *p) {
+        if constexpr (kBytes == 16) { const uint4 r = *(const uint4 *)p; w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w; }
+        else if constexpr (kBytes == 8) { const uint2 r = *(const uint2 *)p; w[0] = r.x; w[1] = r.y; }
+        else if constexpr (kBytes == 4) w[0] = *(const uint32_t *)p;
+        else w[0] = *(const uint16_t *)p;
+    }
+    __device__ __forceinline__ uint32_t bits(int i) const {
+        if constexpr (sizeof(E) == 4) return w[i];
+        else return i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+    }
+};
+
+// c + a b in float32, from the bits of a and b.  Two operands of one 16-bit type go into the mixed-precision fma as they are: exact
+// product, one rounding, and none of the conversions (two per pair of values) that took a third of the inner loop.
+template <class E, class W> __device__ __forceinline__ float fma_bits(uint32_t a, uint32_t b, float c) {
+    if constexpr (sizeof(E) == 4) {
+        return fmaf(__uint_as_float(a), __uint_as_float(b), c);
+    } else {
+        const uint16_t x = (uint16_t)a, y = (uint16_t)b;
+        float d;
+        if constexpr (std::is_same<E, bf16>::value && std::is_same<W, bf16>::value)
+            asm("fma.rn.f32.bf16 %0, %1, %2, %3;" : "=f"(d) : "h"(x), "h"(y), "f"(c));
+        else if constexpr (std::is_same<E, __half>::value && std::is_same<W, __half>::value)
+            asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(x), "h"(y), "f"(c));
+        else
+            d = fmaf(__half2float(__ushort_as_half(x)), __uint_as_float(b << 16), c);
+        return d;
+    }
+}
+
 // ---- images -------------------------------------------------------------------------------------
 
 // An image: rows + 1 neurons (the last one zeros) x SETS values x T = V P tokens, in UNITS of V tokens (16 bytes, or less where a
 // neuron's tokens are fewer).  Unit (n, s, p) is number q = (n SETS + s) P + p.  Units of 16 bytes are stored at
-// q ^ (q / 8 mod 8): whoever writes an image walks along n, and without it the units of 8 neurons would share banks.
+// q ^ (q / 8 mod 8): the units p of a neuron are spread over the banks differently from neuron to neuron, so that whoever
+// walks along n does not stay on one bank.  Within a neuron (n, s, p) lies at swizzle(n SETS P) ^ unit_in_neuron(s, p).
 __host__ __device__ __forceinline__ uint32_t image_units(int rows, int per_row) { return ((uint32_t)(rows + 1) * per_row + 7u) & ~7u; }
 __host__ __device__ __forceinline__ uint32_t swizzle(uint32_t q) { return q ^ ((q >> 3) & 7u); }
+__host__ __device__ constexpr uint32_t unit_in_neuron(int s, int p, int P) { return (uint32_t)(s * P) ^ (P == 8 ? (uint32_t)s : 0u) ^ (uint32_t)p; }
 
 struct Matrix {            // a caller's operand
     const void *data;
@@ -186,93 +243,173 @@ struct PackArgs {
     void *columns;         // [rows][sets][token_stride], or nullptr: what dw_kernel reads (gradients as float)
     int64_t token_stride;
     int rows, tokens;
-    int v, p;              // the image's unit and units per neuron
+    int v, p;              // the image's unit and units per neuron (powers of two)
+    int vector;            // every row of every operand begins on 16 bytes
     int act;
     float clip;
 };
 
 constexpr int kPackThreads = 256;
 
-// One block: 64 neurons x 64 tokens, through shared memory so that reads run along neurons and writes along tokens.
+// `COUNT` neighbours of a row as floats, from column `col` on; zeros behind `cols`.
+template <int COUNT>
+__device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int64_t row, int col, int cols, float (&v)[COUNT]) {
+    if (x.type == MX4) {
+        const int64_t b = row * x.stride + (col >> 5);
+        const float scale = e8m0_value(__ldg(x.scales + b));
+#pragma unroll
+        for (int k = 0; k < COUNT; k += 2) {
+            const uint32_t byte = __ldg((const uint8_t *)x.data + b * 16 + (((col & 31) + k) >> 1));
+            v[k] = col + k < cols ? e2m1_value(byte & 15u) * scale : 0.0f;
+            v[k + 1] = col + k + 1 < cols ? e2m1_value(byte >> 4) * scale : 0.0f;
+        }
+        return;
+    }
+    if (vector && col + COUNT <= cols) {
+        if (x.type == F32) {
+#pragma unroll
+            for (int k = 0; k < COUNT; k += 4) {
+                const float4 r = __ldg((const float4 *)((const float *)x.data + row * x.stride + col + k));
+                v[k] = r.x; v[k + 1] = r.y; v[k + 2] = r.z; v[k + 3] = r.w;
+            }
+            return;
+        }
+        if constexpr (COUNT == 8) {
+            const uint4 r = __ldg((const uint4 *)((const uint16_t *)x.data + row * x.stride + col));
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f32x2 two = x.type == F16 ? widen<__half>(w[k]) : widen<bf16>(w[k]);
+                unpack2(two, v[2 * k], v[2 * k + 1]);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) v[k] = col + k < cols ? load_as_float(x.data, x.type, row * x.stride + col + k) : 0.0f;
+}
+
+// One block: 64 neurons x 64 tokens, through shared memory so that reads run along neurons and writes along tokens.  The tokens of a
+// neuron are permuted in groups of N (16 bytes of the tile), for the writers of neighbouring neurons to hit different banks.
 template <class E, int SETS, bool GRADIENT>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackArgs a) {
-    __shared__ float tile[SETS][64][65];
+    using Tile = typename std::conditional<GRADIENT, float, E>::type;
+    constexpr int N = 16 / (int)sizeof(E);            // neurons a thread loads at a time
+    constexpr int G = 16 / (int)sizeof(Tile);         // tokens of a permuted group
+    constexpr int ROW = 64 + G;
+    __shared__ __align__(16) Tile tile[SETS][64][ROW];
+    const auto at = [](int n, int t) { return t ^ (((n / N) & (64 / G - 1)) * G); };
     const int blocks_n = (a.rows + 63) / 64;
     const int n0 = (int)(blockIdx.x % blocks_n) * 64;
     const int t0 = (int)(blockIdx.x / blocks_n) * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += kPackThreads) {
-        const int t = i >> 6, n = i & 63;
-        float d0 = 0.0f, d1 = 0.0f;
+    for (int i = threadIdx.x; i < 64 * 64 / N; i += kPackThreads) {
+        const int t = i / (64 / N), n = i % (64 / N) * N;
+        float d0[N], d1[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) d0[k] = d1[k] = 0.0f;
         if (t0 + t < a.tokens && n0 + n < a.rows) {
             const int64_t row = t0 + t;
             const int col = n0 + n;
-            if (!GRADIENT) {
-                d0 = a.x.type == MX4 ? mx4_value((const uint8_t *)a.x.data, a.x.scales, a.x.stride, row, col)
-                                     : load_as_float(a.x.data, a.x.type, row * a.x.stride + col);
-            } else {
-                const float dy = load_as_float(a.x.data, a.x.type, row * a.x.stride + col);
-                const float z0 = a.act == NONE && SETS == 1 ? 0.0f : __ldg(a.z0 + row * a.z_stride + col);
-                d0 = dy * activate_slope(z0, a.act, a.clip);
-                if (SETS == 2) {
-                    d0 *= __ldg(a.z1 + row * a.z_stride + col);
-                    d1 = dy * activate(z0, a.act, a.clip);
+            load_row_part<N>(a.x, a.vector, row, col, a.rows, d0);
+            if constexpr (GRADIENT) {
+                float g[N], u[N];
+                const bool saved = SETS == 2 || a.act != NONE;
+                if (saved) load_row_part<N>(Matrix{a.z0, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, g);
+                if (SETS == 2) load_row_part<N>(Matrix{a.z1, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, u);
+                if (saved) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        float value, slope;
+                        activate_both(g[k], a.act, a.clip, value, slope);
+                        if (SETS == 2) { d1[k] = d0[k] * value; slope *= u[k]; }
+                        d0[k] *= slope;
+                        if (col + k >= a.rows) d0[k] = d1[k] = 0.0f;
+                    }
                 }
             }
         }
-        tile[0][n][t] = d0;
-        if (SETS == 2) tile[SETS - 1][n][t] = d1;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            tile[0][n + k][at(n, t)] = from_float<Tile>(d0[k]);
+            if (SETS == 2) tile[SETS - 1][n + k][at(n, t)] = from_float<Tile>(d1[k]);
+        }
     }
     __syncthreads();
     if (a.image) {
-        const int T = a.v * a.p, per_row = a.p * SETS;
+        const int log_p = 31 - __clz(a.p), T = a.v * a.p, per_row = a.p * SETS;
         const uint32_t units = image_units(a.rows, per_row);
-        const bool swizzled = a.v * (int)sizeof(E) == 16;
-        const int per_token_block = 64 / a.v;
-        const int tiles = (a.tokens + T - 1) / T;
+        const int64_t tiles = ((int64_t)a.tokens + T - 1) / T;
         // the last block along n also writes the row of zeros and the units behind it
         const int n_end = n0 + 64 >= a.rows ? (int)((units + per_row - 1) / per_row) - n0 : 64;
-        for (int i = threadIdx.x; i < n_end * SETS * per_token_block; i += kPackThreads) {
-            // along tokens first within a tile, then along n
-            const int p = i % a.p, rest = i / a.p;
-            const int s = rest % SETS, rest2 = rest / SETS;
-            const int n = rest2 % n_end, part = rest2 / n_end;
-            const int t = (part * a.p + p) * a.v;
-            const int tile_index = (t0 + t) / T;
-            const uint32_t q = ((uint32_t)(n0 + n) * SETS + s) * a.p + p;
-            if (tile_index >= tiles || q >= units) continue;
-            E *to = (E *)((char *)a.image + (int64_t)tile_index * a.image_bytes) + (size_t)(swizzled ? swizzle(q) : q) * a.v;
-            const bool real = n < 64 && n0 + n < a.rows;
-            for (int k = 0; k < a.v; ++k) to[k] = from_float<E>(real ? tile[s][n & 63][t + k] : 0.0f);
+        for (int part = 0; part * T < 64; ++part) {
+            const int64_t tile_index = (t0 + part * T) / T;
+            if (tile_index >= tiles) break;
+            char *image = (char *)a.image + tile_index * a.image_bytes;
+            for (int i = threadIdx.x; i < n_end * per_row; i += kPackThreads) {
+                const int p = i & (a.p - 1), s = (i >> log_p) & (SETS - 1), n = (i >> log_p) / SETS;
+                const uint32_t q = (uint32_t)n0 * per_row + i;
+                if (q >= units) break;
+                const bool real = n < 64 && n0 + n < a.rows;
+                const int t = part * T + p * a.v;
+                if (a.v == N) {
+                    uint4 r = make_uint4(0, 0, 0, 0);
+                    if (real) {
+                        if constexpr (!GRADIENT || sizeof(E) == 4) {
+                            r = *(const uint4 *)&tile[s][n][at(n, t)];
+                        } else {
+                            const float4 lo = *(const float4 *)&tile[s][n][at(n, t)], hi = *(const float4 *)&tile[s][n][at(n, t + 4)];
+                            E e[8] = {from_float<E>(lo.x), from_float<E>(lo.y), from_float<E>(lo.z), from_float<E>(lo.w),
+                                      from_float<E>(hi.x), from_float<E>(hi.y), from_float<E>(hi.z), from_float<E>(hi.w)};
+                            r = *(const uint4 *)e;
+                        }
+                    }
+                    ((uint4 *)image)[swizzle(q)] = r;
+                } else {
+                    for (int k = 0; k < a.v; ++k) ((E *)image)[(size_t)q * a.v + k] = from_float<E>(real ? to_float(tile[s][n & 63][at(n & 63, t + k)]) : 0.0f);
+                }
+            }
         }
     }
     if (a.columns) {
-        for (int i = threadIdx.x; i < SETS * 64 * 64; i += kPackThreads) {
-            const int t = i & 63, n = (i >> 6) & 63, s = i >> 12;
+        for (int i = threadIdx.x; i < SETS * 64 * (64 / G); i += kPackThreads) {
+            const int t = i % (64 / G) * G, n = i / (64 / G) % 64, s = i / (64 / G) / 64;
             if (n0 + n >= a.rows) continue;
-            const int64_t at = ((int64_t)(n0 + n) * SETS + s) * a.token_stride + t0 + t;
-            if (GRADIENT) ((float *)a.columns)[at] = tile[s][n][t];
-            else ((E *)a.columns)[at] = from_float<E>(tile[s][n][t]);
+            Tile *to = (Tile *)a.columns + ((int64_t)(n0 + n) * SETS + s) * a.token_stride + t0 + t;
+            *(uint4 *)to = *(const uint4 *)&tile[s][n][at(n, t)];
         }
     }
 }
 
-// The weights of a gather table in its order: [quads][32][4][sets].  Padding gets zero, whatever the caller's matrix holds
-// where a neuron has no connection.
+struct OrderArgs {
+    Matrix w0, w1;
+    const uint32_t *idx, *src;  // the gather table (topology.h)
+    int64_t entries;
+    int slots;
+    int values, p;              // the image's values and units per neuron
+    int swizzled, wide;         // its units are 16 bytes; indexes are 32 bits (image in global memory)
+    void *weights, *index;      // [quads][32][4][sets], [quads][32][4]
+};
+
+// The gather table as a call's gather reads it: the weights in its order, and the place of every gathered neuron in the image.  Padding
+// gets the weight zero, whatever the caller's matrix holds where a neuron has no connection.
 template <class W, int SETS>
-__global__ void __launch_bounds__(256) order_weights_kernel(const Matrix w0, const Matrix w1, const uint32_t *__restrict__ src, int slots,
-                                                            int64_t entries, W *__restrict__ out) {
+__global__ void __launch_bounds__(256) order_kernel(const OrderArgs a) {
     const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= entries) return;
-    const uint32_t s = __ldg(src + e);
-    const uint32_t c = s / (uint32_t)slots, j = s % (uint32_t)slots;
+    if (e >= a.entries) return;
+    const uint32_t s = __ldg(a.src + e), n = __ldg(a.idx + e);
+    const uint32_t c = s / (uint32_t)a.slots, j = s % (uint32_t)a.slots;
+#pragma unroll
     for (int k = 0; k < SETS; ++k) {
-        const Matrix &w = k ? w1 : w0;
+        const Matrix &w = k ? a.w1 : a.w0;
         float v = 0.0f;
         if (s != 0xffffffffu)
             v = w.type == MX4 ? mx4_value((const uint8_t *)w.data, w.scales, w.stride, c, (int)j)
                               : load_as_float(w.data, w.type, (int64_t)c * w.stride + j);
-        out[e * SETS + k] = from_float<W>(v);
+        ((W *)a.weights)[e * SETS + k] = from_float<W>(v);
     }
+    const uint32_t place = a.swizzled ? swizzle(n * (uint32_t)(a.values * a.p)) : n;
+    if (a.wide) ((uint32_t *)a.index)[e] = place;
+    else ((uint16_t *)a.index)[e] = (uint16_t)place;
 }
 
 // ---- the gather ----------------------------------------------------------------------------------
@@ -281,9 +418,9 @@ struct GatherArgs {
     const void *image;          // tiles of image_bytes
     int64_t image_bytes;
     const uint32_t *slice_ptr;  // the gather table (topology.h)
-    const void *idx;            // uint16_t (image in shared memory) or uint32_t
-    const void *weights;        // order_weights_kernel's
-    int outs, tokens, rows, splits;
+    const void *index;          // order_kernel's: uint16_t (image in shared memory) or uint32_t
+    const void *weights;
+    int outs, tokens, splits;
     const float *bias0, *bias1; // or nullptr
     void *y;
     float *z0, *z1;             // pre-activations, or nullptr
@@ -293,7 +430,10 @@ struct GatherArgs {
     float clip;
 };
 
-constexpr int kGatherThreads = 512;
+#ifndef SPDNN_GATHER_THREADS
+#define SPDNN_GATHER_THREADS 768
+#endif
+constexpr int kGatherThreads = SPDNN_GATHER_THREADS;
 
 // Brings `bytes` (a multiple of 16) from global to shared memory, 16 bytes per thread and copy, none of them through registers.
 __device__ __forceinline__ void copy_in(void *dst, const void *src, uint32_t bytes) {
@@ -305,96 +445,149 @@ __device__ __forceinline__ void copy_in(void *dst, const void *src, uint32_t byt
     __syncthreads();
 }
 
+// Four connections of a lane's neuron.
+template <class W, int SETS, bool WIDE> struct Quad {
+    static constexpr int kWords = SETS * (int)sizeof(W);     // 32-bit words of 4 x SETS weights
+    uint32_t index[WIDE ? 4 : 2];
+    uint32_t weight[kWords];
+    __device__ __forceinline__ void load(const GatherArgs &a, size_t at) {
+        if constexpr (WIDE) {
+            const uint4 r = __ldg((const uint4 *)a.index + at);
+            index[0] = r.x; index[1] = r.y; index[2] = r.z; index[3] = r.w;
+        } else {
+            const uint2 r = __ldg((const uint2 *)a.index + at);
+            index[0] = r.x; index[1] = r.y;
+        }
+        if constexpr (kWords == 2) {
+            const uint2 r = __ldg((const uint2 *)a.weights + at);
+            weight[0] = r.x; weight[1] = r.y;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kWords / 4; ++k) {
+                const uint4 r = __ldg((const uint4 *)a.weights + at * (kWords / 4) + k);
+                weight[4 * k] = r.x; weight[4 * k + 1] = r.y; weight[4 * k + 2] = r.z; weight[4 * k + 3] = r.w;
+            }
+        }
+    }
+    // bits of weight `set` of connection `k`
+    __device__ __forceinline__ uint32_t bits(int k, int set) const {
+        const int e = k * SETS + set;
+        if constexpr (sizeof(W) == 4) return weight[e];
+        else return e & 1 ? weight[e >> 1] >> 16 : weight[e >> 1] & 0xffffu;
+    }
+};
+
 // One block: the image of one tile of T = V P tokens, and a range of the gathering neurons.  Unit of work of a warp: 32 / P
 // neurons, P lanes each with V tokens.  S = 1: one gathered value for G sums (forward).  S = 2: two gathered values for one sum
 // (backward of the gated block).  GLOBAL: the image stays in global memory (it does not fit on the SM).
+//
+// The table (index and weights of a quad: up to 24 bytes a lane) comes from L2, where a load takes longer than the
+// arithmetic of a quad: each is requested while the one before it is worked on, across the border of two units too.
 template <class E, class W, int V, int P, int S, int G, bool GLOBAL>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const GatherArgs a) {
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_constant__ GatherArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
-    constexpr int PAIRS = Values<E, V>::kPairs;
     constexpr int SETS = S > G ? S : G;
-    constexpr bool SWIZZLED = V * sizeof(E) == 16;
+    constexpr int UB = V * (int)sizeof(E);
+    constexpr bool SWIZZLED = UB == 16;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
     const char *image = (const char *)a.image + (int64_t)tile * a.image_bytes;
-    if constexpr (!GLOBAL) {
-        copy_in(smem, image, (uint32_t)a.image_bytes);
-        image = (const char *)smem;
-    }
-    const int p = lane % P, sub = lane / P;
+    const int p = lane % P;
     const int slices = (a.outs + 31) / 32;
     const int64_t units = (int64_t)slices * P;
     const int64_t last = units * (split + 1) / a.splits;
-    for (int64_t unit = units * split / a.splits + warp; unit < last; unit += kGatherThreads / 32) {
-        const int slice = (int)(unit / P);
-        const int in_slice = (int)(unit % P) * (32 / P) + sub;
-        const uint32_t q0 = __ldg(a.slice_ptr + slice), q1 = __ldg(a.slice_ptr + slice + 1);
-        f32x2 acc[G][PAIRS];
+    int64_t unit = units * split / a.splits + warp;
+    uint32_t q0 = 0, q1 = 0;
+    if (unit < last) { q0 = __ldg(a.slice_ptr + unit / P); q1 = __ldg(a.slice_ptr + unit / P + 1); }
+    const auto lane_of = [&](int64_t u) { return (int)(u % P) * (32 / P) + lane / P; };
+    Quad<W, SETS, GLOBAL> cur;
+    if (q0 < q1) cur.load(a, (size_t)q0 * 32 + lane_of(unit));
+    if constexpr (!GLOBAL) copy_in(smem, image, (uint32_t)a.image_bytes);
+    uint32_t place[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) place[s] = SWIZZLED ? unit_in_neuron(s, p, P) * 16u : (uint32_t)(s * UB);
+    while (unit < last) {
+        const int64_t next = unit + kGatherThreads / 32;
+        uint32_t n0 = 0, n1 = 0;
+        if (next < last) { n0 = __ldg(a.slice_ptr + next / P); n1 = __ldg(a.slice_ptr + next / P + 1); }
+        float acc[G][V];
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int k = 0; k < PAIRS; ++k) acc[g][k] = 0;
+            for (int k = 0; k < V; ++k) acc[g][k] = 0.0f;
+        Quad<W, SETS, GLOBAL> ahead;
+        if (q0 >= q1 && n0 < n1) cur.load(a, (size_t)n0 * 32 + lane_of(next));
         for (uint32_t q = q0; q < q1; ++q) {
-            const size_t at = (size_t)q * 32 + in_slice;
-            uint32_t rows[4];
-            if constexpr (GLOBAL) {
-                const uint4 r = __ldg((const uint4 *)a.idx + at);
-                rows[0] = r.x; rows[1] = r.y; rows[2] = r.z; rows[3] = r.w;
-            } else {
-                const uint2 r = __ldg((const uint2 *)a.idx + at);
-                rows[0] = r.x & 0xffffu; rows[1] = r.x >> 16; rows[2] = r.y & 0xffffu; rows[3] = r.y >> 16;
-            }
-            Values<W, 4 * SETS <= 16 / (int)sizeof(W) ? 4 * SETS : 16 / (int)sizeof(W)> w[4 * SETS * sizeof(W) > 16 ? 4 * SETS * sizeof(W) / 16 : 1];
-            constexpr int PER = 4 * SETS * sizeof(W) > 16 ? 16 / (int)sizeof(W) : 4 * SETS;
-#pragma unroll
-            for (int k = 0; k < (int)(4 * SETS / PER); ++k) w[k].load((const char *)a.weights + (at * 4 * SETS + (size_t)k * PER) * sizeof(W));
+            const bool inside = q + 1 < q1;
+            if (inside || n0 < n1) ahead.load(a, inside ? (size_t)(q + 1) * 32 + lane_of(unit) : (size_t)n0 * 32 + lane_of(next));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
-                    Values<E, V> x;
-                    const uint32_t unit_in_image = (rows[k] * S + s) * P + p;
+                    Raw<E, V> x;
                     if constexpr (GLOBAL) {
-                        x.load(image + (size_t)(SWIZZLED ? swizzle(unit_in_image) : unit_in_image) * (V * sizeof(E)));
+                        x.load(image + (((size_t)cur.index[k] * 16u) ^ place[s]));
+                    } else if constexpr (SWIZZLED) {
+                        const uint32_t w = cur.index[k >> 1];
+                        x.load(smem + (((k & 1 ? w >> 12 : w << 4) & 0xffff0u) ^ place[s]));
                     } else {
-                        x.load(image + (SWIZZLED ? swizzle(unit_in_image) : unit_in_image) * (uint32_t)(V * sizeof(E)));
+                        const uint32_t w = cur.index[k >> 1];
+                        x.load(smem + (k & 1 ? w >> 16 : w & 0xffffu) * (uint32_t)(S * UB) + place[s]);
                     }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const int e = k * SETS + (S > 1 ? s : g);
-                        float lo, hi;
-                        unpack2(w[e / PER].v[e % PER / 2], lo, hi);
-                        const float one = e % 2 ? hi : lo;
-                        const f32x2 both = pack2(one, one);
+                        const uint32_t w = cur.bits(k, S > 1 ? s : g);
 #pragma unroll
-                        for (int i = 0; i < PAIRS; ++i) acc[g][i] = fma2(x.v[i], both, acc[g][i]);
+                        for (int i = 0; i < V; ++i) acc[g][i] = fma_bits<E, W>(x.bits(i), w, acc[g][i]);
                     }
                 }
             }
+            cur = ahead;
         }
-        const int c = slice * 32 + in_slice;
-        if (c >= a.outs) continue;
-        float z[G][2 * PAIRS];
+        const int c = (int)(unit / P) * 32 + lane_of(unit);
+        if (c < a.outs) {
+            const float b0 = a.bias0 ? __ldg(a.bias0 + c) : 0.0f, b1 = G == 2 && a.bias1 ? __ldg(a.bias1 + c) : 0.0f;
+            const int64_t t0 = (int64_t)tile * (V * P) + p * V;
+            const int count = (int)min((int64_t)V, (int64_t)a.tokens - t0);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float *bias = g ? a.bias1 : a.bias0;
-            const float b = bias ? __ldg(bias + c) : 0.0f;
+            for (int k = 0; k < V; ++k) {
+                acc[0][k] += b0;
+                if (G == 2) acc[G - 1][k] += b1;
+            }
+            if (a.z0) {
+                float *z = a.z0 + t0 * a.z_stride + c;
 #pragma unroll
-            for (int k = 0; k < PAIRS; ++k) {
-                unpack2(acc[g][k], z[g][2 * k], z[g][2 * k + 1]);
-                z[g][2 * k] += b; z[g][2 * k + 1] += b;
+                for (int k = 0; k < V; ++k, z += a.z_stride)
+                    if (k < count) *z = acc[0][k];
+                if (G == 2) {
+                    z = a.z1 + t0 * a.z_stride + c;
+#pragma unroll
+                    for (int k = 0; k < V; ++k, z += a.z_stride)
+                        if (k < count) *z = acc[G - 1][k];
+                }
+            }
+            if (S == 1) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    acc[0][k] = activate<sizeof(E) == 2>(acc[0][k], a.act, a.clip);
+                    if (G == 2) acc[0][k] *= acc[G - 1][k];
+                }
+            }
+            const int64_t at = t0 * a.y_stride + c;
+            if (a.y_type == F32) {
+                float *y = (float *)a.y + at;
+#pragma unroll
+                for (int k = 0; k < V; ++k, y += a.y_stride)
+                    if (k < count) *y = acc[0][k];
+            } else {
+                uint16_t *y = (uint16_t *)a.y + at;
+#pragma unroll
+                for (int k = 0; k < V; ++k, y += a.y_stride)
+                    if (k < count)
+                        *y = a.y_type == F16 ? __half_as_ushort(__float2half_rn(acc[0][k])) : __bfloat16_as_ushort(__float2bfloat16_rn(acc[0][k]));
             }
         }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const int64_t t = (int64_t)tile * (V * P) + p * V + k;
-            if (t >= a.tokens) break;
-            float y = activate(z[0][k], a.act, a.clip);
-            if (G == 2) y *= z[G - 1][k];
-            store_from_float(a.y, a.y_type, t * a.y_stride + c, y);
-            if (a.z0) a.z0[t * a.z_stride + c] = z[0][k];
-            if (G == 2 && a.z1) a.z1[t * a.z_stride + c] = z[G - 1][k];
-        }
+        unit = next; q0 = n0; q1 = n1;
     }
 }
 
