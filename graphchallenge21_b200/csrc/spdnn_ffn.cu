@@ -132,10 +132,10 @@ GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int toke
     const int T = g.v * g.p;
     g.tiles = (tokens + T - 1) / T;
     const int64_t per_sm = g.global ? 2 : std::max<int64_t>(1, std::min<int64_t>(2, kSharedLimit / (g.image_bytes + 1024)));
-    const int64_t slots = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * g.p;
+    const int64_t slots = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * (g.p / lane_units(g.p));
     // Blocks of a tile: clocks of a wave of blocks are those of the image (about 40 bytes a clock) and of the block's units (a
     // connection of 32 lanes about 8 clocks of the SM); the fewest in all waves.
-    const double per_unit = 8.0 * std::max<double>(1.0, (double)t.entries / 32.0 / std::max<int64_t>(1, (t.outs + 31) / 32)) / per_sm;
+    const double per_unit = 8.0 * lane_units(g.p) * std::max<double>(1.0, (double)t.entries / 32.0 / std::max<int64_t>(1, (t.outs + 31) / 32)) / per_sm;
     double best = 0.0;
     for (int64_t s = 1; s <= 2 * slots && (s == 1 || s * 16 <= units); ++s) {
         const int64_t waves = (g.tiles * s + slots - 1) / slots;
@@ -183,7 +183,8 @@ cudaError_t launch_gather(const GatherPlan &g, GatherArgs a, int image_type, int
         if (e != cudaSuccess) return e;
     }
     void *args[] = {&a};
-    return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(kGatherThreads), args, shared, stream);
+    const int threads = gather_threads(g.v * lane_units(g.p) * (s == 2 ? 1 : sets));
+    return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(threads), args, shared, stream);
 }
 
 cudaError_t launch_pack(const PackArgs &a, int image_type, int sets, bool gradient, cudaStream_t stream) {
@@ -203,7 +204,7 @@ cudaError_t launch_order(const GatherPlan &g, const Matrix &w0, const Matrix &w1
     if (!t.entries) return cudaSuccess;
     OrderArgs a{};
     a.w0 = w0; a.w1 = w1; a.idx = t.idx; a.src = t.src; a.entries = t.entries; a.slots = slots; a.values = values; a.p = g.p;
-    a.swizzled = g.v * type_size(image_type) == 16; a.wide = g.global;
+    a.whole = g.v * type_size(image_type) == 16; a.wide = g.global;
     a.weights = weights; a.index = index;
     const unsigned grid = (unsigned)((t.entries + 255) / 256);
     const auto run = [&](auto w) {

@@ -83,7 +83,11 @@ constexpr float kGeluA = 0.79788456080286536f, kGeluB = 0.044715f;
 // v / (1 + e^-w), the shape of SILU (w = v) and of GELU_TANH (w = 2 a (v + b v^3): (1 + tanh(w / 2)) / 2 = 1 / (1 + e^-w)).  FAST:
 // the hardware's exponential and reciprocal, a few 2^-22 off: for results that are rounded to 16 bits, or made of 16-bit operands.
 template <bool FAST> __device__ __forceinline__ float sigmoid_times(float v, float w) {
-    return FAST ? __fdividef(v, 1.0f + __expf(-w)) : v / (1.0f + expf(-w));
+    if (!FAST) return v / (1.0f + expf(-w));
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(w * -1.44269504088896341f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return v * r;
 }
 
 // A NaN stays one (v < 0 is false for it).
@@ -220,12 +224,16 @@ template <class E, class W> __device__ __forceinline__ float fma_bits(uint32_t a
 // ---- images -------------------------------------------------------------------------------------
 
 // An image: rows + 1 neurons (the last one zeros) x SETS values x T = V P tokens, in UNITS of V tokens (16 bytes, or less where a
-// neuron's tokens are fewer).  Unit (n, s, p) is number q = (n SETS + s) P + p.  Units of 16 bytes are stored at
-// q ^ (q / 8 mod 8): the units p of a neuron are spread over the banks differently from neuron to neuron, so that whoever
-// walks along n does not stay on one bank.  Within a neuron (n, s, p) lies at swizzle(n SETS P) ^ unit_in_neuron(s, p).
+// neuron's tokens are fewer).  A neuron has R = SETS P units in a row; unit u = s P + p of neuron n lies at n R + (u ^ x(n)).  x
+// turns the units of neighbouring neurons against each other, so that the bank group of unit 0 (16 bytes, 8 of them) is made of the three
+// low bits of n whatever R is: of bits 0 and 1 and 2 for its highest and middle and lowest bit (R = 2: 1, 0, 2).  So L = 4, 2 or 1 lanes
+// that read a neuron together meet no other neuron's lanes if those neurons differ in bit 0, in bits 0 and 1, in bits 0 to 2;
+// neurons of 8 bytes meet none of sixteen that differ in the bits 0 to 3.  That is what topology.h orders connections by.
 __host__ __device__ __forceinline__ uint32_t image_units(int rows, int per_row) { return ((uint32_t)(rows + 1) * per_row + 7u) & ~7u; }
-__host__ __device__ __forceinline__ uint32_t swizzle(uint32_t q) { return q ^ ((q >> 3) & 7u); }
-__host__ __device__ constexpr uint32_t unit_in_neuron(int s, int p, int P) { return (uint32_t)(s * P) ^ (P == 8 ? (uint32_t)s : 0u) ^ (uint32_t)p; }
+__host__ __device__ __forceinline__ uint32_t unit_place(uint32_t n, uint32_t per_row) {
+    const uint32_t reversed = (n & 1u) << 2 | (n & 2u) | (n >> 2 & 1u);
+    return n * per_row + (reversed & ((per_row < 8u ? per_row : 8u) - 1u));
+}
 
 struct Matrix {            // a caller's operand
     const void *data;
@@ -363,7 +371,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackArgs a) {
                             r = *(const uint4 *)e;
                         }
                     }
-                    ((uint4 *)image)[swizzle(q)] = r;
+                    ((uint4 *)image)[unit_place(n0 + n, per_row) ^ (uint32_t)(s * a.p + p)] = r;
                 } else {
                     for (int k = 0; k < a.v; ++k) ((E *)image)[(size_t)q * a.v + k] = from_float<E>(real ? to_float(tile[s][n & 63][at(n & 63, t + k)]) : 0.0f);
                 }
@@ -386,7 +394,7 @@ struct OrderArgs {
     int64_t entries;
     int slots;
     int values, p;              // the image's values and units per neuron
-    int swizzled, wide;         // its units are 16 bytes; indexes are 32 bits (image in global memory)
+    int whole, wide;            // its units are 16 bytes; indexes are 32 bits (image in global memory)
     void *weights, *index;      // [quads][32][4][sets], [quads][32][4]
 };
 
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(256) order_kernel(const OrderArgs a) {
                               : load_as_float(w.data, w.type, (int64_t)c * w.stride + j);
         ((W *)a.weights)[e * SETS + k] = from_float<W>(v);
     }
-    const uint32_t place = a.swizzled ? swizzle(n * (uint32_t)(a.values * a.p)) : n;
+    const uint32_t place = a.whole ? unit_place(n, (uint32_t)(a.values * a.p)) : n;
     if (a.wide) ((uint32_t *)a.index)[e] = place;
     else ((uint16_t *)a.index)[e] = (uint16_t)place;
 }
@@ -430,10 +438,16 @@ struct GatherArgs {
     float clip;
 };
 
-#ifndef SPDNN_GATHER_THREADS
-#define SPDNN_GATHER_THREADS 768
+// Units a lane reads per gathered value, and threads per block.  Two units halve what index, weights and the loop cost per fma; with more sums
+// than 16 in registers a block of 1024 threads would spill.
+#ifndef SPDNN_NV
+#define SPDNN_NV 2
 #endif
-constexpr int kGatherThreads = SPDNN_GATHER_THREADS;
+#ifndef SPDNN_BIG
+#define SPDNN_BIG 768
+#endif
+__host__ __device__ constexpr int lane_units(int P) { return P < SPDNN_NV ? P : SPDNN_NV; }
+__host__ __device__ constexpr int gather_threads(int sums) { return sums <= 16 ? 1024 : SPDNN_BIG; }
 
 // Brings `bytes` (a multiple of 16) from global to shared memory, 16 bytes per thread and copy, none of them through registers.
 __device__ __forceinline__ void copy_in(void *dst, const void *src, uint32_t bytes) {
@@ -477,115 +491,139 @@ template <class W, int SETS, bool WIDE> struct Quad {
     }
 };
 
-// One block: the image of one tile of T = V P tokens, and a range of the gathering neurons.  Unit of work of a warp: 32 / P
-// neurons, P lanes each with V tokens.  S = 1: one gathered value for G sums (forward).  S = 2: two gathered values for one sum
-// (backward of the gated block).  GLOBAL: the image stays in global memory (it does not fit on the SM).
+template <class F> __device__ __forceinline__ void with_activation(int act, const F &f) {
+    switch (act) {
+        case RELU: f(std::integral_constant<int, RELU>()); return;
+        case CLIP: f(std::integral_constant<int, CLIP>()); return;
+        case SILU: f(std::integral_constant<int, SILU>()); return;
+        case GELU: f(std::integral_constant<int, GELU>()); return;
+        case GELU_TANH: f(std::integral_constant<int, GELU_TANH>()); return;
+        default: return;
+    }
+}
+
+// One block: the image of one tile of T = V P tokens, and a range of the gathering neurons.  Unit of work of a warp: 32 / L neurons, L
+// lanes each with NV units of V tokens.  S = 1: one gathered value for G sums (forward).  S = 2: two gathered values for one
+// sum (backward of the gated block).  GLOBAL: the image stays in global memory (it does not fit on the SM).
 //
-// The table (index and weights of a quad: up to 24 bytes a lane) comes from L2, where a load takes longer than the
-// arithmetic of a quad: each is requested while the one before it is worked on, across the border of two units too.
+// The table (index and weights of a quad: up to 24 bytes a lane) comes from L2, where a load takes longer than the arithmetic of a
+// quad: each is requested while the one before it is worked on, the first of a unit before the last of the one before it.
 template <class E, class W, int V, int P, int S, int G, bool GLOBAL>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_constant__ GatherArgs a) {
+__global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_kernel(const __grid_constant__ GatherArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int SETS = S > G ? S : G;
     constexpr int UB = V * (int)sizeof(E);
-    constexpr bool SWIZZLED = UB == 16;
+    constexpr bool WHOLE = UB == 16;
+    constexpr int NV = lane_units(P), L = P / NV;
+    constexpr int WARPS = gather_threads(V * NV * G) / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
     const char *image = (const char *)a.image + (int64_t)tile * a.image_bytes;
-    const int p = lane % P;
-    const int slices = (a.outs + 31) / 32;
-    const int64_t units = (int64_t)slices * P;
+    const int j = lane % L;
+    const int64_t units = (int64_t)((a.outs + 31) / 32) * L;
     const int64_t last = units * (split + 1) / a.splits;
     int64_t unit = units * split / a.splits + warp;
     uint32_t q0 = 0, q1 = 0;
-    if (unit < last) { q0 = __ldg(a.slice_ptr + unit / P); q1 = __ldg(a.slice_ptr + unit / P + 1); }
-    const auto lane_of = [&](int64_t u) { return (int)(u % P) * (32 / P) + lane / P; };
-    Quad<W, SETS, GLOBAL> cur;
-    if (q0 < q1) cur.load(a, (size_t)q0 * 32 + lane_of(unit));
+    if (unit < last) { q0 = __ldg(a.slice_ptr + unit / L); q1 = __ldg(a.slice_ptr + unit / L + 1); }
+    const auto in_slice = [&](int64_t u) { return (int)(u % L) * (32 / L) + lane / L; };
+    Quad<W, SETS, GLOBAL> cur, ahead;
+    if (q0 < q1) cur.load(a, (size_t)q0 * 32 + in_slice(unit));
     if constexpr (!GLOBAL) copy_in(smem, image, (uint32_t)a.image_bytes);
-    uint32_t place[S];
-#pragma unroll
-    for (int s = 0; s < S; ++s) place[s] = SWIZZLED ? unit_in_neuron(s, p, P) * 16u : (uint32_t)(s * UB);
     while (unit < last) {
-        const int64_t next = unit + kGatherThreads / 32;
+        const int64_t next = unit + WARPS;
         uint32_t n0 = 0, n1 = 0;
-        if (next < last) { n0 = __ldg(a.slice_ptr + next / P); n1 = __ldg(a.slice_ptr + next / P + 1); }
-        float acc[G][V];
+        if (next < last) { n0 = __ldg(a.slice_ptr + next / L); n1 = __ldg(a.slice_ptr + next / L + 1); }
+        float acc[G][NV * V];
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[g][k] = 0.0f;
-        Quad<W, SETS, GLOBAL> ahead;
-        if (q0 >= q1 && n0 < n1) cur.load(a, (size_t)n0 * 32 + lane_of(next));
-        for (uint32_t q = q0; q < q1; ++q) {
-            const bool inside = q + 1 < q1;
-            if (inside || n0 < n1) ahead.load(a, inside ? (size_t)(q + 1) * 32 + lane_of(unit) : (size_t)n0 * 32 + lane_of(next));
+            for (int k = 0; k < NV * V; ++k) acc[g][k] = 0.0f;
+        const auto work = [&](const Quad<W, SETS, GLOBAL> &quad) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    Raw<E, V> x;
+                for (int i = 0; i < NV; ++i) {
+                    Raw<E, V * (WHOLE ? 1 : S)> x[WHOLE ? S : 1];     // a neuron of few tokens: both values in one load
                     if constexpr (GLOBAL) {
-                        x.load(image + (((size_t)cur.index[k] * 16u) ^ place[s]));
-                    } else if constexpr (SWIZZLED) {
-                        const uint32_t w = cur.index[k >> 1];
-                        x.load(smem + (((k & 1 ? w >> 12 : w << 4) & 0xffff0u) ^ place[s]));
+#pragma unroll
+                        for (int s = 0; s < S; ++s) x[s].load(image + (((size_t)quad.index[k] * 16u) ^ ((uint32_t)(s * P + i * L + j) * 16u)));
                     } else {
-                        const uint32_t w = cur.index[k >> 1];
-                        x.load(smem + (k & 1 ? w >> 16 : w & 0xffffu) * (uint32_t)(S * UB) + place[s]);
+                        const uint32_t w = quad.index[k >> 1];
+                        if constexpr (WHOLE) {
+#pragma unroll
+                            for (int s = 0; s < S; ++s) x[s].load(smem + (((k & 1 ? w >> 12 : w << 4) & 0xffff0u) ^ ((uint32_t)(s * P + i * L + j) * 16u)));
+                        } else {
+                            x[0].load(smem + (k & 1 ? w >> 16 : w & 0xffffu) * (uint32_t)(S * UB));
+                        }
                     }
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const uint32_t w = cur.bits(k, S > 1 ? s : g);
+                    for (int s = 0; s < S; ++s)
 #pragma unroll
-                        for (int i = 0; i < V; ++i) acc[g][i] = fma_bits<E, W>(x.bits(i), w, acc[g][i]);
-                    }
+                        for (int g = 0; g < G; ++g) {
+                            const uint32_t w = quad.bits(k, S > 1 ? s : g);
+#pragma unroll
+                            for (int v = 0; v < V; ++v)
+                                acc[g][i * V + v] = fma_bits<E, W>(WHOLE ? x[WHOLE ? s : 0].bits(v) : x[0].bits(s * V + v), w, acc[g][i * V + v]);
+                        }
                 }
+        };
+        if (q0 < q1) {
+            size_t at = (size_t)q0 * 32 + in_slice(unit);
+            const size_t end = (size_t)(q1 - 1) * 32;
+#pragma unroll 2
+            for (; at < end; at += 32) {
+                ahead.load(a, at + 32);
+                work(cur);
+                cur = ahead;
             }
+            if (n0 < n1) ahead.load(a, (size_t)n0 * 32 + in_slice(next));
+            work(cur);
             cur = ahead;
+        } else if (n0 < n1) {
+            cur.load(a, (size_t)n0 * 32 + in_slice(next));
         }
-        const int c = (int)(unit / P) * 32 + lane_of(unit);
+        const int c = (int)(unit / L) * 32 + in_slice(unit);
         if (c < a.outs) {
             const float b0 = a.bias0 ? __ldg(a.bias0 + c) : 0.0f, b1 = G == 2 && a.bias1 ? __ldg(a.bias1 + c) : 0.0f;
-            const int64_t t0 = (int64_t)tile * (V * P) + p * V;
-            const int count = (int)min((int64_t)V, (int64_t)a.tokens - t0);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
+            for (int k = 0; k < NV * V; ++k) {
                 acc[0][k] += b0;
                 if (G == 2) acc[G - 1][k] += b1;
             }
-            if (a.z0) {
-                float *z = a.z0 + t0 * a.z_stride + c;
+            const int64_t t0 = (int64_t)tile * (V * P) + j * V;
+            // token k of the lane is t0 + (k / V) L V + k % V
+            const auto store = [&](auto *to, int64_t stride, const auto &value) {
+                to += t0 * stride + c;
+                const int left = (int)min((int64_t)(P * V), (int64_t)a.tokens - t0);
 #pragma unroll
-                for (int k = 0; k < V; ++k, z += a.z_stride)
-                    if (k < count) *z = acc[0][k];
-                if (G == 2) {
-                    z = a.z1 + t0 * a.z_stride + c;
+                for (int i = 0; i < NV; ++i) {
+                    if (left >= i * L * V + V) {
 #pragma unroll
-                    for (int k = 0; k < V; ++k, z += a.z_stride)
-                        if (k < count) *z = acc[G - 1][k];
+                        for (int v = 0; v < V; ++v) to[v * stride] = value(i * V + v);
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < V; ++v)
+                            if (i * L * V + v < left) to[v * stride] = value(i * V + v);
+                    }
+                    to += L * V * stride;
                 }
+            };
+            if (a.z0) {
+                store(a.z0, a.z_stride, [&](int k) { return acc[0][k]; });
+                if (G == 2) store(a.z1, a.z_stride, [&](int k) { return acc[G - 1][k]; });
             }
             if (S == 1) {
+                with_activation(a.act, [&](auto act) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    acc[0][k] = activate<sizeof(E) == 2>(acc[0][k], a.act, a.clip);
-                    if (G == 2) acc[0][k] *= acc[G - 1][k];
-                }
+                    for (int k = 0; k < NV * V; ++k) acc[0][k] = activate<sizeof(E) == 2>(acc[0][k], act.value, a.clip);
+                });
+                if (G == 2)
+#pragma unroll
+                    for (int k = 0; k < NV * V; ++k) acc[0][k] *= acc[G - 1][k];
             }
-            const int64_t at = t0 * a.y_stride + c;
-            if (a.y_type == F32) {
-                float *y = (float *)a.y + at;
-#pragma unroll
-                for (int k = 0; k < V; ++k, y += a.y_stride)
-                    if (k < count) *y = acc[0][k];
-            } else {
-                uint16_t *y = (uint16_t *)a.y + at;
-#pragma unroll
-                for (int k = 0; k < V; ++k, y += a.y_stride)
-                    if (k < count)
-                        *y = a.y_type == F16 ? __half_as_ushort(__float2half_rn(acc[0][k])) : __bfloat16_as_ushort(__float2bfloat16_rn(acc[0][k]));
-            }
+            if (a.y_type == F32) store((float *)a.y, a.y_stride, [&](int k) { return acc[0][k]; });
+            else if (a.y_type == F16) store((__half *)a.y, a.y_stride, [&](int k) { return __float2half_rn(acc[0][k]); });
+            else store((bf16 *)a.y, a.y_stride, [&](int k) { return __float2bfloat16_rn(acc[0][k]); });
         }
         unit = next; q0 = n0; q1 = n1;
     }

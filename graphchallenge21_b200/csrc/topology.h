@@ -7,8 +7,11 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
+#include <new>
 #include <string>
+#include <thread>
 #include <vector>
 
 namespace spdnn_impl {
@@ -40,7 +43,63 @@ struct Topology {
 constexpr int64_t kMostEntries = 1ll << 30;
 constexpr int kMostSlots = 4096;       // as canonicalize_layer
 
-// lists[i] = (row, source) pairs of gathering neuron i, through a callback that calls emit(row, source) in order
+// Orders the connections of 16 neighbouring neurons, whose lanes read their k-th connections at the same time, so that those fall on
+// different banks: of the sixteen (eight aligned, four, two) neurons the gathered rows should differ in the bits 0 to 3 (0 to 2, 0 and 1, 0)
+// of their numbers; spdnn_ffn.cuh says why.  Step by step and neuron by neuron the connection with the fewest meetings, of equals
+// one from the class (the four bits) that has most left.  Without it 2.1 wavefronts of shared memory a load where 1 would do.
+class BankOrder {
+public:
+    struct Entry { uint32_t row, source; };
+    std::vector<Entry> lists[16];      // of every neuron, in any order; run() puts them in the order of the steps
+    void run() {
+        size_t longest = 0;
+        for (int l = 0; l < 16; ++l) {
+            longest = std::max(longest, lists[l].size());
+            std::fill(left_[l], left_[l] + 16, 0);
+            for (const Entry &e : lists[l]) ++left_[l][e.row & 15];
+            uint32_t at = 0;
+            for (int c = 0; c < 16; ++c) { next_[l][c] = at; at += left_[l][c]; }
+            sorted_[l].resize(lists[l].size());
+            for (const Entry &e : lists[l]) sorted_[l][next_[l][e.row & 15]++] = e;
+            lists[l].clear();
+        }
+        for (size_t k = 0; k < longest; ++k) {
+            uint32_t pair[8][2] = {}, quad[4][4] = {}, oct[2][8] = {}, hex[16] = {};
+            for (int l = 0; l < 16; ++l) {
+                if (lists[l].size() + 1 > sorted_[l].size()) continue;
+                int best = -1;
+                uint32_t best_cost = 0;
+                for (int c = 0; c < 16; ++c) {
+                    const uint32_t meetings = hex[c] + oct[l / 8][c & 7] + quad[l / 4][c & 3] + pair[l / 2][c & 1];
+                    const uint32_t cost = 4096u * meetings + 4095u - std::min<uint32_t>(left_[l][c], 4095u);
+                    if (left_[l][c] && (best < 0 || cost < best_cost)) { best = c; best_cost = cost; }
+                }
+                ++hex[best]; ++oct[l / 8][best & 7]; ++quad[l / 4][best & 3]; ++pair[l / 2][best & 1];
+                --left_[l][best];
+                lists[l].push_back(sorted_[l][--next_[l][best]]);
+            }
+        }
+    }
+private:
+    std::vector<Entry> sorted_[16];
+    uint32_t left_[16][16], next_[16][16];
+};
+
+// Runs f(begin, end) over [0, n) in a few host threads (large topologies: 16384 neurons of 32 connections take 15 ms in one).
+template <class F>
+inline void in_threads(int n, int64_t work, const F &f) {
+    const int threads = (int)std::min<int64_t>(std::min<int64_t>(std::max(1u, std::thread::hardware_concurrency()), 8), work / 32768 + 1);
+    std::vector<std::thread> more;
+    int begun = 0;
+    try {
+        for (; begun + 1 < threads; ++begun) more.emplace_back(f, (int)((int64_t)n * begun / threads), (int)((int64_t)n * (begun + 1) / threads));
+    } catch (...) {                    // no more threads to be had: the rest is done here
+    }
+    f((int)((int64_t)n * begun / threads), n);
+    for (std::thread &t : more) t.join();
+}
+
+// lists(i, emit) calls emit(row, source) for the connections of gathering neuron i
 template <class Lists>
 inline std::string build_gather_table(int outs, int rows, const std::vector<uint32_t> &count, const Lists &lists, GatherTable &t) {
     t.outs = outs; t.rows = rows;
@@ -56,14 +115,27 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
     }
     t.idx.assign((size_t)quads * 128, (uint32_t)rows);
     t.src.assign((size_t)quads * 128, kNoSource);
-    for (int i = 0; i < outs; ++i) {
-        size_t at = (size_t)t.slice_ptr[i / 32] * 128 + (size_t)(i % 32) * 4;
-        int k = 0;
-        lists(i, [&](uint32_t row, uint32_t source) {
-            const size_t e = at + (size_t)(k / 4) * 128 + (k % 4);
-            t.idx[e] = row; t.src[e] = source; ++k;
-        });
-    }
+    std::atomic<bool> failed{false};
+    in_threads(slices * 2, quads * 128, [&](int begin, int end) {
+        try {
+            BankOrder order;
+            for (int group = begin; group < end; ++group) {
+                const int first = group * 16;
+                for (int l = 0; l < 16; ++l)
+                    if (first + l < outs) lists(first + l, [&](uint32_t row, uint32_t source) { order.lists[l].push_back({row, source}); });
+                order.run();
+                for (int l = 0; l < 16; ++l) {
+                    const size_t at = (size_t)t.slice_ptr[first / 32] * 128 + (size_t)((first + l) % 32) * 4;
+                    for (size_t k = 0; k < order.lists[l].size(); ++k) {
+                        const size_t e = at + k / 4 * 128 + k % 4;
+                        t.idx[e] = order.lists[l][k].row; t.src[e] = order.lists[l][k].source;
+                    }
+                    order.lists[l].clear();
+                }
+            }
+        } catch (...) { failed = true; }
+    });
+    if (failed) throw std::bad_alloc();
     return "";
 }
 
