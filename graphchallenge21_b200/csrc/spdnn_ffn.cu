@@ -145,6 +145,15 @@ GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int toke
     return g;
 }
 
+// How many neurons are read at a time by the gather that many tokens of `rows` neurons get (plan_gather), for the order of connections: the
+// image's bytes per neuron, and with them the lanes per neuron, do not depend on the type.  Fewer tokens may read more at a time.
+int neurons_at_a_time(int rows, int sets) {
+    int p = 8;
+    while (p > 1 && image_size(rows, sets, 8, p, 2) > kSharedLimit) p /= 2;
+    if (image_size(rows, sets, 8, p, 2) > kSharedLimit) return 16;
+    return 8 / (p / lane_units(p));
+}
+
 template <class E, class W, int S, int G>
 const void *gather_variant(const GatherPlan &g) {
     constexpr int F = 16 / (int)sizeof(E);
@@ -447,7 +456,8 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
     spdnn_topology *t = nullptr;
     try {
         t = new spdnn_topology();
-        const std::string why = build_topology(inputs, outputs, col_ptr, row_idx, t->host);
+        const std::string why = build_topology(inputs, outputs, col_ptr, row_idx, neurons_at_a_time(std::max(inputs, 1), 1),
+                                               neurons_at_a_time(std::max(outputs, 1), 2), t->host);
         if (!why.empty()) {
             delete t;
             return fail(err, err_len, SPDNN_ERR_ARG, why);
@@ -568,21 +578,26 @@ const char *check_mx4(const void *codes, const uint8_t *scales, int64_t rows, in
     return check_operand(m, rows, cols, false);
 }
 
-unsigned mx4_grid(int64_t groups) { return (unsigned)std::min<int64_t>((groups + kMx4Threads - 1) / kMx4Threads, 1 << 20); }
+unsigned mx4_grid(int64_t groups) { return (unsigned)std::min<int64_t>((groups + kMx4Threads * kMx4Batch - 1) / (kMx4Threads * kMx4Batch), 1 << 20); }
 
 template <class E>
 cudaError_t quantize(const spdnn_operand_t *x, int64_t rows, int cols, uint8_t *codes, uint8_t *scales, cudaStream_t stream) {
     const int blocks = (cols + 31) / 32;
-    const bool vector = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && x->stride * (int64_t)sizeof(E) % 16 == 0;
-    return launch(vector ? mx4_quantize_kernel<E, true> : mx4_quantize_kernel<E, false>, mx4_grid(rows * blocks * 4), kMx4Threads, stream,
-                  (const E *)x->data, x->stride, rows, cols, blocks, (uint32_t *)codes, scales);
+    const uintptr_t both = reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->stride * (int64_t)sizeof(E));
+    const auto kernel = both % 16 == 0  ? mx4_quantize_kernel<E, 16>
+                        : both % 8 == 0 ? mx4_quantize_kernel<E, 8>
+                        : both % 4 == 0 ? mx4_quantize_kernel<E, 4>
+                                        : mx4_quantize_kernel<E, (int)sizeof(E)>;
+    return launch(kernel, mx4_grid(rows * blocks * 4), kMx4Threads, stream, (const E *)x->data, x->stride, rows, cols, blocks, (uint32_t *)codes,
+                  scales);
 }
 
 template <class E>
 cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *y, cudaStream_t stream) {
     const int blocks = (cols + 31) / 32;
-    return launch(mx4_dequantize_kernel<E>, mx4_grid(rows * blocks * 4), kMx4Threads, stream, (const uint32_t *)codes, scales, rows, cols, blocks,
-                  (E *)const_cast<void *>(y->data), y->stride);
+    const bool vector = reinterpret_cast<uintptr_t>(y->data) % (4 * sizeof(E)) == 0 && y->stride % 4 == 0;
+    return launch(vector ? mx4_dequantize_kernel<E, true> : mx4_dequantize_kernel<E, false>, mx4_grid(rows * ((cols + 3) / 4)), kMx4Threads, stream,
+                  codes, scales, rows, cols, blocks, (E *)const_cast<void *>(y->data), y->stride);
 }
 
 }  // namespace

@@ -55,15 +55,21 @@ __device__ __forceinline__ void store_from_float(void *p, int type, int64_t at, 
     else ((bf16 *)p)[at] = __float2bfloat16_rn(v);
 }
 
-// E2M1: twice the magnitude of codes 0..7 is 0 1 2 3 4 6 8 12
+// E2M1 (sign, two bits of exponent, one of mantissa) shifted into the place of a float's exponent and mantissa is its value times
+// 2^-126, the subnormal code among them.
 __device__ __forceinline__ float e2m1_value(uint32_t code) {
-    const float m = 0.5f * (float)((0xC8643210u >> (4 * (code & 7u))) & 15u);
-    return (code & 8u) ? -m : m;
+    return __uint_as_float((code & 7u) << 22 | (code & 8u) << 28) * 0x1p126f;
 }
 
 // E8M0: 2^(byte - 127), 255 is NaN; 2^-127 is a subnormal float
 __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+}
+
+// The values of a word of codes, lowest half-byte first.
+template <int COUNT> __device__ __forceinline__ void e2m1_values(uint32_t word, float (&v)[COUNT]) {
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) v[k] = e2m1_value(word >> (4 * k));
 }
 
 // Element `col` of row `row` of a microscaled matrix: codes [rows][blocks][16], scales [rows][blocks].  The product with the
@@ -145,13 +151,18 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 }
 
 // Two values of a 32-bit word of a 16-bit type as a pair of floats (exact).
-template <class E> __device__ __forceinline__ f32x2 widen(uint32_t w);
+template <class E> __device__ __forceinline__ f32x2 widen(uint32_t w);        // 16-bit types only
 template <> __device__ __forceinline__ f32x2 widen<bf16>(uint32_t w) {
     return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 template <> __device__ __forceinline__ f32x2 widen<__half>(uint32_t w) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
     return pack2(f.x, f.y);
+}
+
+template <class E> __device__ __forceinline__ f32x2 widen_word(uint32_t w) {
+    if constexpr (sizeof(E) == 4) return 0;
+    else return widen<E>(w);
 }
 
 // V consecutive values of one neuron as pairs of floats (V = 1: one pair with a zero).
@@ -201,7 +212,21 @@ template <class E, int V> struct Raw {
         if constexpr (sizeof(E) == 4) return w[i];
         else return i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (kBytes + 3) / 4; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void set(int i, E v) {        // of a cleared one
+        if constexpr (sizeof(E) == 4) w[i] = __float_as_uint(v);
+        else w[i >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t *>(&v) << (16 * (i & 1));
+    }
 };
+
+template <class E> __device__ __forceinline__ float bits_to_float(uint32_t b) {
+    if constexpr (sizeof(E) == 4) return __uint_as_float(b);
+    else if constexpr (std::is_same<E, bf16>::value) return __uint_as_float(b << 16);
+    else return __half2float(__ushort_as_half((uint16_t)b));
+}
 
 // c + a b in float32, from the bits of a and b.  Two operands of one 16-bit type go into the mixed-precision fma as they are: exact
 // product, one rounding, and none of the conversions (two per pair of values) that took a third of the inner loop.
@@ -226,9 +251,9 @@ template <class E, class W> __device__ __forceinline__ float fma_bits(uint32_t a
 // An image: rows + 1 neurons (the last one zeros) x SETS values x T = V P tokens, in UNITS of V tokens (16 bytes, or less where a
 // neuron's tokens are fewer).  A neuron has R = SETS P units in a row; unit u = s P + p of neuron n lies at n R + (u ^ x(n)).  x
 // turns the units of neighbouring neurons against each other, so that the bank group of unit 0 (16 bytes, 8 of them) is made of the three
-// low bits of n whatever R is: of bits 0 and 1 and 2 for its highest and middle and lowest bit (R = 2: 1, 0, 2).  So L = 4, 2 or 1 lanes
-// that read a neuron together meet no other neuron's lanes if those neurons differ in bit 0, in bits 0 and 1, in bits 0 to 2;
-// neurons of 8 bytes meet none of sixteen that differ in the bits 0 to 3.  That is what topology.h orders connections by.
+// low bits of n whatever R is: of bits 0 and 1 and 2 for its highest and middle and lowest bit (R = 2: 1, 0, 2).  Eight lanes are served
+// at a time (16 of 8 bytes).  So where L = 4, 2 or 1 lanes read a neuron together, the 2, 4 or 8 neurons of eight lanes do not meet if
+// they differ modulo 2, 4 or 8, and sixteen neurons of 8 bytes if they do modulo 16: what topology.h orders connections by.
 __host__ __device__ __forceinline__ uint32_t image_units(int rows, int per_row) { return ((uint32_t)(rows + 1) * per_row + 7u) & ~7u; }
 __host__ __device__ __forceinline__ uint32_t unit_place(uint32_t n, uint32_t per_row) {
     const uint32_t reversed = (n & 1u) << 2 | (n & 2u) | (n >> 2 & 1u);
@@ -265,12 +290,11 @@ __device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int6
     if (x.type == MX4) {
         const int64_t b = row * x.stride + (col >> 5);
         const float scale = e8m0_value(__ldg(x.scales + b));
+        const uint8_t *from = (const uint8_t *)x.data + b * 16 + ((col & 31) >> 1);
+        float e[COUNT];
+        e2m1_values(COUNT == 8 ? __ldg((const uint32_t *)from) : __ldg((const uint16_t *)from), e);
 #pragma unroll
-        for (int k = 0; k < COUNT; k += 2) {
-            const uint32_t byte = __ldg((const uint8_t *)x.data + b * 16 + (((col & 31) + k) >> 1));
-            v[k] = col + k < cols ? e2m1_value(byte & 15u) * scale : 0.0f;
-            v[k + 1] = col + k + 1 < cols ? e2m1_value(byte >> 4) * scale : 0.0f;
-        }
+        for (int k = 0; k < COUNT; ++k) v[k] = col + k < cols ? e[k] * scale : 0.0f;
         return;
     }
     if (vector && col + COUNT <= cols) {
@@ -295,6 +319,26 @@ __device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int6
     }
 #pragma unroll
     for (int k = 0; k < COUNT; ++k) v[k] = col + k < cols ? load_as_float(x.data, x.type, row * x.stride + col + k) : 0.0f;
+}
+
+// The units of fewer than 16 bytes of a block's neurons: 16 bytes at a time.  (An image is whole groups of 16 bytes, and so is what the
+// 64 neurons before n0 take.)
+template <class E, int SETS, int V, class Tile, class At>
+__device__ __forceinline__ void small_units(char *image, int64_t image_bytes, int parts, const Tile &tile, const At &at, int n0, int n_end,
+                                            uint32_t units, int rows) {
+    constexpr int N = 16 / (int)sizeof(E);
+    const int first = (int)((uint32_t)n0 * SETS * V / N);
+    const int here = (int)(min((uint32_t)(n0 + n_end) * SETS, units) * V / N) - first;
+    for (int i = threadIdx.x; i < parts * here; i += kPackThreads) {
+        const int part = i / here, g = first + i - part * here;
+        E e[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int q = (g * N + k) / V, n = q / SETS - n0, s = q % SETS;
+            e[k] = from_float<E>(n < 64 && n0 + n < rows ? to_float(tile[s][n & 63][at(n & 63, part * V + k % V)]) : 0.0f);
+        }
+        ((uint4 *)(image + part * image_bytes))[g] = *(const uint4 *)e;
+    }
 }
 
 // One block: 64 neurons x 64 tokens, through shared memory so that reads run along neurons and writes along tokens.  The tokens of a
@@ -349,33 +393,32 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackArgs a) {
         const int64_t tiles = ((int64_t)a.tokens + T - 1) / T;
         // the last block along n also writes the row of zeros and the units behind it
         const int n_end = n0 + 64 >= a.rows ? (int)((units + per_row - 1) / per_row) - n0 : 64;
-        for (int part = 0; part * T < 64; ++part) {
-            const int64_t tile_index = (t0 + part * T) / T;
-            if (tile_index >= tiles) break;
-            char *image = (char *)a.image + tile_index * a.image_bytes;
-            for (int i = threadIdx.x; i < n_end * per_row; i += kPackThreads) {
-                const int p = i & (a.p - 1), s = (i >> log_p) & (SETS - 1), n = (i >> log_p) / SETS;
-                const uint32_t q = (uint32_t)n0 * per_row + i;
-                if (q >= units) break;
-                const bool real = n < 64 && n0 + n < a.rows;
-                const int t = part * T + p * a.v;
-                if (a.v == N) {
-                    uint4 r = make_uint4(0, 0, 0, 0);
-                    if (real) {
-                        if constexpr (!GRADIENT || sizeof(E) == 4) {
-                            r = *(const uint4 *)&tile[s][n][at(n, t)];
-                        } else {
-                            const float4 lo = *(const float4 *)&tile[s][n][at(n, t)], hi = *(const float4 *)&tile[s][n][at(n, t + 4)];
-                            E e[8] = {from_float<E>(lo.x), from_float<E>(lo.y), from_float<E>(lo.z), from_float<E>(lo.w),
-                                      from_float<E>(hi.x), from_float<E>(hi.y), from_float<E>(hi.z), from_float<E>(hi.w)};
-                            r = *(const uint4 *)e;
-                        }
+        const int64_t tile0 = t0 / T;
+        const int parts = (int)min((int64_t)(64 / T), tiles - tile0);
+        if (a.v == N) {
+            const int units_here = min(n_end * per_row, (int)(units - (uint32_t)n0 * per_row));
+            for (int i = threadIdx.x; i < parts * units_here; i += kPackThreads) {
+                const int part = i / units_here, u = i - part * units_here;
+                const int p = u & (a.p - 1), s = (u >> log_p) & (SETS - 1), n = (u >> log_p) / SETS;
+                const int t = part * T + p * N;
+                uint4 r = make_uint4(0, 0, 0, 0);
+                if (n < 64 && n0 + n < a.rows) {
+                    if constexpr (!GRADIENT || sizeof(E) == 4) {
+                        r = *(const uint4 *)&tile[s][n][at(n, t)];
+                    } else {
+                        const float4 lo = *(const float4 *)&tile[s][n][at(n, t)], hi = *(const float4 *)&tile[s][n][at(n, t + 4)];
+                        E e[8] = {from_float<E>(lo.x), from_float<E>(lo.y), from_float<E>(lo.z), from_float<E>(lo.w),
+                                  from_float<E>(hi.x), from_float<E>(hi.y), from_float<E>(hi.z), from_float<E>(hi.w)};
+                        r = *(const uint4 *)e;
                     }
-                    ((uint4 *)image)[unit_place(n0 + n, per_row) ^ (uint32_t)(s * a.p + p)] = r;
-                } else {
-                    for (int k = 0; k < a.v; ++k) ((E *)image)[(size_t)q * a.v + k] = from_float<E>(real ? to_float(tile[s][n & 63][at(n & 63, t + k)]) : 0.0f);
                 }
+                ((uint4 *)((char *)a.image + (tile0 + part) * a.image_bytes))[unit_place(n0 + n, per_row) ^ (uint32_t)(s * a.p + p)] = r;
             }
+        } else {
+            char *image = (char *)a.image + tile0 * a.image_bytes;
+            if (a.v == 1) small_units<E, SETS, 1>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
+            else if (a.v == 2) small_units<E, SETS, 2>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
+            else small_units<E, SETS, (N > 4 ? 4 : 2)>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
         }
     }
     if (a.columns) {
@@ -644,19 +687,37 @@ struct DwArgs {
 constexpr int kDwSlots = 16;
 constexpr int kDwThreads = 128;
 
+// Sums of `COUNT` (16 or 32) values over the lanes of a warp: lane l returns that of value l mod COUNT.  Every exchange halves the values a
+// lane still holds, so it takes COUNT - 1 shuffles (and one) instead of five for each.
+template <int COUNT> __device__ __forceinline__ float sum_lanes(float (&v)[COUNT]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = COUNT / 2; s; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < s; ++i) {
+            const bool upper = lane & s;
+            const float send = upper ? v[i] : v[i + s], keep = upper ? v[i + s] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+        }
+    if (COUNT == 16) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
+    return v[0];
+}
+
 // A warp owns kDwSlots connections of one output: every lane sums its tokens' products in registers, the lanes are joined at the
-// end.  Adjacent warps take adjacent outputs, whose inputs are often the same rows (blocks of a butterfly).
+// end.  Adjacent warps take adjacent outputs, whose inputs are often the same rows (blocks of a butterfly).  What bounds it is bringing
+// the rows from L2, so the loads of several are in flight before the first is used.  A connection that is not there reads row 0 (or, in the
+// lanes behind the last token, any row's first tokens with a gradient of zero) and its sum is dropped.
 template <class E, int G>
 __global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
     constexpr int V = 16 / sizeof(E);
     constexpr int PAIRS = V / 2;
+    constexpr int BATCH = 4;
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * (kDwThreads / 32) + (threadIdx.x >> 5);
     const int c = (int)(unit % a.outputs), chunk = (int)(unit / a.outputs);
     if (chunk >= a.chunks) return;
     const int j0 = chunk * kDwSlots, slots = min(kDwSlots, a.slots - j0);
-    const int32_t *rows = a.rows + (int64_t)c * a.slots + j0;
-    const int mine = lane < slots ? __ldg(rows + lane) : -1;
+    const int mine = lane < slots ? __ldg(a.rows + (int64_t)c * a.slots + j0 + lane) : -1;
     f32x2 acc[kDwSlots][G], bias[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) bias[g] = 0;
@@ -668,11 +729,11 @@ __global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
     const E *x = (const E *)a.x;
     const float *d = a.d + (int64_t)c * G * a.token_stride;
     for (int64_t t0 = 0; t0 < a.token_stride; t0 += 32 * V) {
-        const int64_t t = t0 + lane * V;
-        const bool inside = t < a.token_stride;
+        const bool inside = t0 + lane * V < a.token_stride;
+        const int64_t t = inside ? t0 + lane * V : 0;
         f32x2 dv[G][PAIRS];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int i = 0; i < PAIRS; i += 2) {
                 Values<float, 4> part;
@@ -681,45 +742,51 @@ __global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
                 dv[g][i] = part.v[0]; dv[g][i + 1] = part.v[1];
             }
 #pragma unroll
-            for (int i = 0; i < PAIRS; ++i) bias[g] = fma2(dv[g][i], ones, bias[g]);
-        }
+        for (int j = 0; j < kDwSlots; j += BATCH) {
+            Raw<E, V> raw[BATCH];
 #pragma unroll
-        for (int j = 0; j < kDwSlots; ++j) {
-            const int row = __shfl_sync(0xffffffffu, mine, j);
-            if (row >= 0) {
-                Values<E, V> xv;
-                xv.zero();
-                if (inside) xv.load(x + (int64_t)row * a.token_stride + t);
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-#pragma unroll
-                    for (int i = 0; i < PAIRS; ++i) acc[j][g] = fma2(xv.v[i], dv[g][i], acc[j][g]);
+            for (int k = 0; k < BATCH; ++k) {
+                const int row = max(__shfl_sync(0xffffffffu, mine, j + k), 0);
+                raw[k].load(x + (int64_t)row * a.token_stride + t);
             }
-        }
-    }
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        float *out = (g ? a.dw1 : a.dw0) + (int64_t)c * a.slots + j0;
-        float keep = 0.0f;
+            for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                for (int i = 0; i < PAIRS; ++i) {
+                    const f32x2 xv = sizeof(E) == 4 ? pack2(__uint_as_float(raw[k].bits(2 * i)), __uint_as_float(raw[k].bits(2 * i + 1)))
+                                                    : widen_word<E>(raw[k].w[i]);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) acc[j + k][g] = fma2(xv, dv[g][i], acc[j + k][g]);
+                }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) bias[g] = fma2(dv[g][i], ones, bias[g]);
+    }
+    float sums[kDwSlots * G];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int j = 0; j < kDwSlots; ++j) {
             float lo, hi;
             unpack2(acc[j][g], lo, hi);
-            float v = lo + hi;
-#pragma unroll
-            for (int s = 16; s; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-            if (lane == j) keep = v;
+            sums[g * kDwSlots + j] = lo + hi;
         }
-        if (lane < slots) out[lane] = keep;
-        float *db = g ? a.db1 : a.db0;
-        if (chunk == 0 && db) {
-            float lo, hi;
-            unpack2(bias[g], lo, hi);
-            float v = lo + hi;
+    const float sum = sum_lanes(sums);
+    const int j = lane & 15, g = lane >> 4;
+    const int row = __shfl_sync(0xffffffffu, mine, j);
+    if (g < G && j < slots) (g ? a.dw1 : a.dw0)[(int64_t)c * a.slots + j0 + j] = row >= 0 ? sum : 0.0f;
+    if (chunk) return;
 #pragma unroll
-            for (int s = 16; s; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-            if (lane == 0) db[c] = v;
-        }
+    for (int s = 0; s < G; ++s) {
+        float lo, hi;
+        unpack2(bias[s], lo, hi);
+        float v = lo + hi;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+        float *db = s ? a.db1 : a.db0;
+        if (lane == 0 && db) db[c] = v;
     }
 }
 

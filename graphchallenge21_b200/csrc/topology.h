@@ -43,46 +43,99 @@ struct Topology {
 constexpr int64_t kMostEntries = 1ll << 30;
 constexpr int kMostSlots = 4096;       // as canonicalize_layer
 
-// Orders the connections of 16 neighbouring neurons, whose lanes read their k-th connections at the same time, so that those fall on
-// different banks: of the sixteen (eight aligned, four, two) neurons the gathered rows should differ in the bits 0 to 3 (0 to 2, 0 and 1, 0)
-// of their numbers; spdnn_ffn.cuh says why.  Step by step and neuron by neuron the connection with the fewest meetings, of equals
-// one from the class (the four bits) that has most left.  Without it 2.1 wavefronts of shared memory a load where 1 would do.
+// Orders the connections of `lanes` (2, 4, 8 or 16) neighbouring neurons, whose lanes read their k-th connections at the same time, so
+// that those fall on different banks: into steps in which the gathered rows belong to different CLASSES, row mod `lanes` (spdnn_ffn.cuh
+// says why these).  Every neuron has a connection in every step, so as long as no class has more connections left than there are
+// steps, a matching of neurons to classes exists in which no class occurs twice (an edge colouring of the bipartite multigraph
+// of neurons and classes); where one has more, steps in which classes occur twice take the surplus off all such
+// classes at once.  Of a random topology (8 lanes, 32 connections) that leaves 1.25 wavefronts per load of eight lanes, 2.6 in any order.
 class BankOrder {
 public:
     struct Entry { uint32_t row, source; };
+    explicit BankOrder(int lanes) : lanes_(lanes) {}
     std::vector<Entry> lists[16];      // of every neuron, in any order; run() puts them in the order of the steps
     void run() {
-        size_t longest = 0;
-        for (int l = 0; l < 16; ++l) {
-            longest = std::max(longest, lists[l].size());
-            std::fill(left_[l], left_[l] + 16, 0);
-            for (const Entry &e : lists[l]) ++left_[l][e.row & 15];
-            uint32_t at = 0;
-            for (int c = 0; c < 16; ++c) { next_[l][c] = at; at += left_[l][c]; }
+        int steps = 0;
+        std::fill(total_, total_ + lanes_, 0);
+        for (int l = 0; l < lanes_; ++l) {
+            steps = std::max(steps, (int)lists[l].size());
+            std::fill(left_[l], left_[l] + lanes_, 0);
+            for (const Entry &e : lists[l]) ++left_[l][e.row & (lanes_ - 1)];
+            int at = 0;
+            for (int c = 0; c < lanes_; ++c) { next_[l][c] = at; at += left_[l][c]; total_[c] += left_[l][c]; }
             sorted_[l].resize(lists[l].size());
-            for (const Entry &e : lists[l]) sorted_[l][next_[l][e.row & 15]++] = e;
+            for (const Entry &e : lists[l]) sorted_[l][next_[l][e.row & (lanes_ - 1)]++] = e;
             lists[l].clear();
         }
-        for (size_t k = 0; k < longest; ++k) {
-            uint32_t pair[8][2] = {}, quad[4][4] = {}, oct[2][8] = {}, hex[16] = {};
-            for (int l = 0; l < 16; ++l) {
-                if (lists[l].size() + 1 > sorted_[l].size()) continue;
-                int best = -1;
-                uint32_t best_cost = 0;
-                for (int c = 0; c < 16; ++c) {
-                    const uint32_t meetings = hex[c] + oct[l / 8][c & 7] + quad[l / 4][c & 3] + pair[l / 2][c & 1];
-                    const uint32_t cost = 4096u * meetings + 4095u - std::min<uint32_t>(left_[l][c], 4095u);
-                    if (left_[l][c] && (best < 0 || cost < best_cost)) { best = c; best_cost = cost; }
+        for (; steps > 0; --steps) {
+            int by_total[16];
+            for (int c = 0; c < lanes_; ++c) by_total[c] = c;
+            std::sort(by_total, by_total + lanes_, [&](int x, int y) { return total_[x] != total_[y] ? total_[x] > total_[y] : x < y; });
+            std::fill(class_of_, class_of_ + 16, -1);
+            std::fill(used_, used_ + 16, 0);
+            cap_ = total_[by_total[0]] > steps ? 2 : 1;
+            // classes without slack first: they must occur in this step (twice where they have a surplus) ...
+            for (int i = 0; i < lanes_ && total_[by_total[i]] >= steps; ++i)
+                for (int k = total_[by_total[i]] > steps ? 2 : 1; k > 0; --k) {
+                    std::fill(seen_, seen_ + 16, false);
+                    if (!give_class(by_total[i])) break;
                 }
-                ++hex[best]; ++oct[l / 8][best & 7]; ++quad[l / 4][best & 3]; ++pair[l / 2][best & 1];
-                --left_[l][best];
-                lists[l].push_back(sorted_[l][--next_[l][best]]);
+            // ... then every neuron a class; where none is free, the least used of its own
+            for (int l = 0; l < lanes_; ++l) {
+                if (class_of_[l] >= 0 || lists[l].size() == sorted_[l].size()) continue;
+                std::fill(seen_, seen_ + 16, false);
+                if (!give_neuron(l, by_total)) {
+                    int best = -1;
+                    for (int i = 0; i < lanes_; ++i) {
+                        const int c = by_total[i];
+                        if (left_[l][c] && (best < 0 || used_[c] < used_[best])) best = c;
+                    }
+                    class_of_[l] = best; ++used_[best];
+                }
+            }
+            for (int l = 0; l < lanes_; ++l) {
+                const int c = class_of_[l];
+                if (c < 0) continue;
+                --left_[l][c]; --total_[c];
+                lists[l].push_back(sorted_[l][--next_[l][c]]);
             }
         }
     }
 private:
+    // augmenting paths; a neuron or class that was served stays served
+    bool give_class(int c) {
+        for (int l = 0; l < lanes_; ++l)
+            if (class_of_[l] < 0 && left_[l][c]) { class_of_[l] = c; ++used_[c]; return true; }
+        seen_[c] = true;
+        for (int l = 0; l < lanes_; ++l) {
+            const int other = class_of_[l];
+            if (other < 0 || seen_[other] || !left_[l][c]) continue;
+            if (!give_class(other)) continue;          // another neuron takes `other` on
+            --used_[other]; class_of_[l] = c; ++used_[c];
+            return true;
+        }
+        return false;
+    }
+    bool give_neuron(int l, const int *order) {
+        for (int i = 0; i < lanes_; ++i)
+            if (left_[l][order[i]] && used_[order[i]] < cap_) { class_of_[l] = order[i]; ++used_[order[i]]; return true; }
+        for (int i = 0; i < lanes_; ++i) {
+            const int c = order[i];
+            if (!left_[l][c] || seen_[c]) continue;
+            seen_[c] = true;
+            for (int m = 0; m < lanes_; ++m) {
+                if (class_of_[m] != c) continue;
+                if (!give_neuron(m, order)) continue;  // it moved to another class and left its place in this one
+                --used_[c]; class_of_[l] = c; ++used_[c];
+                return true;
+            }
+        }
+        return false;
+    }
+    int lanes_, cap_ = 1;
     std::vector<Entry> sorted_[16];
-    uint32_t left_[16][16], next_[16][16];
+    int left_[16][16], next_[16][16], total_[16], class_of_[16], used_[16];
+    bool seen_[16];
 };
 
 // Runs f(begin, end) over [0, n) in a few host threads (large topologies: 16384 neurons of 32 connections take 15 ms in one).
@@ -99,9 +152,9 @@ inline void in_threads(int n, int64_t work, const F &f) {
     for (std::thread &t : more) t.join();
 }
 
-// lists(i, emit) calls emit(row, source) for the connections of gathering neuron i
+// lists(i, emit) calls emit(row, source) for the connections of gathering neuron i; lanes: see BankOrder
 template <class Lists>
-inline std::string build_gather_table(int outs, int rows, const std::vector<uint32_t> &count, const Lists &lists, GatherTable &t) {
+inline std::string build_gather_table(int outs, int rows, const std::vector<uint32_t> &count, const Lists &lists, int lanes, GatherTable &t) {
     t.outs = outs; t.rows = rows;
     const int slices = (outs + 31) / 32;
     t.slice_ptr.assign((size_t)slices + 1, 0);
@@ -116,15 +169,15 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
     t.idx.assign((size_t)quads * 128, (uint32_t)rows);
     t.src.assign((size_t)quads * 128, kNoSource);
     std::atomic<bool> failed{false};
-    in_threads(slices * 2, quads * 128, [&](int begin, int end) {
+    in_threads(slices * 32 / lanes, quads * 128, [&](int begin, int end) {
         try {
-            BankOrder order;
+            BankOrder order(lanes);
             for (int group = begin; group < end; ++group) {
-                const int first = group * 16;
-                for (int l = 0; l < 16; ++l)
+                const int first = group * lanes;
+                for (int l = 0; l < lanes; ++l)
                     if (first + l < outs) lists(first + l, [&](uint32_t row, uint32_t source) { order.lists[l].push_back({row, source}); });
                 order.run();
-                for (int l = 0; l < 16; ++l) {
+                for (int l = 0; l < lanes; ++l) {
                     const size_t at = (size_t)t.slice_ptr[first / 32] * 128 + (size_t)((first + l) % 32) * 4;
                     for (size_t k = 0; k < order.lists[l].size(); ++k) {
                         const size_t e = at + k / 4 * 128 + k % 4;
@@ -140,7 +193,9 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
 }
 
 // Returns an empty string on success, else the reason the topology is rejected.
-inline std::string build_topology(int inputs, int outputs, const int32_t *col_ptr, const int32_t *row_idx, Topology &t) {
+// forward_lanes, backward_lanes: see BankOrder.
+inline std::string build_topology(int inputs, int outputs, const int32_t *col_ptr, const int32_t *row_idx, int forward_lanes, int backward_lanes,
+                                  Topology &t) {
     if (inputs <= 0 || outputs <= 0 || inputs >= (1 << 26) || outputs >= (1 << 26)) return "inputs and outputs must be in [1, 2^26)";
     if (!col_ptr) return "col_ptr is null";
     if (col_ptr[0] != 0) return "col_ptr[0] must be 0";
@@ -175,7 +230,7 @@ inline std::string build_topology(int inputs, int outputs, const int32_t *col_pt
     std::string why = build_gather_table(outputs, inputs, in_count, [&](int c, auto emit) {
         const int32_t *r = t.rows.data() + (size_t)c * most;
         for (uint32_t k = 0; k < in_count[c]; ++k) emit((uint32_t)r[k], (uint32_t)((size_t)c * most + k));
-    }, t.forward);
+    }, forward_lanes, t.forward);
     if (!why.empty()) return why;
     // the transposed lists, outputs ascending
     std::vector<size_t> start((size_t)inputs + 1, 0);
@@ -189,7 +244,7 @@ inline std::string build_topology(int inputs, int outputs, const int32_t *col_pt
         }
     return build_gather_table(inputs, outputs, out_count, [&](int i, auto emit) {
         for (size_t e = start[i]; e < start[i + 1]; ++e) emit(by_input[e] / (uint32_t)most, by_input[e]);
-    }, t.backward);
+    }, backward_lanes, t.backward);
 }
 
 }  // namespace spdnn_impl
