@@ -36,7 +36,8 @@ struct spdnn_topology {
     int device = -1;                // -1: analysis only
     int sm_count = 0;
     DeviceTable forward, backward;
-    int32_t *rows = nullptr;
+    int32_t *rows = nullptr;        // canonical
+    void *few_rows = nullptr;       // canonical as few_kernel reads them
 };
 
 namespace {
@@ -95,6 +96,23 @@ void release(DeviceTable &d) {
     d = DeviceTable();
 }
 
+int few_stride(int slots) { return (slots + 3) / 4 * 4; }
+
+template <class T>
+cudaError_t upload_few_rows(spdnn_topology &top, T **to) {
+    const int stride = few_stride(top.host.slots);
+    std::vector<T> rows((size_t)top.host.outputs * stride, (T)top.host.inputs);
+    for (int c = 0; c < top.host.outputs; ++c)
+        for (int k = 0; k < top.host.slots; ++k) {
+            const int32_t r = top.host.rows[(size_t)c * top.host.slots + k];
+            if (r >= 0) rows[(size_t)c * stride + k] = (T)r;
+        }
+    return upload(to, rows);
+}
+cudaError_t upload_few_rows(spdnn_topology &top) {
+    return top.host.inputs < 65536 ? upload_few_rows(top, (uint16_t **)&top.few_rows) : upload_few_rows(top, (int32_t **)&top.few_rows);
+}
+
 int type_size(int type) { return type == F32 ? 4 : 2; }
 bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
 int64_t aligned(int64_t n) { return (n + 255) & ~255ll; }
@@ -107,6 +125,9 @@ struct GatherPlan {
 };
 
 constexpr int64_t kSharedLimit = 227 * 1024;
+#ifndef SPDNN_FEW
+#define SPDNN_FEW 16
+#endif
 
 int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
@@ -134,13 +155,14 @@ GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int toke
     const int64_t per_sm = g.global ? 2 : std::max<int64_t>(1, std::min<int64_t>(2, kSharedLimit / (g.image_bytes + 1024)));
     const int64_t slots = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * (g.p / lane_units(g.p));
     // Blocks of a tile: clocks of a wave of blocks are those of the image (about 40 bytes a clock) and of the block's units (a
-    // connection of 32 lanes about 8 clocks of the SM); the fewest in all waves.
+    // connection of 32 lanes about 8 clocks of the SM); the fewest in all waves, of the splits that fill 1 to 16 waves.
     const double per_unit = 8.0 * lane_units(g.p) * std::max<double>(1.0, (double)t.entries / 32.0 / std::max<int64_t>(1, (t.outs + 31) / 32)) / per_sm;
     double best = 0.0;
-    for (int64_t s = 1; s <= 2 * slots && (s == 1 || s * 16 <= units); ++s) {
+    for (int64_t w = 0; w <= 16; ++w) {
+        const int64_t s = std::max<int64_t>(1, std::min<int64_t>(w * slots / g.tiles, units / 16));
         const int64_t waves = (g.tiles * s + slots - 1) / slots;
         const double cost = waves * ((g.global ? 0.0 : g.image_bytes / 40.0) + 1000.0 + (double)((units + s - 1) / s) * per_unit);
-        if (s == 1 || cost < best) { best = cost; g.splits = (int)s; }
+        if (w == 0 || cost < best) { best = cost; g.splits = (int)s; }
     }
     return g;
 }
@@ -308,8 +330,9 @@ int check_call(const Call &c, bool backward) {
     return SPDNN_OK;
 }
 
+constexpr const char *kAnalysisOnly = "the topology was created for analysis only (device -1)";
+
 int check_run(const Call &c, int64_t need) {
-    if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, "the topology was created for analysis only (device -1)");
     if (!c.workspace || c.workspace_bytes < need)
         return fail(c.err, c.err_len, SPDNN_ERR_ARG, "the workspace is smaller than spdnn_layer_workspace asks for: " + std::to_string(need) + " bytes");
     if (reinterpret_cast<uintptr_t>(c.workspace) % 256) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "the workspace must be aligned to 256 bytes");
@@ -321,6 +344,60 @@ int check_blocks(const Call &c, const GatherPlan &g) {
     if (pack > 0x7fffffffll || g.tiles * g.splits > 0x7fffffffll)
         return fail(c.err, c.err_len, SPDNN_ERR_LIMIT, "tokens times neurons is too large for one call: split the tokens");
     return SPDNN_OK;
+}
+
+// Tokens that one launch of few_kernel takes at a time, or 0: the images' way.
+int few_tokens(const spdnn_topology &top, int tokens, int x_type) {
+    const int64_t row = (int64_t)(top.host.inputs + 1) * type_size(image_type(x_type));
+    if (tokens > SPDNN_FEW) return 0;
+    int T = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
+    if (x_type == F32) T = std::min(T, 4);
+    while (T > 1 && row * T > kSharedLimit / 2) T /= 2;
+    return row * T <= kSharedLimit && (tokens + T - 1) / T <= 4 ? T : 0;
+}
+
+template <class E, class W, bool MX, int G>
+const void *few_variant(int T) {
+    switch (T) {
+        case 1: return (const void *)few_kernel<E, W, MX, 1, G>;
+        case 2: return (const void *)few_kernel<E, W, MX, 2, G>;
+        case 4: return (const void *)few_kernel<E, W, MX, 4, G>;
+        default:
+            if constexpr (sizeof(E) == 2) return (const void *)few_kernel<E, W, MX, 8, G>;
+            else return nullptr;
+    }
+}
+
+cudaError_t launch_few(const Call &c, int T, const float *b0, const float *b1) {
+    const Topology &h = c.top->host;
+    FewArgs a{};
+    a.x = matrix(c.x); a.w0 = matrix(c.w[0]); a.w1 = matrix(c.w[1]);
+    a.rows = c.top->few_rows; a.row_stride = few_stride(h.slots); a.slots = h.slots; a.inputs = h.inputs; a.outputs = h.outputs; a.tokens = c.tokens;
+    a.bias0 = b0; a.bias1 = b1;
+    a.y = const_cast<void *>(c.y->data); a.y_stride = c.y->stride; a.y_type = c.y->type; a.act = c.act; a.clip = c.clip;
+    if (c.z[0]) { a.z0 = (float *)const_cast<void *>(c.z[0]->data); a.z_stride = c.z[0]->stride; }
+    if (c.z[1]) a.z1 = (float *)const_cast<void *>(c.z[1]->data);
+    a.vector_x = on_16_bytes(c.x);
+    a.vector_w = 1;
+    for (int s = 0; s < c.sets; ++s)
+        a.vector_w &= reinterpret_cast<uintptr_t>(c.w[s]->data) % (4 * type_size(c.w[s]->type)) == 0 && c.w[s]->stride % 4 == 0;
+    const int it = image_type(c.x->type), w = c.w[0]->type;
+    const auto of = [&](auto e) {
+        using E = decltype(e);
+        if (w == MX4) return c.sets == 2 ? few_variant<E, bf16, true, 2>(T) : few_variant<E, bf16, true, 1>(T);
+        return c.sets == 2 ? few_variant<E, E, false, 2>(T) : few_variant<E, E, false, 1>(T);
+    };
+    const void *kernel = it == F32 ? of(float()) : it == F16 ? of(__half()) : of(bf16());
+    const size_t shared = (size_t)(h.inputs + 1) * T * type_size(it);
+    if (shared > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t want = (h.outputs + kFewThreads / 8 - 1) / (kFewThreads / 8);
+    const int per_sm = shared > (size_t)kSharedLimit / 4 ? 1 : 4;
+    void *args[] = {&a};
+    return cudaLaunchKernel(kernel, dim3((unsigned)std::min<int64_t>(want, (int64_t)per_sm * c.top->sm_count), (unsigned)((c.tokens + T - 1) / T)),
+                            dim3(kFewThreads), args, shared, c.stream);
 }
 
 int run_forward(const Call &c, const float *b0, const float *b1) {
@@ -336,7 +413,13 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     if (!bad && c.sets == 2 && !c.z[0] != !c.z[1]) bad = "save both pre-activations or none";
     if (!bad && c.sets == 2 && c.z[0] && c.z[0]->stride != c.z[1]->stride) bad = "both pre-activations must have one stride";
     if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
-    if (c.tokens == 0 && c.top->device >= 0) return SPDNN_OK;
+    if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, kAnalysisOnly);
+    if (c.tokens == 0) return SPDNN_OK;
+    if (const int T = few_tokens(*c.top, c.tokens, c.x->type)) {
+        OnDevice guard(c.top->device);
+        const cudaError_t e = guard.status == cudaSuccess ? launch_few(c, T, b0, b1) : guard.status;
+        return e == cudaSuccess ? SPDNN_OK : fail_cuda(c.err, c.err_len, e);
+    }
     const DeviceTable &t = c.top->forward;
     const int it = image_type(c.x->type), wt = ordered_type(c.x->type, c.w[0]->type);
     const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), 1, type_size(it));
@@ -391,6 +474,7 @@ int run_backward(const Call &c, const Gradients &d) {
     if (!bad && c.sets == 2 && !d.dw[0] != !d.dw[1]) bad = "ask for the gradients of both sets of weights or of none";
     if (!bad && !d.dw[0] && (d.db[0] || d.db[1])) bad = "the gradients of the biases come with those of the weights";
     if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
+    if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, kAnalysisOnly);
     const DeviceTable &t = c.top->backward;
     const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), c.sets, type_size(type));
     const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, type, type, true);
@@ -472,6 +556,7 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
         if (e == cudaSuccess) e = upload(t->forward, t->host.forward);
         if (e == cudaSuccess) e = upload(t->backward, t->host.backward);
         if (e == cudaSuccess) e = upload(&t->rows, t->host.rows);
+        if (e == cudaSuccess) e = upload_few_rows(*t);
         t->device = device;
         if (e != cudaSuccess) {
             spdnn_topology_destroy(t);
@@ -498,6 +583,7 @@ extern "C" void spdnn_topology_destroy(spdnn_topology_t *top) {
         release(top->forward);
         release(top->backward);
         cudaFree(top->rows);
+        cudaFree(top->few_rows);
     }
     delete top;
 }
@@ -525,6 +611,10 @@ extern "C" int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, in
     if (check_types(x_type, w_type, backward != 0)) return SPDNN_ERR_ARG;
     if (top->device < 0) return SPDNN_ERR_STATE;
     const int it = image_type(x_type), wt = ordered_type(x_type, w_type);
+    if (!backward && few_tokens(*top, tokens, x_type)) {
+        *bytes = 0;
+        return SPDNN_OK;
+    }
     const DeviceTable &t = backward ? top->backward : top->forward;
     const GatherPlan g = plan_gather(*top, t, std::max(tokens, 1), backward ? sets : 1, type_size(it));
     *bytes = layout(*top, g, t, tokens, sets, it, wt, backward != 0).total;

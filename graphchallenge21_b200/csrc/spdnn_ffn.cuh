@@ -672,6 +672,136 @@ __global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_
     }
 }
 
+// ---- a few tokens ----------------------------------------------------------------------------------
+
+struct FewArgs {
+    Matrix x, w0, w1;
+    const void *rows;          // canonical rows [outputs][stride] of the topology: uint16_t where inputs < 65536, else int32_t; `inputs` = none
+    int row_stride;            // slots rounded up to a multiple of 4
+    int slots, inputs, outputs, tokens;
+    const float *bias0, *bias1;
+    void *y;
+    float *z0, *z1;
+    int64_t y_stride, z_stride;
+    int y_type, act;
+    float clip;
+    int vector_x, vector_w;    // every row of x on 16 bytes; every row of the weights on four elements
+};
+
+constexpr int kFewThreads = 512;
+
+// Four weights of a row, from slot j on (a multiple of 4), as floats; zeros behind the last slot.
+template <class W, bool MX>
+__device__ __forceinline__ void four_weights(const Matrix &m, bool vector, int c, int j, int slots, float (&w)[4]) {
+    if constexpr (MX) {
+        const int64_t b = (int64_t)c * m.stride + (j >> 5);
+        const float scale = e8m0_value(__ldg(m.scales + b));
+        e2m1_values(__ldg((const uint16_t *)((const uint8_t *)m.data + b * 16 + ((j & 31) >> 1))), w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] *= scale;
+    } else {
+        const W *from = (const W *)m.data + (int64_t)c * m.stride + j;
+        if (vector && j + 4 <= slots) {
+            Raw<W, 4> r;
+            r.load(from);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = bits_to_float<W>(r.bits(k));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = j + k < slots ? to_float(from[k]) : 0.0f;
+        }
+    }
+}
+
+// Forward pass of up to T tokens in one launch that reads the caller's operands as they are: with few tokens the latency of a call is what
+// counts, and laying out image and weights first would take longer than the sums.  Eight lanes share a neuron, four connections
+// of 32 each; the tokens' activations lie in shared memory [inputs + 1][T] (the last row zeros, where missing connections point).
+template <class E, class W, bool MX, int T, int G>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant__ FewArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    E *x = (E *)smem;
+    const int t0 = blockIdx.y * T;
+    constexpr int N = 16 / (int)sizeof(E);
+    const int tokens = min(T, a.tokens - t0);
+    for (int i = threadIdx.x; i < (a.inputs + N) / N; i += kFewThreads) {
+        E e[T][N];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            float v[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = 0.0f;
+            if (t < tokens && i * N < a.inputs) load_row_part<N>(a.x, a.vector_x, t0 + t, i * N, a.inputs, v);
+#pragma unroll
+            for (int k = 0; k < N; ++k) e[t][k] = from_float<E>(v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (i * N + k <= a.inputs) {
+#pragma unroll
+                for (int t = 0; t < T; ++t) x[(i * N + k) * T + t] = e[t][k];
+            }
+    }
+    __syncthreads();
+    const int j0 = (threadIdx.x & 7) * 4;
+    // every lane of a warp stays for the shuffles: neurons behind the last are computed as the last one and not stored
+    for (int first = blockIdx.x * (kFewThreads / 8); first < a.outputs; first += gridDim.x * (kFewThreads / 8)) {
+        const int mine = first + (threadIdx.x >> 3), c = min(mine, a.outputs - 1);
+        float acc[G][T];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int t = 0; t < T; ++t) acc[g][t] = 0.0f;
+        for (int j = j0; j < a.slots; j += 32) {
+            uint32_t row[4];
+            if (a.inputs < 65536) {
+                const uint2 r = __ldg((const uint2 *)((const uint16_t *)a.rows + (int64_t)c * a.row_stride + j));
+                row[0] = r.x & 0xffffu; row[1] = r.x >> 16; row[2] = r.y & 0xffffu; row[3] = r.y >> 16;
+            } else {
+                const uint4 r = __ldg((const uint4 *)((const int32_t *)a.rows + (int64_t)c * a.row_stride + j));
+                row[0] = r.x; row[1] = r.y; row[2] = r.z; row[3] = r.w;
+            }
+            float w[G][4];
+            four_weights<W, MX>(a.w0, a.vector_w, c, j, a.slots, w[0]);
+            if (G == 2) four_weights<W, MX>(a.w1, a.vector_w, c, j, a.slots, w[G - 1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                Raw<E, T> v;
+                v.load(x + row[k] * T);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    // a missing connection's weight is whatever the matrix holds there
+                    const float one = row[k] == (uint32_t)a.inputs ? 0.0f : w[g][k];
+#pragma unroll
+                    for (int t = 0; t < T; ++t) acc[g][t] = fmaf(bits_to_float<E>(v.bits(t)), one, acc[g][t]);
+                }
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int s = 4; s; s >>= 1) acc[g][t] += __shfl_xor_sync(0xffffffffu, acc[g][t], s);
+        // lane t of the eight stores token t
+        float g = acc[0][0], u = acc[G - 1][0];
+#pragma unroll
+        for (int t = 1; t < T; ++t)
+            if ((threadIdx.x & 7) == t) { g = acc[0][t]; u = acc[G - 1][t]; }
+        const int t = threadIdx.x & 7;
+        if (mine >= a.outputs || t >= tokens) continue;
+        const int64_t token = t0 + t;
+        g += a.bias0 ? __ldg(a.bias0 + c) : 0.0f;
+        if (G == 2) u += a.bias1 ? __ldg(a.bias1 + c) : 0.0f;
+        if (a.z0) {
+            a.z0[token * a.z_stride + c] = g;
+            if (G == 2) a.z1[token * a.z_stride + c] = u;
+        }
+        float y = activate<sizeof(E) == 2>(g, a.act, a.clip);
+        if (G == 2) y *= u;
+        store_from_float(a.y, a.y_type, token * a.y_stride + c, y);
+    }
+}
+
 // ---- gradients of the weights ----------------------------------------------------------------------
 
 struct DwArgs {

@@ -22,12 +22,15 @@ F32, F16, BF16, MX4_TYPE = 0, 1, 2, 3
 _ERR_LEN = 256
 
 
-def _type_of(dtype):
+_TYPES = {}          # torch type -> SPDNN_F32 ..., filled when torch is first needed
+_byref, _Operand = C.byref, _lib.Operand
+
+
+def _torch():
     import torch
-    t = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
-    if t is None:
-        raise SpDNNError(-1, f"type {dtype} is not float32, float16 or bfloat16")
-    return t
+    if not _TYPES:
+        _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return torch
 
 
 def _call(fn, *args):
@@ -37,17 +40,11 @@ def _call(fn, *args):
         raise SpDNNError(rc, err.value.decode())
 
 
-def _stream(device):
-    import torch
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def _ref(operand):
-    return None if operand is None else C.byref(operand)
-
-
-def _data(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+def _stream(device: int) -> int:
+    """The handle of torch's current stream; ``torch.cuda.current_stream`` makes an object for it, in twenty times the time."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 class MX4:
@@ -63,10 +60,7 @@ class MX4:
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device or not codes.is_cuda:
             raise SpDNNError(-1, "codes and scales must be contiguous and on one GPU")
         self.codes, self.scales, self.cols = codes, scales, int(cols)
-
-    @property
-    def shape(self):
-        return (int(self.codes.shape[0]), self.cols)
+        self.shape = (int(codes.shape[0]), self.cols)
 
     @property
     def device(self):
@@ -74,50 +68,83 @@ class MX4:
 
     def dequantize(self, dtype=None, out=None):
         """The values as a tensor (float32 unless ``dtype`` or ``out`` says otherwise)."""
-        import torch
+        torch = _torch()
+        device = self.codes.get_device()
         if out is None:
             out = torch.empty(self.shape, dtype=dtype or torch.float32, device=self.device)
-        elif out.device != self.device:
-            raise SpDNNError(-1, "out lives on another device")
-        operand = _operand(out, self.shape, "out")
-        with torch.cuda.device(self.device):
-            _call(_lib.load().spdnn_mx4_dequantize, _data(self.codes), _data(self.scales), self.shape[0], self.cols,
-                  C.byref(operand), _stream(self.device))
+        operand = _operand(out, *self.shape, device, "out")
+        with _On(device):
+            _call(_lib.load().spdnn_mx4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
+                  _byref(operand), _stream(device))
         return out
 
 
-def _operand(t, shape, name):
+class _On:
+    """``torch.cuda.device`` where the current device is another one."""
+
+    def __init__(self, device):
+        cuda = _torch().cuda
+        self._guard = None if cuda.current_device() == device else cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _operand(t, rows, cols, device, name):
+    """The C operand of a matrix [rows, cols] on GPU ``device`` (None: any)."""
     if isinstance(t, MX4):
-        if t.shape != tuple(shape):
-            raise SpDNNError(-1, f"{name} must be {tuple(shape)}, not {t.shape}")
-        return _lib.Operand(t.codes.data_ptr(), t.scales.data_ptr(), int(t.codes.shape[1]), MX4_TYPE, 0)
-    if not hasattr(t, "is_cuda") or not t.is_cuda:
-        raise SpDNNError(-1, f"{name} must be a CUDA tensor")
-    if tuple(t.shape) != tuple(shape):
-        raise SpDNNError(-1, f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise SpDNNError(-1, f"{name} must have adjacent elements in a row (stride 1)")
-    stride = int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
-    return _lib.Operand(t.data_ptr(), None, stride, _type_of(t.dtype), 0)
+        if t.shape != (rows, cols):
+            raise SpDNNError(-1, f"{name} must be {(rows, cols)}, not {t.shape}")
+        on, operand = t.codes.get_device(), _Operand(t.codes.data_ptr(), t.scales.data_ptr(), (cols + 31) // 32, MX4_TYPE, 0)
+    else:
+        if not hasattr(t, "is_cuda") or not t.is_cuda:
+            raise SpDNNError(-1, f"{name} must be a CUDA tensor")
+        if t.shape != (rows, cols):
+            raise SpDNNError(-1, f"{name} must be {(rows, cols)}, not {tuple(t.shape)}")
+        stride, step = t.stride()
+        if step != 1 and cols > 1:
+            raise SpDNNError(-1, f"{name} must have adjacent elements in a row (stride 1)")
+        kind = _TYPES.get(t.dtype)
+        if kind is None:
+            raise SpDNNError(-1, f"{name} is {t.dtype}, not float32, float16 or bfloat16")
+        on, operand = t.get_device(), _Operand(t.data_ptr(), None, stride if rows > 1 else cols, kind, 0)
+    if on != device and device is not None:
+        raise SpDNNError(-1, f"{name} lives on another device than the topology or matrix")
+    return operand
 
 
 def mx4_quantize(x) -> MX4:
     """``x`` [rows, cols] (float32, float16 or bfloat16, rows of any stride) as microscaled 4-bit floats."""
-    import torch
+    torch = _torch()
     if not hasattr(x, "is_cuda") or x.dim() != 2 or x.shape[1] < 1:
         raise SpDNNError(-1, "x must be a matrix with at least one column")
-    operand = _operand(x, x.shape, "x")
-    rows, cols = int(x.shape[0]), int(x.shape[1])
+    rows, cols = x.shape
+    operand = _operand(x, rows, cols, None, "x")
     blocks = (cols + 31) // 32
-    codes = torch.empty((rows, blocks, 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _call(_lib.load().spdnn_mx4_quantize, C.byref(operand), rows, cols, _data(codes), _data(scales), _stream(x.device))
+    codes = x.new_empty((rows, blocks, 16), dtype=torch.uint8)
+    scales = x.new_empty((rows, blocks), dtype=torch.uint8)
+    device = x.get_device()
+    with _On(device):
+        _call(_lib.load().spdnn_mx4_quantize, _byref(operand), rows, cols, codes.data_ptr(), scales.data_ptr(), _stream(device))
     return MX4(codes, scales, cols)
 
 
-class Saved(tuple):
-    """What a forward call with ``save=True`` keeps for its backward call: one pre-activation matrix (float32) per set of weights."""
+class Saved:
+    """What a forward call with ``save=True`` keeps for its backward call: the pre-activations, float32 [sets, tokens, outputs]."""
+
+    def __init__(self, z):
+        self.z = z
+
+    def __len__(self):
+        return self.z.shape[0]
+
+    def __iter__(self):
+        return iter(self.z)
 
 
 class SparseTopology:
@@ -127,6 +154,7 @@ class SparseTopology:
     def __init__(self, inputs: int, outputs: int, col_ptr, row_idx, device: int | None = 0):
         self._top = C.c_void_p()
         self._lib = _lib.load()
+        self._sizes = {}                 # workspaces: a function of these arguments and the topology
         col_ptr = np.ascontiguousarray(col_ptr, dtype=np.int32)
         row_idx = np.ascontiguousarray(row_idx, dtype=np.int32)
         if col_ptr.shape != (outputs + 1,):
@@ -189,94 +217,104 @@ class SparseTopology:
 
     # -- calls -----------------------------------------------------------------------
     def _prepare(self, x, weights, biases, activation):
+        """(tokens, operands of x and the weights, the activation's number) of a call, checked as far as the C side cannot."""
         if not self._top:
             raise SpDNNError(-4, "the topology is closed")
         if self.device is None:
             raise SpDNNError(-4, "the topology was created for analysis only (device None)")
-        if activation not in ACTIVATIONS:
+        kind = ACTIVATIONS.get(activation)
+        if kind is None:
             raise SpDNNError(-1, f"activation must be one of {sorted(ACTIVATIONS)}")
+        torch = _torch()
         if len(x.shape) != 2:
             raise SpDNNError(-1, f"x must be [tokens, {self.inputs}]")
-        tokens = int(x.shape[0])
-        ops = [_operand(x, (tokens, self.inputs), "x")] + [_operand(w, (self.outputs, self.slots), "weights") for w in weights]
-        self._same_device(x, *weights, *biases)
-        import torch
+        tokens = x.shape[0]
+        ops = [_operand(x, tokens, self.inputs, self.device, "x")]
+        for w in weights:
+            ops.append(_operand(w, self.outputs, self.slots, self.device, "weights"))
         for b in biases:
-            if b is not None and (b.dtype != torch.float32 or tuple(b.shape) != (self.outputs,) or not b.is_contiguous()):
-                raise SpDNNError(-1, f"a bias must be contiguous float32 [{self.outputs}]")
-        return tokens, ops
+            if b is not None and (b.dtype != torch.float32 or b.shape != (self.outputs,) or b.get_device() != self.device
+                                  or not b.is_contiguous()):
+                raise SpDNNError(-1, f"a bias must be contiguous float32 [{self.outputs}] on the topology's device")
+        return tokens, ops, kind
 
-    def _same_device(self, *tensors):
-        for t in tensors:
-            if t is not None and t.device.index != self.device:
-                raise SpDNNError(-1, "a tensor lives on another device than the topology")
+    def _workspace(self, x, *key):
+        """(pointer, bytes, what keeps it alive) of a call's workspace; ``key``: tokens, sets, types of x and w, backward."""
+        size = self._sizes.get(key)
+        if size is None:
+            n = C.c_int64()
+            rc = self._lib.spdnn_layer_workspace(self._top, *key, _byref(n))
+            if rc != 0:
+                raise SpDNNError(rc, "these types of activations and weights do not go together")
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            size = self._sizes[key] = n.value
+        if not size:
+            return None, 0, None
+        ws = x.new_empty(size, dtype=_torch().uint8)
+        return ws.data_ptr(), size, ws
 
-    def _workspace(self, tokens, sets, x_type, w_type, backward, device):
-        import torch
-        n = C.c_int64()
-        rc = self._lib.spdnn_layer_workspace(self._top, tokens, sets, x_type, w_type, int(backward), C.byref(n))
-        if rc != 0:
-            raise SpDNNError(rc, "these types of activations and weights do not go together")
-        return torch.empty(n.value, dtype=torch.uint8, device=device), n.value
+    def _saved_operands(self, z, tokens):
+        at, step = z.data_ptr(), tokens * self.outputs * 4
+        return [_byref(_Operand(at + s * step, None, self.outputs, F32, 0)) for s in range(z.shape[0])]
 
-    def _forward(self, x, weights, biases, activation, clip, save, out_dtype, out):
-        import torch
-        tokens, ops = self._prepare(x, weights, biases, activation)
+    def _forward(self, fn, x, weights, biases, activation, clip, save, out_dtype, out):
+        tokens, ops, kind = self._prepare(x, weights, biases, activation)
+        like = x.codes if isinstance(x, MX4) else x
         if out is None:
-            if out_dtype is None:
-                if isinstance(x, MX4):
-                    raise SpDNNError(-1, "out_dtype is needed for microscaled activations")
-                out_dtype = x.dtype
-            out = torch.empty((tokens, self.outputs), dtype=out_dtype, device=x.device)
-        self._same_device(out)
-        y = _operand(out, (tokens, self.outputs), "out")
-        saved = None
+            if out_dtype is None and like is not x:
+                raise SpDNNError(-1, "out_dtype is needed for microscaled activations")
+            out = like.new_empty((tokens, self.outputs), dtype=out_dtype)
+        y = _operand(out, tokens, self.outputs, self.device, "out")
         if save:
-            if isinstance(x, MX4):
+            if like is not x:
                 raise SpDNNError(-1, "microscaled activations have no backward pass: nothing to save")
-            saved = Saved(torch.empty((tokens, self.outputs), dtype=torch.float32, device=x.device) for _ in weights)
-        z = [_operand(s, (tokens, self.outputs), "saved") for s in saved] if save else [None] * len(weights)
-        ws, size = self._workspace(tokens, len(weights), ops[0].type, ops[1].type, False, x.device)
-        fn = self._lib.spdnn_gated if len(weights) == 2 else self._lib.spdnn_linear
-        _call(fn, self._top, tokens, *map(_ref, ops), *map(_data, biases), ACTIVATIONS[activation], float(clip), _ref(y),
-              *map(_ref, z), _data(ws), size, _stream(x.device))
+            saved = Saved(x.new_empty((len(weights), tokens, self.outputs), dtype=_torch().float32))
+            z = self._saved_operands(saved.z, tokens)
+        else:
+            z = [None] * len(weights)
+        ws, size, keep = self._workspace(like, tokens, len(weights), ops[0].type, ops[1].type, 0)
+        _call(fn, self._top, tokens, *map(_byref, ops), *[None if b is None else b.data_ptr() for b in biases], kind, clip, _byref(y), *z,
+              ws, size, _stream(self.device))
         return (out, saved) if save else out
 
     def linear(self, x, w, bias=None, activation: str = "none", clip: float = 32.0, save: bool = False, out_dtype=None, out=None):
         """``act(x W + bias)``: x [tokens, inputs], w [outputs, slots] (of x's type, or ``MX4``), bias float32 [outputs].
         ``save``: also return what ``linear_backward`` needs."""
-        return self._forward(x, [w], [bias], activation, clip, save, out_dtype, out)
+        return self._forward(self._lib.spdnn_linear, x, [w], [bias], activation, clip, save, out_dtype, out)
 
     def gated(self, x, w_gate, w_up, bias_gate=None, bias_up=None, activation: str = "silu", clip: float = 32.0,
               save: bool = False, out_dtype=None, out=None):
         """``act(x Wg + bg) * (x Wu + bu)``, both projections in one pass; ``save`` as in ``linear``."""
-        return self._forward(x, [w_gate, w_up], [bias_gate, bias_up], activation, clip, save, out_dtype, out)
+        return self._forward(self._lib.spdnn_gated, x, [w_gate, w_up], [bias_gate, bias_up], activation, clip, save, out_dtype, out)
 
-    def _backward(self, dy, x, weights, saved, activation, clip, need_dx, need_dw):
-        import torch
-        tokens, ops = self._prepare(x, weights, [], activation)
-        shape = (tokens, self.outputs)
-        if not isinstance(saved, Saved) or len(saved) != len(weights):
+    def _backward(self, fn, dy, x, weights, saved, activation, clip, need_dx, need_dw):
+        tokens, ops, kind = self._prepare(x, weights, (), activation)
+        if isinstance(x, MX4):
+            raise SpDNNError(-1, "microscaled activations have no backward pass")
+        z = getattr(saved, "z", None)
+        if z is None or z.shape != (len(weights), tokens, self.outputs) or z.get_device() != self.device:
             raise SpDNNError(-1, "saved must be what the forward call returned")
-        self._same_device(dy, *saved)
-        dy_op = _operand(dy, shape, "dy")
-        z = [_operand(s, shape, "saved") for s in saved]
-        dx = torch.empty((tokens, self.inputs), dtype=x.dtype, device=x.device) if need_dx else None
-        dw = [torch.empty((self.outputs, self.slots), dtype=torch.float32, device=x.device) if need_dw else None for _ in weights]
-        db = [torch.empty(self.outputs, dtype=torch.float32, device=x.device) if need_dw else None for _ in weights]
-        dx_op = _operand(dx, (tokens, self.inputs), "dx") if need_dx else None
-        ws, size = self._workspace(tokens, len(weights), ops[0].type, ops[1].type, True, x.device)
-        fn = self._lib.spdnn_gated_backward if len(weights) == 2 else self._lib.spdnn_linear_backward
-        _call(fn, self._top, tokens, _ref(dy_op), *map(_ref, ops), *map(_ref, z), ACTIVATIONS[activation], float(clip), _ref(dx_op),
-              *map(_data, dw), *map(_data, db), _data(ws), size, _stream(x.device))
-        return (dx, *dw, *db)
+        dy_op = _byref(_operand(dy, tokens, self.outputs, self.device, "dy"))
+        dx = dx_op = None
+        if need_dx:
+            dx = x.new_empty((tokens, self.inputs))
+            dx_op = _byref(_operand(dx, tokens, self.inputs, self.device, "dx"))
+        f32 = _torch().float32
+        grads = [None] * (2 * len(weights))
+        if need_dw:
+            grads = [x.new_empty((self.outputs, self.slots), dtype=f32) for _ in weights] + [x.new_empty(self.outputs, dtype=f32) for _ in weights]
+        ws, size, keep = self._workspace(x, tokens, len(weights), ops[0].type, ops[1].type, 1)
+        _call(fn, self._top, tokens, dy_op, *map(_byref, ops), *self._saved_operands(z, tokens), kind, clip, dx_op,
+              *[None if t is None else t.data_ptr() for t in grads], ws, size, _stream(self.device))
+        return (dx, *grads)
 
     def linear_backward(self, dy, x, w, saved, activation: str = "none", clip: float = 32.0, need_dx: bool = True, need_dw: bool = True):
         """Gradients ``(dx, dw, dbias)`` of ``linear(..., save=True)`` for dL/dy = ``dy`` (of x's type): dx of x's type, dw
         [outputs, slots] and dbias in float32; what is not needed is None."""
-        return self._backward(dy, x, [w], saved, activation, clip, need_dx, need_dw)
+        return self._backward(self._lib.spdnn_linear_backward, dy, x, [w], saved, activation, clip, need_dx, need_dw)
 
     def gated_backward(self, dy, x, w_gate, w_up, saved, activation: str = "silu", clip: float = 32.0, need_dx: bool = True,
                        need_dw: bool = True):
         """Gradients ``(dx, dw_gate, dw_up, dbias_gate, dbias_up)`` of ``gated(..., save=True)``."""
-        return self._backward(dy, x, [w_gate, w_up], saved, activation, clip, need_dx, need_dw)
+        return self._backward(self._lib.spdnn_gated_backward, dy, x, [w_gate, w_up], saved, activation, clip, need_dx, need_dw)

@@ -262,7 +262,8 @@ int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int *outputs, 
 int spdnn_topology_rows(const spdnn_topology_t *top, int32_t *rows, int64_t capacity);
 
 /* Bytes of device workspace (aligned to 256) that a call needs: sets 1 = spdnn_linear, 2 = spdnn_gated, or their backward calls.
- * Its contents need not be kept between calls; calls that may overlap need one each. */
+ * Its contents need not be kept between calls; calls that may overlap need one each.  0 (forward calls of few tokens): none is
+ * needed, workspace may be NULL. */
 int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, int sets, int x_type, int w_type, int backward, int64_t *bytes);
 
 /* y[tokens][outputs] = act(x W + bias).  x [tokens][inputs] and w [outputs][slots]: one float type, or w MX4 with any x, or x

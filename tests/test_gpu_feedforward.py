@@ -438,15 +438,16 @@ def test_refusals_on_the_gpu():
 def test_a_workspace_that_is_too_small_is_refused():
     import ctypes as C
     from graphchallenge21_b200 import _lib
-    p = Problem(5, 40, 30, 4, F32, 1)
+    p = Problem(300, 40, 30, 4, F32, 1)
     lib = _lib.load()
     n = C.c_int64()
-    assert lib.spdnn_layer_workspace(p.top._top, 5, 1, 0, 0, 0, C.byref(n)) == 0 and n.value > 0
+    assert lib.spdnn_layer_workspace(p.top._top, 1, 1, 0, 0, 0, C.byref(n)) == 0 and n.value == 0      # one token needs none
+    assert lib.spdnn_layer_workspace(p.top._top, 300, 1, 0, 0, 0, C.byref(n)) == 0 and n.value > 0
     ws = torch.empty(n.value + 256, dtype=torch.uint8, device="cuda")
-    y = torch.empty(5, 30, device="cuda")
+    y = torch.empty(300, 30, device="cuda")
     o = lambda t: C.byref(_lib.Operand(t.data_ptr(), None, t.stride(0), 0, 0))  # noqa: E731
     err = C.create_string_buffer(256)
-    call = lambda at, size: lib.spdnn_linear(p.top._top, 5, o(p.x), o(p.w[0]), None, 0, 32.0, o(y), None, ws.data_ptr() + at, size, None,  # noqa: E731
+    call = lambda at, size: lib.spdnn_linear(p.top._top, 300, o(p.x), o(p.w[0]), None, 0, 32.0, o(y), None, ws.data_ptr() + at, size, None,  # noqa: E731
                                              err, 256)
     assert call(0, n.value - 1) == -1 and b"workspace" in err.value
     assert call(16, n.value) == -1 and b"aligned" in err.value
