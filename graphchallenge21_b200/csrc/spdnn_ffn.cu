@@ -125,9 +125,6 @@ struct GatherPlan {
 };
 
 constexpr int64_t kSharedLimit = 227 * 1024;
-#ifndef SPDNN_FEW
-#define SPDNN_FEW 16
-#endif
 
 int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
@@ -218,31 +215,37 @@ cudaError_t launch_gather(const GatherPlan &g, GatherArgs a, int image_type, int
     return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(threads), args, shared, stream);
 }
 
-cudaError_t launch_pack(const PackArgs &a, int image_type, int sets, bool gradient, cudaStream_t stream) {
-    const int64_t blocks = (int64_t)((a.rows + 63) / 64) * ((a.tokens + 63) / 64);
-    const unsigned grid = (unsigned)blocks;
-    const auto run = [&](auto e) {
+unsigned pack_blocks(const PackArgs &a) { return (unsigned)((int64_t)((a.rows + 63) / 64) * ((a.tokens + 63) / 64)); }
+
+// What a call's gather (and dw_kernel) read.  gradient: the backward call, whose gathered values are dL/dz.
+cudaError_t launch_prepare(const PrepareArgs &args, int x_blocks, int sets, bool gradient, int image_type, int weight_type, cudaStream_t stream) {
+    const int64_t grid = (int64_t)args.order_blocks + args.main_blocks + x_blocks;
+    if (!grid) return cudaSuccess;
+    const auto run = [&](auto e, auto w) {
         using E = decltype(e);
-        if (!gradient) return launch(pack_kernel<E, 1, false>, grid, kPackThreads, stream, a);
-        return sets == 1 ? launch(pack_kernel<E, 1, true>, grid, kPackThreads, stream, a) : launch(pack_kernel<E, 2, true>, grid, kPackThreads, stream, a);
+        using W = decltype(w);
+        if (gradient) {
+            if constexpr (std::is_same<E, W>::value)
+                return sets == 2 ? launch(prepare_kernel<E, W, 2, true>, (unsigned)grid, kPackThreads, stream, args)
+                                 : launch(prepare_kernel<E, W, 1, true>, (unsigned)grid, kPackThreads, stream, args);
+            return cudaErrorInvalidValue;
+        }
+        return sets == 2 ? launch(prepare_kernel<E, W, 2, false>, (unsigned)grid, kPackThreads, stream, args)
+                         : launch(prepare_kernel<E, W, 1, false>, (unsigned)grid, kPackThreads, stream, args);
     };
-    return image_type == F32 ? run(float()) : image_type == F16 ? run(__half()) : run(bf16());
+    if (image_type == F32) return run(float(), float());
+    if (image_type == BF16) return run(bf16(), bf16());
+    return weight_type == F16 ? run(__half(), __half()) : run(__half(), bf16());
 }
 
-// weights, index: where the call's table goes
-cudaError_t launch_order(const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int values, int sets,
-                         int weight_type, int image_type, void *weights, void *index, cudaStream_t stream) {
-    if (!t.entries) return cudaSuccess;
-    OrderArgs a{};
+// The part of it that orders a table.
+void order_part(PrepareArgs &args, const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int values, int image_type,
+                void *weights, void *index) {
+    OrderArgs &a = args.order;
     a.w0 = w0; a.w1 = w1; a.idx = t.idx; a.src = t.src; a.entries = t.entries; a.slots = slots; a.values = values; a.p = g.p;
     a.whole = g.v * type_size(image_type) == 16; a.wide = g.global;
     a.weights = weights; a.index = index;
-    const unsigned grid = (unsigned)((t.entries + 255) / 256);
-    const auto run = [&](auto w) {
-        using W = decltype(w);
-        return sets == 2 ? launch(order_kernel<W, 2>, grid, 256, stream, a) : launch(order_kernel<W, 1>, grid, 256, stream, a);
-    };
-    return weight_type == F32 ? run(float()) : weight_type == F16 ? run(__half()) : run(bf16());
+    args.order_blocks = (unsigned)((t.entries + kPackThreads - 1) / kPackThreads);
 }
 
 // The type activations have in an image, and weights in a gather table's order.  Microscaled values are exact in bf16 (two bits of
@@ -341,15 +344,17 @@ int check_run(const Call &c, int64_t need) {
 
 int check_blocks(const Call &c, const GatherPlan &g) {
     const int64_t pack = (int64_t)((std::max(c.top->host.inputs, c.top->host.outputs) + 63) / 64) * ((c.tokens + 63) / 64);
-    if (pack > 0x7fffffffll || g.tiles * g.splits > 0x7fffffffll)
+    if (pack > 0x3fffffffll || g.tiles * g.splits > 0x7fffffffll)
         return fail(c.err, c.err_len, SPDNN_ERR_LIMIT, "tokens times neurons is too large for one call: split the tokens");
     return SPDNN_OK;
 }
 
-// Tokens that one launch of few_kernel takes at a time, or 0: the images' way.
+// Tokens that one launch of few_kernel takes at a time, or 0: the images' way.  It wins up to about 2^22 multiply-adds a set (us, few_kernel
+// against the images: 4096 -> 16384, 32 connections, bf16, 8 tokens 11.1 and 12.4, 12 tokens 19.5 and 14.8; 1024 -> 4096, 24 tokens
+// 11.8 and 13.2), in at most four groups of tokens.
 int few_tokens(const spdnn_topology &top, int tokens, int x_type) {
     const int64_t row = (int64_t)(top.host.inputs + 1) * type_size(image_type(x_type));
-    if (tokens > SPDNN_FEW) return 0;
+    if (tokens * (int64_t)top.host.outputs * top.host.slots > 1ll << 22 && tokens > 1) return 0;
     int T = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
     if (x_type == F32) T = std::min(T, 4);
     while (T > 1 && row * T > kSharedLimit / 2) T /= 2;
@@ -428,13 +433,13 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     OnDevice guard(c.top->device);
     if (guard.status != cudaSuccess) return fail_cuda(c.err, c.err_len, guard.status);
     char *base = (char *)c.workspace;
-    cudaError_t e = launch_order(g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, 1, c.sets, wt, it, base + ws.weights, base + ws.index, c.stream);
-    if (e == cudaSuccess) {
-        PackArgs p{};
-        p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
-        p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x);
-        e = launch_pack(p, it, 1, false, c.stream);
-    }
+    PrepareArgs prep{};
+    order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, 1, it, base + ws.weights, base + ws.index);
+    PackArgs &p = prep.main;
+    p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
+    p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x);
+    prep.main_blocks = pack_blocks(p);
+    cudaError_t e = launch_prepare(prep, 0, c.sets, false, it, wt, c.stream);
     if (e == cudaSuccess) {
         GatherArgs a{};
         a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
@@ -484,7 +489,9 @@ int run_backward(const Call &c, const Gradients &d) {
     char *base = (char *)c.workspace;
     const int64_t stride = ((int64_t)c.tokens + 63) / 64 * 64;
     if (c.tokens > 0 && e == cudaSuccess) {
-        PackArgs p{};
+        PrepareArgs prep{};
+        if (d.dx) order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, type, base + ws.weights, base + ws.index);
+        PackArgs &p = prep.main;
         p.x = matrix(d.dy);
         if (c.z[0]) { p.z0 = (const float *)c.z[0]->data; p.z_stride = c.z[0]->stride; }
         if (c.z[1]) p.z1 = (const float *)c.z[1]->data;
@@ -492,25 +499,20 @@ int run_backward(const Call &c, const Gradients &d) {
         p.rows = h.outputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.act = c.act; p.clip = c.clip;
         p.image = d.dx ? base + ws.image : nullptr; p.image_bytes = g.image_bytes;
         p.columns = d.dw[0] ? base + ws.d_columns : nullptr; p.token_stride = stride;
-        e = launch_pack(p, type, c.sets, true, c.stream);
+        prep.main_blocks = p.image || p.columns ? pack_blocks(p) : 0;
+        PackArgs &x = prep.x;
+        x.x = matrix(c.x); x.rows = h.inputs; x.tokens = c.tokens; x.v = x.p = 1; x.vector = on_16_bytes(c.x);
+        x.columns = base + ws.x_columns; x.token_stride = stride;
+        e = launch_prepare(prep, d.dw[0] ? pack_blocks(x) : 0, c.sets, true, type, type, c.stream);
     }
     if (c.tokens > 0 && d.dx && e == cudaSuccess) {
-        e = launch_order(g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, c.sets, type, type, base + ws.weights, base + ws.index, c.stream);
-        if (e == cudaSuccess) {
-            GatherArgs a{};
-            a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
-            a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
-            a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
-            e = launch_gather(g, a, type, type, c.sets, 1, c.stream);
-        }
+        GatherArgs a{};
+        a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
+        a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
+        a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
+        e = launch_gather(g, a, type, type, c.sets, 1, c.stream);
     }
     if (d.dw[0] && e == cudaSuccess) {
-        if (c.tokens > 0) {
-            PackArgs p{};
-            p.x = matrix(c.x); p.rows = h.inputs; p.tokens = c.tokens; p.v = p.p = 1; p.vector = on_16_bytes(c.x);
-            p.columns = base + ws.x_columns; p.token_stride = stride;
-            e = launch_pack(p, type, 1, false, c.stream);
-        }
         if (e == cudaSuccess) {
             DwArgs a{};
             a.x = base + ws.x_columns; a.d = (const float *)(base + ws.d_columns); a.rows = c.top->rows; a.token_stride = stride;
@@ -668,17 +670,27 @@ const char *check_mx4(const void *codes, const uint8_t *scales, int64_t rows, in
     return check_operand(m, rows, cols, false);
 }
 
-unsigned mx4_grid(int64_t groups) { return (unsigned)std::min<int64_t>((groups + kMx4Threads * kMx4Batch - 1) / (kMx4Threads * kMx4Batch), 1 << 20); }
+unsigned mx4_grid(int64_t groups, int batch) { return (unsigned)std::min<int64_t>((groups + kMx4Threads * batch - 1) / (kMx4Threads * batch), 1 << 20); }
+
+// Groups of a thread: several, whose loads are in flight together, where that leaves the GPU full (8191 x 4100 bf16 28.4 us with one, 24.0
+// with four; 16384 x 32 fp32 2.0 and 2.9).
+bool mx4_batched(int64_t groups) { return groups >= 1 << 20; }
 
 template <class E>
 cudaError_t quantize(const spdnn_operand_t *x, int64_t rows, int cols, uint8_t *codes, uint8_t *scales, cudaStream_t stream) {
     const int blocks = (cols + 31) / 32;
     const uintptr_t both = reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->stride * (int64_t)sizeof(E));
-    const auto kernel = both % 16 == 0  ? mx4_quantize_kernel<E, 16>
-                        : both % 8 == 0 ? mx4_quantize_kernel<E, 8>
-                        : both % 4 == 0 ? mx4_quantize_kernel<E, 4>
-                                        : mx4_quantize_kernel<E, (int)sizeof(E)>;
-    return launch(kernel, mx4_grid(rows * blocks * 4), kMx4Threads, stream, (const E *)x->data, x->stride, rows, cols, blocks, (uint32_t *)codes,
+    const int64_t groups = rows * blocks * 4;
+    const auto choose = [&](auto batch) {
+        constexpr int B = decltype(batch)::value;
+        return both % 16 == 0  ? mx4_quantize_kernel<E, 16, B>
+               : both % 8 == 0 ? mx4_quantize_kernel<E, 8, B>
+               : both % 4 == 0 ? mx4_quantize_kernel<E, 4, B>
+                               : mx4_quantize_kernel<E, (int)sizeof(E), B>;
+    };
+    const int batch = mx4_batched(groups) ? kMx4Batch : 1;
+    const auto kernel = batch == 1 ? choose(std::integral_constant<int, 1>()) : choose(std::integral_constant<int, kMx4Batch>());
+    return launch(kernel, mx4_grid(groups, batch), kMx4Threads, stream, (const E *)x->data, x->stride, rows, cols, blocks, (uint32_t *)codes,
                   scales);
 }
 
@@ -686,7 +698,11 @@ template <class E>
 cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int cols, const spdnn_operand_t *y, cudaStream_t stream) {
     const int blocks = (cols + 31) / 32;
     const bool vector = reinterpret_cast<uintptr_t>(y->data) % (4 * sizeof(E)) == 0 && y->stride % 4 == 0;
-    return launch(vector ? mx4_dequantize_kernel<E, true> : mx4_dequantize_kernel<E, false>, mx4_grid(rows * ((cols + 3) / 4)), kMx4Threads, stream,
+    const int64_t groups = rows * ((cols + 3) / 4);
+    const int batch = mx4_batched(groups) ? kMx4Batch : 1;
+    const auto kernel = batch == 1 ? (vector ? mx4_dequantize_kernel<E, true, 1> : mx4_dequantize_kernel<E, false, 1>)
+                                   : (vector ? mx4_dequantize_kernel<E, true, kMx4Batch> : mx4_dequantize_kernel<E, false, kMx4Batch>);
+    return launch(kernel, mx4_grid(groups, batch), kMx4Threads, stream,
                   codes, scales, rows, cols, blocks, (E *)const_cast<void *>(y->data), y->stride);
 }
 

@@ -108,8 +108,11 @@ template <bool FAST> __device__ __forceinline__ float activate(float v, int act,
     }
 }
 
+// 1 / (1 + e^-w)
+template <bool FAST> __device__ __forceinline__ float sigmoid(float w) { return sigmoid_times<FAST>(1.0f, w); }
+
 // act(v) and act'(v) for the backward pass
-__device__ __forceinline__ void activate_both(float v, int act, float clip, float &value, float &slope) {
+template <bool FAST> __device__ __forceinline__ void activate_both(float v, int act, float clip, float &value, float &slope) {
     switch (act) {
         case RELU: value = v < 0.0f ? 0.0f : v; slope = v > 0.0f ? 1.0f : v != v ? v : 0.0f; return;
         case CLIP:
@@ -117,7 +120,7 @@ __device__ __forceinline__ void activate_both(float v, int act, float clip, floa
             slope = v > 0.0f && v < clip ? 1.0f : v != v ? v : 0.0f;
             return;
         case SILU: {
-            const float s = 1.0f / (1.0f + expf(-v));
+            const float s = sigmoid<FAST>(v);
             value = v * s; slope = s * (1.0f + v * (1.0f - s));
             return;
         }
@@ -127,7 +130,7 @@ __device__ __forceinline__ void activate_both(float v, int act, float clip, floa
             return;
         }
         case GELU_TANH: {
-            const float s = 1.0f / (1.0f + expf(-2.0f * kGeluA * (v + kGeluB * v * v * v)));
+            const float s = sigmoid<FAST>(2.0f * kGeluA * (v + kGeluB * v * v * v));
             value = v * s; slope = s + v * s * (1.0f - s) * 2.0f * kGeluA * (1.0f + 3.0f * kGeluB * v * v);
             return;
         }
@@ -284,6 +287,12 @@ struct PackArgs {
 
 constexpr int kPackThreads = 256;
 
+// The tile of a block: a row of 64 tokens and 16 bytes for every set and neuron; of gradients in float32.
+template <class E, int SETS, bool GRADIENT> __host__ __device__ constexpr int pack_tile_bytes() {
+    using Tile = typename std::conditional<GRADIENT, float, E>::type;
+    return SETS * 64 * (64 + 16 / (int)sizeof(Tile)) * (int)sizeof(Tile);
+}
+
 // `COUNT` neighbours of a row as floats, from column `col` on; zeros behind `cols`.
 template <int COUNT>
 __device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int64_t row, int col, int cols, float (&v)[COUNT]) {
@@ -344,16 +353,17 @@ __device__ __forceinline__ void small_units(char *image, int64_t image_bytes, in
 // One block: 64 neurons x 64 tokens, through shared memory so that reads run along neurons and writes along tokens.  The tokens of a
 // neuron are permuted in groups of N (16 bytes of the tile), for the writers of neighbouring neurons to hit different banks.
 template <class E, int SETS, bool GRADIENT>
-__global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackArgs a) {
+__device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, unsigned char *shared) {
     using Tile = typename std::conditional<GRADIENT, float, E>::type;
     constexpr int N = 16 / (int)sizeof(E);            // neurons a thread loads at a time
     constexpr int G = 16 / (int)sizeof(Tile);         // tokens of a permuted group
     constexpr int ROW = 64 + G;
-    __shared__ __align__(16) Tile tile[SETS][64][ROW];
+    static_assert(sizeof(Tile[SETS][64][ROW]) == pack_tile_bytes<E, SETS, GRADIENT>(), "the tile");
+    Tile (&tile)[SETS][64][ROW] = *reinterpret_cast<Tile (*)[SETS][64][ROW]>(shared);
     const auto at = [](int n, int t) { return t ^ (((n / N) & (64 / G - 1)) * G); };
     const int blocks_n = (a.rows + 63) / 64;
-    const int n0 = (int)(blockIdx.x % blocks_n) * 64;
-    const int t0 = (int)(blockIdx.x / blocks_n) * 64;
+    const int n0 = (int)(block % blocks_n) * 64;
+    const int t0 = (int)(block / blocks_n) * 64;
     for (int i = threadIdx.x; i < 64 * 64 / N; i += kPackThreads) {
         const int t = i / (64 / N), n = i % (64 / N) * N;
         float d0[N], d1[N];
@@ -372,7 +382,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackArgs a) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
                         float value, slope;
-                        activate_both(g[k], a.act, a.clip, value, slope);
+                        activate_both<sizeof(E) == 2>(g[k], a.act, a.clip, value, slope);
                         if (SETS == 2) { d1[k] = d0[k] * value; slope *= u[k]; }
                         d0[k] *= slope;
                         if (col + k >= a.rows) d0[k] = d1[k] = 0.0f;
@@ -444,8 +454,8 @@ struct OrderArgs {
 // The gather table as a call's gather reads it: the weights in its order, and the place of every gathered neuron in the image.  Padding
 // gets the weight zero, whatever the caller's matrix holds where a neuron has no connection.
 template <class W, int SETS>
-__global__ void __launch_bounds__(256) order_kernel(const OrderArgs a) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void order_block(const OrderArgs &a, unsigned block) {
+    const int64_t e = (int64_t)block * kPackThreads + threadIdx.x;
     if (e >= a.entries) return;
     const uint32_t s = __ldg(a.src + e), n = __ldg(a.idx + e);
     const uint32_t c = s / (uint32_t)a.slots, j = s % (uint32_t)a.slots;
@@ -461,6 +471,23 @@ __global__ void __launch_bounds__(256) order_kernel(const OrderArgs a) {
     const uint32_t place = a.whole ? unit_place(n, (uint32_t)(a.values * a.p)) : n;
     if (a.wide) ((uint32_t *)a.index)[e] = place;
     else ((uint16_t *)a.index)[e] = (uint16_t)place;
+}
+
+// Everything that a call lays out, in one launch (a launch takes longer than most of these blocks): the table, then image and columns
+// of the gathered values, then (backward) the columns of x.
+struct PrepareArgs {
+    OrderArgs order;
+    PackArgs main, x;
+    unsigned order_blocks, main_blocks;     // the rest are x's
+};
+
+template <class E, class W, int SETS, bool GRADIENT>
+__global__ void __launch_bounds__(kPackThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
+    constexpr int MAIN = pack_tile_bytes<E, GRADIENT ? SETS : 1, GRADIENT>(), X = pack_tile_bytes<E, 1, false>();
+    __shared__ __align__(16) unsigned char shared[MAIN > X ? MAIN : X];
+    if (blockIdx.x < a.order_blocks) order_block<W, SETS>(a.order, blockIdx.x);
+    else if (blockIdx.x - a.order_blocks < a.main_blocks) pack_block<E, GRADIENT ? SETS : 1, GRADIENT>(a.main, blockIdx.x - a.order_blocks, shared);
+    else if (GRADIENT) pack_block<E, 1, false>(a.x, blockIdx.x - a.order_blocks - a.main_blocks, shared);
 }
 
 // ---- the gather ----------------------------------------------------------------------------------

@@ -29,17 +29,17 @@ __device__ __forceinline__ int64_t quotient(int64_t i, uint32_t n) {
 constexpr int kMx4Batch = 4;      // groups of a thread whose loads are in flight together
 
 // Four lanes share a block, eight elements each.  BYTES: what the base and the row stride are multiples of, 16 at most.
-template <class E, int BYTES>
+template <class E, int BYTES, int BATCH>
 __global__ void __launch_bounds__(kMx4Threads) mx4_quantize_kernel(const E *__restrict__ x, int64_t stride, int64_t rows, int cols, int blocks,
                                                                    uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     const int64_t groups = rows * blocks * 4;
-    const int64_t step = (int64_t)gridDim.x * kMx4Threads * kMx4Batch;
+    const int64_t step = (int64_t)gridDim.x * kMx4Threads * BATCH;
     // whole warps stay together for the shuffles
-    for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * kMx4Batch + (threadIdx.x & ~31); first < groups; first += step) {
+    for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * BATCH + (threadIdx.x & ~31); first < groups; first += step) {
         constexpr int PER = BYTES / (int)sizeof(E);
-        Raw<E, PER> part[kMx4Batch][8 / PER];
+        Raw<E, PER> part[BATCH][8 / PER];
 #pragma unroll
-        for (int m = 0; m < kMx4Batch; ++m) {
+        for (int m = 0; m < BATCH; ++m) {
             const int64_t i = first + m * kMx4Threads + (threadIdx.x & 31);
 #pragma unroll
             for (int h = 0; h < 8 / PER; ++h) part[m][h].clear();
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_quantize_kernel(const E *__re
             }
         }
 #pragma unroll
-        for (int m = 0; m < kMx4Batch; ++m) {
+        for (int m = 0; m < BATCH; ++m) {
             const int64_t i = first + m * kMx4Threads + (threadIdx.x & 31);
             float v[8];
             // the largest magnitude as bits: they are ordered as the values are, and NaN and infinity are the largest
@@ -89,18 +89,18 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_quantize_kernel(const E *__re
 }
 
 // Groups of four values (16 bytes of float32, 8 of the 16-bit types).  VECTOR: base and row stride are multiples of that.
-template <class E, bool VECTOR>
+template <class E, bool VECTOR, int BATCH>
 __global__ void __launch_bounds__(kMx4Threads) mx4_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t rows,
                                                                      int cols, int blocks, E *__restrict__ y, int64_t stride) {
     const uint32_t per_row = (uint32_t)(cols + 3) / 4;
     const int64_t groups = rows * per_row;
-    const int64_t step = (int64_t)gridDim.x * kMx4Threads * kMx4Batch;
-    for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * kMx4Batch + threadIdx.x; first < groups; first += step) {
-        uint32_t word[kMx4Batch], scale[kMx4Batch];
-        int64_t row[kMx4Batch];
-        int col[kMx4Batch];
+    const int64_t step = (int64_t)gridDim.x * kMx4Threads * BATCH;
+    for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * BATCH + threadIdx.x; first < groups; first += step) {
+        uint32_t word[BATCH], scale[BATCH];
+        int64_t row[BATCH];
+        int col[BATCH];
 #pragma unroll
-        for (int m = 0; m < kMx4Batch; ++m) {
+        for (int m = 0; m < BATCH; ++m) {
             const int64_t i = min(first + m * kMx4Threads, groups - 1);
             row[m] = quotient(i, per_row);
             col[m] = (int)(i - row[m] * per_row) * 4;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_dequantize_kernel(const uint8
             scale[m] = __ldg(scales + block);
         }
 #pragma unroll
-        for (int m = 0; m < kMx4Batch; ++m) {
+        for (int m = 0; m < BATCH; ++m) {
             if (first + m * kMx4Threads >= groups) break;
             float v[4];
             e2m1_values(word[m], v);
