@@ -29,6 +29,13 @@ struct DeviceTable {
     int outs = 0, rows = 0;
 };
 
+struct DeviceBlocks {
+    uint32_t *chunk_ptr = nullptr, *rows = nullptr, *src = nullptr;
+    int32_t *members = nullptr;
+    int blocks = 0;                 // 0: this direction has none
+    int64_t chunks = 0;
+};
+
 }  // namespace
 
 struct spdnn_topology {
@@ -36,6 +43,7 @@ struct spdnn_topology {
     int device = -1;                // -1: analysis only
     int sm_count = 0;
     DeviceTable forward, backward;
+    DeviceBlocks forward_blocks, backward_blocks;
     int32_t *rows = nullptr;        // canonical
     void *few_rows = nullptr;       // canonical as few_kernel reads them
 };
@@ -91,6 +99,21 @@ cudaError_t upload(DeviceTable &d, const GatherTable &t) {
     return e;
 }
 
+cudaError_t upload(DeviceBlocks &d, const BlockTable &t) {
+    if (!t.blocks) return cudaSuccess;
+    d.blocks = t.blocks; d.chunks = (int64_t)t.chunk_ptr.back();
+    cudaError_t e = upload(&d.chunk_ptr, t.chunk_ptr);
+    if (e == cudaSuccess) e = upload(&d.rows, t.rows);
+    if (e == cudaSuccess) e = upload(&d.src, t.src);
+    if (e == cudaSuccess) e = upload(&d.members, t.members);
+    return e;
+}
+
+void release(DeviceBlocks &d) {
+    cudaFree(d.chunk_ptr); cudaFree(d.rows); cudaFree(d.src); cudaFree(d.members);
+    d = DeviceBlocks();
+}
+
 void release(DeviceTable &d) {
     cudaFree(d.slice_ptr); cudaFree(d.idx); cudaFree(d.src);
     d = DeviceTable();
@@ -122,17 +145,34 @@ struct GatherPlan {
     int v = 1, p = 1, splits = 1;
     int64_t tiles = 0, image_bytes = 0;
     bool global = false;
+    bool blocks = false;            // by blocks, on the tensor cores: 64 tokens per tile
 };
 
 constexpr int64_t kSharedLimit = 227 * 1024;
+#ifndef SPDNN_BLOCK_TOKENS
+#define SPDNN_BLOCK_TOKENS 17
+#endif
 
 int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
 }
 
-GatherPlan plan_gather(const spdnn_topology &top, const DeviceTable &t, int tokens, int sets, int size) {
+// Blocks take 16-bit operands of one type and whole tiles of 64 tokens.
+bool go_by_blocks(const DeviceBlocks &b, int tokens, int image_type, int weight_type) {
+    return b.blocks && tokens >= SPDNN_BLOCK_TOKENS && image_type != F32 && image_type == weight_type;
+}
+
+GatherPlan plan_gather(const spdnn_topology &top, bool forward, int tokens, int sets, int image_type, int weight_type) {
+    const DeviceTable &t = forward ? top.forward : top.backward;
     GatherPlan g;
-    const int full = 16 / size;
+    const int size = type_size(image_type), full = 16 / size;
+    if (go_by_blocks(forward ? top.forward_blocks : top.backward_blocks, tokens, image_type, weight_type)) {
+        g.blocks = true;
+        g.v = 8; g.p = 8;
+        g.image_bytes = image_size(t.rows, sets, 8, 8, 2);
+        g.tiles = ((int64_t)tokens + 63) / 64;
+        return g;
+    }
     bool found = false;
     for (int T = full * 8; T >= 1 && !found; T /= 2) {
         const int v = T < full ? T : full, p = T / v;
@@ -215,6 +255,28 @@ cudaError_t launch_gather(const GatherPlan &g, GatherArgs a, int image_type, int
     return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(threads), args, shared, stream);
 }
 
+// The same gather by blocks; of `a` what is not the gather table's.
+cudaError_t launch_blocks(const spdnn_topology &top, const GatherPlan &g, const DeviceBlocks &b, const GatherArgs &a, int image_type, int s, int sets,
+                          cudaStream_t stream) {
+    BlockArgs k{};
+    k.image = a.image; k.image_bytes = g.image_bytes; k.chunk_ptr = b.chunk_ptr; k.rows = b.rows; k.members = b.members; k.weights = a.weights;
+    k.chunks = b.chunks; k.blocks = b.blocks; k.tokens = a.tokens; k.bias0 = a.bias0; k.bias1 = a.bias1;
+    k.y = a.y; k.z0 = a.z0; k.z1 = a.z1; k.y_stride = a.y_stride; k.z_stride = a.z_stride; k.y_type = a.y_type; k.act = a.act; k.clip = a.clip;
+    k.whole_y = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * type_size(a.y_type) % 16 == 0;
+    k.whole_z = (reinterpret_cast<uintptr_t>(a.z0) | reinterpret_cast<uintptr_t>(a.z1)) % 16 == 0 && a.z_stride % 4 == 0;
+    const auto of = [&](auto e) {
+        using E = decltype(e);
+        return s == 2 ? block_kernel<E, 2, 1> : sets == 2 ? block_kernel<E, 1, 2> : block_kernel<E, 1, 1>;
+    };
+    const auto kernel = image_type == BF16 ? of(bf16()) : of(__half());
+    const int shared = kBlockWarps * kBlockStages * block_stage_bytes(s == 2 ? 1 : sets);
+    const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return e;
+    const int64_t want = ((int64_t)b.blocks * g.tiles + kBlockWarps - 1) / kBlockWarps;
+    void *args[] = {&k};
+    return cudaLaunchKernel((const void *)kernel, dim3((unsigned)std::min<int64_t>(want, top.sm_count)), dim3(kBlockWarps * 32), args, (size_t)shared, stream);
+}
+
 unsigned pack_blocks(const PackArgs &a) { return (unsigned)((int64_t)((a.rows + 63) / 64) * ((a.tokens + 63) / 64)); }
 
 // What a call's gather (and dw_kernel) read.  gradient: the backward call, whose gathered values are dL/dz.
@@ -239,8 +301,14 @@ cudaError_t launch_prepare(const PrepareArgs &args, int x_blocks, int sets, bool
 }
 
 // The part of it that orders a table.
-void order_part(PrepareArgs &args, const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, int slots, int values, int image_type,
-                void *weights, void *index) {
+void order_part(PrepareArgs &args, const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, const DeviceBlocks &b, int slots,
+                int sets, int values, int image_type, void *weights, void *index) {
+    if (g.blocks) {
+        args.by_blocks = 1;
+        args.blocks = OrderBlocksArgs{w0, w1, b.src, b.chunks, slots, weights};
+        args.order_blocks = (unsigned)((b.chunks * 512 * sets + kPackThreads - 1) / kPackThreads);
+        return;
+    }
     OrderArgs &a = args.order;
     a.w0 = w0; a.w1 = w1; a.idx = t.idx; a.src = t.src; a.entries = t.entries; a.slots = slots; a.values = values; a.p = g.p;
     a.whole = g.v * type_size(image_type) == 16; a.wide = g.global;
@@ -270,8 +338,9 @@ struct Workspace {
 Workspace layout(const spdnn_topology &top, const GatherPlan &g, const DeviceTable &t, int tokens, int sets, int image, int weight, bool backward) {
     Workspace w;
     int64_t at = 0;
-    w.weights = at; at += aligned(t.entries * sets * type_size(weight));
-    w.index = at; at += aligned(t.entries * (g.global ? 4 : 2));
+    const DeviceBlocks &b = backward ? top.backward_blocks : top.forward_blocks;
+    w.weights = at; at += aligned((g.blocks ? b.chunks * 512 : t.entries) * sets * type_size(weight));
+    w.index = at; at += g.blocks ? 0 : aligned(t.entries * (g.global ? 4 : 2));
     w.image = at; at += aligned(g.tiles * g.image_bytes);
     if (backward) {
         const int64_t stride = (tokens + 63) / 64 * 64;
@@ -427,14 +496,14 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     }
     const DeviceTable &t = c.top->forward;
     const int it = image_type(c.x->type), wt = ordered_type(c.x->type, c.w[0]->type);
-    const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), 1, type_size(it));
+    const GatherPlan g = plan_gather(*c.top, true, std::max(c.tokens, 1), 1, it, wt);
     const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, it, wt, false);
     if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
     OnDevice guard(c.top->device);
     if (guard.status != cudaSuccess) return fail_cuda(c.err, c.err_len, guard.status);
     char *base = (char *)c.workspace;
     PrepareArgs prep{};
-    order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, 1, it, base + ws.weights, base + ws.index);
+    order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->forward_blocks, h.slots, c.sets, 1, it, base + ws.weights, base + ws.index);
     PackArgs &p = prep.main;
     p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
     p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x);
@@ -448,7 +517,7 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
         a.y = const_cast<void *>(c.y->data); a.y_stride = c.y->stride; a.y_type = c.y->type;
         if (c.z[0]) { a.z0 = (float *)const_cast<void *>(c.z[0]->data); a.z_stride = c.z[0]->stride; }
         if (c.z[1]) a.z1 = (float *)const_cast<void *>(c.z[1]->data);
-        e = launch_gather(g, a, it, wt, 1, c.sets, c.stream);
+        e = g.blocks ? launch_blocks(*c.top, g, c.top->forward_blocks, a, it, 1, c.sets, c.stream) : launch_gather(g, a, it, wt, 1, c.sets, c.stream);
     }
     if (e != cudaSuccess) return fail_cuda(c.err, c.err_len, e);
     return SPDNN_OK;
@@ -481,7 +550,7 @@ int run_backward(const Call &c, const Gradients &d) {
     if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
     if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, kAnalysisOnly);
     const DeviceTable &t = c.top->backward;
-    const GatherPlan g = plan_gather(*c.top, t, std::max(c.tokens, 1), c.sets, type_size(type));
+    const GatherPlan g = plan_gather(*c.top, false, std::max(c.tokens, 1), c.sets, type, type);
     const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, type, type, true);
     if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
     OnDevice guard(c.top->device);
@@ -490,7 +559,7 @@ int run_backward(const Call &c, const Gradients &d) {
     const int64_t stride = ((int64_t)c.tokens + 63) / 64 * 64;
     if (c.tokens > 0 && e == cudaSuccess) {
         PrepareArgs prep{};
-        if (d.dx) order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, h.slots, c.sets, type, base + ws.weights, base + ws.index);
+        if (d.dx) order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->backward_blocks, h.slots, c.sets, c.sets, type, base + ws.weights, base + ws.index);
         PackArgs &p = prep.main;
         p.x = matrix(d.dy);
         if (c.z[0]) { p.z0 = (const float *)c.z[0]->data; p.z_stride = c.z[0]->stride; }
@@ -510,7 +579,7 @@ int run_backward(const Call &c, const Gradients &d) {
         a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
         a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
         a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
-        e = launch_gather(g, a, type, type, c.sets, 1, c.stream);
+        e = g.blocks ? launch_blocks(*c.top, g, c.top->backward_blocks, a, type, c.sets, 1, c.stream) : launch_gather(g, a, type, type, c.sets, 1, c.stream);
     }
     if (d.dw[0] && e == cudaSuccess) {
         if (e == cudaSuccess) {
@@ -557,6 +626,8 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&t->sm_count, cudaDevAttrMultiProcessorCount, device);
         if (e == cudaSuccess) e = upload(t->forward, t->host.forward);
         if (e == cudaSuccess) e = upload(t->backward, t->host.backward);
+        if (e == cudaSuccess) e = upload(t->forward_blocks, t->host.forward_blocks);
+        if (e == cudaSuccess) e = upload(t->backward_blocks, t->host.backward_blocks);
         if (e == cudaSuccess) e = upload(&t->rows, t->host.rows);
         if (e == cudaSuccess) e = upload_few_rows(*t);
         t->device = device;
@@ -567,6 +638,8 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
         // the tables are on the device: only the canonical rows are asked for again
         t->host.forward = GatherTable();
         t->host.backward = GatherTable();
+        t->host.forward_blocks = BlockTable();
+        t->host.backward_blocks = BlockTable();
         *out = t;
         return SPDNN_OK;
     } catch (const std::bad_alloc &) {
@@ -584,6 +657,8 @@ extern "C" void spdnn_topology_destroy(spdnn_topology_t *top) {
         OnDevice guard(top->device);
         release(top->forward);
         release(top->backward);
+        release(top->forward_blocks);
+        release(top->backward_blocks);
         cudaFree(top->rows);
         cudaFree(top->few_rows);
     }
@@ -618,7 +693,7 @@ extern "C" int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, in
         return SPDNN_OK;
     }
     const DeviceTable &t = backward ? top->backward : top->forward;
-    const GatherPlan g = plan_gather(*top, t, std::max(tokens, 1), backward ? sets : 1, type_size(it));
+    const GatherPlan g = plan_gather(*top, !backward, std::max(tokens, 1), backward ? sets : 1, it, wt);
     *bytes = layout(*top, g, t, tokens, sets, it, wt, backward != 0).total;
     return SPDNN_OK;
 }

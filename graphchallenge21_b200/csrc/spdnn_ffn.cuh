@@ -473,11 +473,46 @@ __device__ __forceinline__ void order_block(const OrderArgs &a, unsigned block) 
     else ((uint16_t *)a.index)[e] = (uint16_t)place;
 }
 
+struct OrderBlocksArgs {
+    Matrix w0, w1;
+    const uint32_t *src;        // the block table (topology.h)
+    int64_t chunks;
+    int slots;
+    void *weights;
+};
+
+// The weights of a block table as mma.m16n8k16 takes them for its second operand: of a chunk, per step of 16 rows and per set 16 bytes a
+// lane, the fragments of the block's neurons 0-7 and 8-15.  SPREAD (backward): the sets are planes of their own.
+template <class W, int SETS, bool SPREAD>
+__device__ __forceinline__ void order_blocks_block(const OrderBlocksArgs &a, unsigned block) {
+    const int64_t e = (int64_t)block * kPackThreads + threadIdx.x;
+    if (e >= a.chunks * 512 * SETS) return;
+    const int v = (int)(e & 3), half = (int)(e >> 2 & 1), lane = (int)(e >> 3 & 31);
+    int64_t chunk = e >> 8;                            // [chunk][step][set] or [set][chunk][step]
+    int set = 0;
+    if (!SPREAD) { set = (int)(chunk % SETS); chunk /= SETS; }
+    const int step = (int)(chunk & 1);
+    chunk >>= 1;
+    if (SPREAD) { set = (int)(chunk / a.chunks); chunk -= set * a.chunks; }
+    const int row = step * 16 + (lane & 3) * 2 + (v & 1) + (v >> 1) * 8, neuron = half * 8 + lane / 4;
+    const uint32_t s = __ldg(a.src + (chunk * 32 + row) * 16 + neuron);
+    const Matrix &w = set ? a.w1 : a.w0;
+    float value = 0.0f;
+    if (s != 0xffffffffu) {
+        const uint32_t c = s / (uint32_t)a.slots, j = s % (uint32_t)a.slots;
+        value = w.type == MX4 ? mx4_value((const uint8_t *)w.data, w.scales, w.stride, c, (int)j)
+                              : load_as_float(w.data, w.type, (int64_t)c * w.stride + j);
+    }
+    ((W *)a.weights)[e] = from_float<W>(value);
+}
+
 // Everything that a call lays out, in one launch (a launch takes longer than most of these blocks): the table, then image and columns
 // of the gathered values, then (backward) the columns of x.
 struct PrepareArgs {
     OrderArgs order;
+    OrderBlocksArgs blocks;
     PackArgs main, x;
+    int by_blocks;                          // the gather goes by blocks: their weights are ordered, not the gather table's
     unsigned order_blocks, main_blocks;     // the rest are x's
 };
 
@@ -485,8 +520,10 @@ template <class E, class W, int SETS, bool GRADIENT>
 __global__ void __launch_bounds__(kPackThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
     constexpr int MAIN = pack_tile_bytes<E, GRADIENT ? SETS : 1, GRADIENT>(), X = pack_tile_bytes<E, 1, false>();
     __shared__ __align__(16) unsigned char shared[MAIN > X ? MAIN : X];
-    if (blockIdx.x < a.order_blocks) order_block<W, SETS>(a.order, blockIdx.x);
-    else if (blockIdx.x - a.order_blocks < a.main_blocks) pack_block<E, GRADIENT ? SETS : 1, GRADIENT>(a.main, blockIdx.x - a.order_blocks, shared);
+    if (blockIdx.x < a.order_blocks) {
+        if (!a.by_blocks) order_block<W, SETS>(a.order, blockIdx.x);
+        else if constexpr (sizeof(W) == 2) order_blocks_block<W, SETS, GRADIENT>(a.blocks, blockIdx.x);
+    } else if (blockIdx.x - a.order_blocks < a.main_blocks) pack_block<E, GRADIENT ? SETS : 1, GRADIENT>(a.main, blockIdx.x - a.order_blocks, shared);
     else if (GRADIENT) pack_block<E, 1, false>(a.x, blockIdx.x - a.order_blocks - a.main_blocks, shared);
 }
 
@@ -827,6 +864,238 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
         if (G == 2) y *= u;
         store_from_float(a.y, a.y_type, token * a.y_stride + c, y);
     }
+}
+
+// ---- the gather by blocks ---------------------------------------------------------------------------
+
+struct BlockArgs {
+    const void *image;           // tiles of 64 tokens: rows of 128 bytes per neuron and value
+    int64_t image_bytes;
+    const uint32_t *chunk_ptr, *rows;   // the block table
+    const int32_t *members;
+    const void *weights;         // order_blocks_block's
+    int64_t chunks;
+    int blocks, tokens;
+    const float *bias0, *bias1;
+    void *y;
+    float *z0, *z1;
+    int64_t y_stride, z_stride;
+    int y_type, act;
+    float clip;
+    int whole_y, whole_z;        // rows of y, of z begin on 16 bytes: blocks of 16 neighbours are stored in whole sectors
+};
+
+#ifndef SPDNN_BW
+#define SPDNN_BW 16
+#define SPDNN_BS 2
+#endif
+constexpr int kBlockWarps = SPDNN_BW, kBlockStages = SPDNN_BS;
+__host__ __device__ constexpr int block_stage_bytes(int G) { return 32 * 128 + 1024 * G; }
+
+// Stores 64 tokens x 16 neighbouring neurons of a warp's fragments (value(m, half, i), laid out as block_kernel's accumulators) through 4 KB of
+// shared memory of its own, 16 bytes a lane: fragments hold two neighbours of eight tokens, an eighth of a sector each.
+template <class T, class F>
+__device__ __forceinline__ void store_block(unsigned char *stage, T *to, int64_t stride, int tokens, const F &value) {
+    const int lane = threadIdx.x & 31;
+    constexpr int PIECES = (int)sizeof(T);             // of 16 bytes in a row of 16 neurons (4 or 2), turned against each other by token
+    const auto place = [](int token, int piece) { return token * (16 * PIECES) + ((piece ^ (PIECES == 4 ? token >> 1 & 3 : token >> 2 & 1)) * 16); };
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = m * 16 + i * 8 + lane / 4;
+                const float lo = value(m, half, 2 * i), hi = value(m, half, 2 * i + 1);
+                if constexpr (sizeof(T) == 4) {
+                    *(float2 *)(stage + place(token, half * 2 + (lane >> 1 & 1)) + (lane & 1) * 8) = make_float2(lo, hi);
+                } else {
+                    T both[2] = {from_float<T>(lo), from_float<T>(hi)};
+                    *(uint32_t *)(stage + place(token, half) + (lane & 3) * 4) = *(const uint32_t *)both;
+                }
+            }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2 * PIECES; ++i) {
+        const int token = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+        if (token < tokens) *(uint4 *)((char *)(to + token * stride) + piece * 16) = *(const uint4 *)(stage + place(token, piece));
+    }
+}
+
+template <class E> __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<E, bf16>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void copy_16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// A warp takes 64 tokens of a block (16 neurons over the same rows) at a time: a chunk of 32 rows x 64 tokens and its weights come into the warp's
+// own stages with cp.async, three chunks ahead; ldmatrix.trans turns 16 rows x 16 tokens into a fragment of tokens x rows, wherever the rows
+// came from, and the products (16 tokens x 8 neurons x 16 rows) run on the tensor cores.  One gathered value serves 16 neurons and
+// both sets, where gather_kernel's serves one: what is left is bringing the rows in (each is used by as many blocks as list it) and the results
+// out.  The contraction is 16 wide: mma.sync, not tcgen05, whose tile of 128 tokens and its round trip through tensor memory would have the
+// same bytes to move, and those bound this kernel.
+template <class E, int S, int G>
+__global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_constant__ BlockArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int STAGE = block_stage_bytes(G);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t stages = (uint32_t)__cvta_generic_to_shared(smem) + warp * kBlockStages * STAGE;
+    const unsigned char *stages_ptr = smem + warp * kBlockStages * STAGE;
+    const int tiles = (a.tokens + 63) / 64;
+    const int64_t units = (int64_t)a.blocks * tiles, warps = (int64_t)gridDim.x * kBlockWarps, me = (int64_t)blockIdx.x * kBlockWarps + warp;
+    const int64_t first = units * me / warps, last = units * (me + 1) / warps;
+
+    // where the copies are: unit, chunk of its list, which begins at chunk `begin` and has `count`; S sets one after another
+    int64_t ahead = first;
+    uint32_t begin = 0, count = 0, at = 0;
+    const auto open = [&] {                            // skips blocks without connections
+        for (; ahead < last; ++ahead) {
+            const int b = (int)(ahead / tiles);
+            begin = __ldg(a.chunk_ptr + b);
+            count = __ldg(a.chunk_ptr + b + 1) - begin;
+            at = 0;
+            if (count) return;
+        }
+    };
+    open();
+    uint32_t row = ahead < last ? __ldg(a.rows + (size_t)begin * 32 + lane) : 0u;
+    int fill = 0;
+    const auto request = [&] {
+        if (ahead < last) {
+            const uint32_t set = S == 2 && at >= count ? 1u : 0u, chunk = begin + at - set * count;
+            const char *image = (const char *)a.image + (ahead % tiles) * a.image_bytes;
+            const uint32_t stage = stages + fill * STAGE;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = i * 4 + lane / 8, q = lane & 7;
+                const uint32_t n = __shfl_sync(0xffffffffu, row, k);
+                const uint32_t x = (n & 1u) << 2 | (n & 2u) | (n >> 2 & 1u);           // unit_place's turn
+                copy_16(stage + k * 128 + q * 16, image + ((size_t)n * S + set) * 128 + (((q ^ (k & 7)) ^ x) * 16));
+            }
+            const char *w = (const char *)a.weights + ((size_t)set * a.chunks + chunk) * (1024 * G);
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i) copy_16(stage + 4096 + (i * 32 + lane) * 16, w + (i * 32 + lane) * 16);
+            if (++at == count * S) { ++ahead; open(); }
+            if (ahead < last) row = __ldg(a.rows + (size_t)(begin + (S == 2 && at >= count ? at - count : at)) * 32 + lane);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        fill = fill + 1 == kBlockStages ? 0 : fill + 1;
+    };
+    for (int i = 0; i + 1 < kBlockStages; ++i) request();
+
+    int drain = 0;
+    for (int64_t unit = first; unit < last; ++unit) {
+        const int b = (int)(unit / tiles);
+        const uint32_t chunks = (__ldg(a.chunk_ptr + b + 1) - __ldg(a.chunk_ptr + b)) * S;
+        float acc[4][2 * G][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int f = 0; f < 2 * G; ++f)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[m][f][k] = 0.0f;
+        for (uint32_t c = 0; c < chunks; ++c) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kBlockStages - 2) : "memory");
+            __syncwarp();
+            request();                                 // into the stage that was drained last
+            const uint32_t stage = stages + drain * STAGE;
+            const unsigned char *w = stages_ptr + drain * STAGE + 4096;
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                uint4 frag[G];
+#pragma unroll
+                for (int g = 0; g < G; ++g) frag[g] = *(const uint4 *)(w + ((step * G + g) * 32 + lane) * 16);
+                const int r = lane & 7, k = step * 16 + (lane >> 4) * 8 + r;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    uint32_t x[4];
+                    const int unit_of = m * 2 + (lane >> 3 & 1);
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(stage + k * 128 + ((unit_of ^ r) * 16)) : "memory");
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        mma_16x8x16<E>(acc[m][2 * g], x, frag[g].x, frag[g].y);
+                        mma_16x8x16<E>(acc[m][2 * g + 1], x, frag[g].z, frag[g].w);
+                    }
+                }
+            }
+            __syncwarp();
+            drain = drain + 1 == kBlockStages ? 0 : drain + 1;
+        }
+        // acc[m][2 g + half][i]: token 16 m + lane / 4 + 8 (i / 2), neuron 8 half + 2 (lane % 4) + i % 2
+        const int64_t tile0 = (unit % tiles) * 64;
+        const int tokens = (int)min((int64_t)64, a.tokens - tile0);
+        const int32_t *members = a.members + (size_t)b * 16;
+        const int head = __ldg(members);
+        // sixteen neighbours, on 16 bytes of any type
+        const bool neighbours = __ldg(members + 15) - head == 15 && head % 8 == 0;
+        // the stage that was drained last is free until the next request
+        unsigned char *scratch = smem + warp * kBlockStages * STAGE + (drain == 0 ? kBlockStages - 1 : drain - 1) * STAGE;
+        int2 c[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            c[half] = __ldg((const int2 *)(members + half * 8) + (lane & 3));
+            float b0[2] = {0, 0}, b1[2] = {0, 0};
+            if (a.bias0) { if (c[half].x >= 0) b0[0] = __ldg(a.bias0 + c[half].x); if (c[half].y >= 0) b0[1] = __ldg(a.bias0 + c[half].y); }
+            if (G == 2 && a.bias1) { if (c[half].x >= 0) b1[0] = __ldg(a.bias1 + c[half].x); if (c[half].y >= 0) b1[1] = __ldg(a.bias1 + c[half].y); }
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[m][half][i] += b0[i & 1];
+                    if (G == 2) acc[m][2 * G - 2 + half][i] += b1[i & 1];
+                }
+        }
+        const auto store = [&](auto *to, int64_t stride, bool whole, const auto &value) {
+            to += tile0 * stride;
+            if (whole && neighbours) {
+                store_block(scratch, to + head, stride, tokens, value);
+                return;
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int token = m * 16 + i / 2 * 8 + lane / 4, neuron = i & 1 ? c[half].y : c[half].x;
+                        if (token < tokens && neuron >= 0) to[token * stride + neuron] = from_float<typename std::remove_pointer<decltype(to)>::type>(value(m, half, i));
+                    }
+        };
+        if (a.z0) {
+            store(a.z0, a.z_stride, a.whole_z, [&](int m, int half, int i) { return acc[m][half][i]; });
+            if (G == 2) store(a.z1, a.z_stride, a.whole_z, [&](int m, int half, int i) { return acc[m][2 * G - 2 + half][i]; });
+        }
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][half][i] = activate<true>(acc[m][half][i], act.value, a.clip);
+        });
+        if (G == 2)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][half][i] *= acc[m][2 * G - 2 + half][i];
+        const auto result = [&](int m, int half, int i) { return acc[m][half][i]; };
+        if (a.y_type == F32) store((float *)a.y, a.y_stride, a.whole_y, result);
+        else if (a.y_type == F16) store((__half *)a.y, a.y_stride, a.whole_y, result);
+        else store((bf16 *)a.y, a.y_stride, a.whole_y, result);
+        __syncwarp();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---- gradients of the weights ----------------------------------------------------------------------

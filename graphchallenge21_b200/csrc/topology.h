@@ -12,6 +12,7 @@
 #include <new>
 #include <string>
 #include <thread>
+#include <unordered_map>
 #include <vector>
 
 namespace spdnn_impl {
@@ -30,6 +31,16 @@ struct GatherTable {
     std::vector<uint32_t> src;         // [quads][32][4] position in the canonical weights, kNoSource = padding
 };
 
+// Gathering neurons that gather the SAME rows (the 16 outputs of a butterfly's block), up to 16 to a block: a small dense product, which the
+// tensor cores take.  Rows in chunks of 32, chunk by chunk.
+struct BlockTable {
+    int blocks = 0;                    // 0: not worth it (too few neurons share their rows)
+    std::vector<uint32_t> chunk_ptr;   // [blocks + 1] first chunk of a block
+    std::vector<uint32_t> rows;        // [chunks][32] gathered row, padding = the row of zeros
+    std::vector<uint32_t> src;         // [chunks][32][16] position in the canonical weights, kNoSource = padding
+    std::vector<int32_t> members;      // [blocks][16] gathering neuron, -1 = none
+};
+
 struct Topology {
     int inputs = 0, outputs = 0;
     int slots = 0;                     // connections per output neuron, at least 1
@@ -37,11 +48,17 @@ struct Topology {
     int64_t connections = 0;
     std::vector<int32_t> rows;         // [outputs][slots] ascending input per output, -1 behind the last
     GatherTable forward, backward;
+    BlockTable forward_blocks, backward_blocks;
 };
 
 // Most entries of a gather table (4 bytes of index, 4 of source): a slice is as long as its longest neuron.
 constexpr int64_t kMostEntries = 1ll << 30;
 constexpr int kMostSlots = 4096;       // as canonicalize_layer
+// Blocks are used where their products have at most this many times the connections.
+#ifndef SPDNN_BLOCK_WASTE
+#define SPDNN_BLOCK_WASTE 4
+#endif
+constexpr int64_t kBlockWaste = SPDNN_BLOCK_WASTE;
 
 // Orders the connections of `lanes` (2, 4, 8 or 16) neighbouring neurons, whose lanes read their k-th connections at the same time, so
 // that those fall on different banks: into steps in which the gathered rows belong to different CLASSES, row mod `lanes` (spdnn_ffn.cuh
@@ -192,6 +209,65 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
     return "";
 }
 
+// The blocks of a gather.  start[i]: where the entries of neuron i begin in row_of / source_of (start has outs + 1 entries).
+template <class Row, class Source>
+inline void build_block_table(int outs, int rows, const std::vector<size_t> &start, const Row &row_of, const Source &source_of, BlockTable &t) {
+    const auto length = [&](int i) { return start[i + 1] - start[i]; };
+    std::unordered_map<uint64_t, int> newest;          // hash of a list -> the class that was opened last for it
+    std::vector<int> first, older;                     // of a class: its first neuron; the class before it with the same hash
+    std::vector<std::vector<int32_t>> members;
+    const auto same = [&](int i, int j) {
+        if (length(i) != length(j)) return false;
+        for (size_t k = 0; k < length(i); ++k)
+            if (row_of(start[i] + k) != row_of(start[j] + k)) return false;
+        return true;
+    };
+    for (int i = 0; i < outs; ++i) {
+        uint64_t h = 0x9E3779B97F4A7C15ull ^ length(i);
+        for (size_t k = start[i]; k < start[i + 1]; ++k) h = (h ^ row_of(k)) * 0xBF58476D1CE4E5B9ull, h ^= h >> 29;
+        const auto found = newest.find(h);
+        int c = found == newest.end() ? -1 : found->second;
+        while (c >= 0 && !same(first[c], i)) c = older[c];
+        if (c < 0) {
+            c = (int)first.size();
+            // mostly neurons of their own: no use in reading on
+            if (c >= 1024 && (int64_t)c * 2 > i) return;
+            first.push_back(i);
+            older.push_back(found == newest.end() ? -1 : found->second);
+            members.emplace_back();
+            newest[h] = c;
+        }
+        members[c].push_back(i);
+    }
+    int64_t chunks = 0, blocks = 0;
+    for (size_t c = 0; c < first.size(); ++c) {
+        const int64_t b = ((int64_t)members[c].size() + 15) / 16;
+        blocks += b;
+        chunks += b * (int64_t)((length(first[c]) + 31) / 32);
+    }
+    const int64_t entries = (int64_t)start[outs];
+    if (!entries || chunks * 512 > entries * kBlockWaste) return;
+    t.blocks = (int)blocks;
+    t.chunk_ptr.assign(1, 0);
+    t.chunk_ptr.reserve(blocks + 1);
+    t.rows.assign((size_t)chunks * 32, (uint32_t)rows);
+    t.src.assign((size_t)chunks * 512, kNoSource);
+    t.members.assign((size_t)blocks * 16, -1);
+    size_t block = 0, chunk = 0;
+    for (size_t c = 0; c < first.size(); ++c)
+        for (size_t m = 0; m < members[c].size(); m += 16, ++block) {
+            const size_t n = length(first[c]);
+            for (size_t k = 0; k < n; ++k) {
+                t.rows[chunk * 32 + k] = row_of(start[first[c]] + k);
+                for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j)
+                    t.src[(chunk * 32 + k) * 16 + (j - m)] = source_of(start[members[c][j]] + k);
+            }
+            for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j) t.members[block * 16 + (j - m)] = members[c][j];
+            chunk += (n + 31) / 32;
+            t.chunk_ptr.push_back((uint32_t)chunk);
+        }
+}
+
 // Returns an empty string on success, else the reason the topology is rejected.
 // forward_lanes, backward_lanes: see BankOrder.
 inline std::string build_topology(int inputs, int outputs, const int32_t *col_ptr, const int32_t *row_idx, int forward_lanes, int backward_lanes,
@@ -232,16 +308,23 @@ inline std::string build_topology(int inputs, int outputs, const int32_t *col_pt
         for (uint32_t k = 0; k < in_count[c]; ++k) emit((uint32_t)r[k], (uint32_t)((size_t)c * most + k));
     }, forward_lanes, t.forward);
     if (!why.empty()) return why;
+    std::vector<size_t> in_start((size_t)outputs + 1, 0);
+    for (int c = 0; c < outputs; ++c) in_start[c + 1] = (size_t)col_ptr[c + 1];
     // the transposed lists, outputs ascending
     std::vector<size_t> start((size_t)inputs + 1, 0);
     for (int i = 0; i < inputs; ++i) start[i + 1] = start[i] + out_count[i];
-    std::vector<uint32_t> by_input((size_t)nnz);
+    std::vector<uint32_t> by_input((size_t)nnz), flat((size_t)nnz);
     std::vector<size_t> at(start.begin(), start.end() - 1);
     for (int c = 0; c < outputs; ++c)
         for (uint32_t k = 0; k < in_count[c]; ++k) {
             const size_t p = (size_t)c * most + k;
             by_input[at[t.rows[p]]++] = (uint32_t)p;
+            flat[in_start[c] + k] = (uint32_t)p;
         }
+    build_block_table(outputs, inputs, in_start, [&](size_t e) { return (uint32_t)t.rows[flat[e]]; }, [&](size_t e) { return flat[e]; },
+                      t.forward_blocks);
+    build_block_table(inputs, outputs, start, [&](size_t e) { return by_input[e] / (uint32_t)most; }, [&](size_t e) { return by_input[e]; },
+                      t.backward_blocks);
     return build_gather_table(inputs, outputs, out_count, [&](int i, auto emit) {
         for (size_t e = start[i]; e < start[i + 1]; ++e) emit(by_input[e] / (uint32_t)most, by_input[e]);
     }, backward_lanes, t.backward);

@@ -453,3 +453,57 @@ def test_a_workspace_that_is_too_small_is_refused():
     assert call(16, n.value) == -1 and b"aligned" in err.value
     assert call(0, n.value) == 0
     torch.cuda.synchronize()
+
+
+# ---- neurons that share their inputs -------------------------------------------------------------
+
+def shared_rows(inputs, outputs, slots, group, scattered, seed=0):
+    """[outputs, slots]: groups of `group` outputs read the same inputs, every input is read by whole groups of inputs too where the
+    sizes allow it (a butterfly); scattered: both sides renumbered at random.  One group reads nothing."""
+    rng = np.random.default_rng(seed)
+    groups = (outputs + group - 1) // group
+    base = np.stack([np.sort(rng.permutation(inputs // group)[: (slots + group - 1) // group]) for _ in range(groups)])
+    rows = (base[:, :, None] * group + np.arange(group)).reshape(groups, -1)[:, :slots]
+    rows[groups // 2] = -1
+    rows = np.repeat(rows, group, axis=0)[:outputs]
+    if scattered:
+        renumber = rng.permutation(inputs)
+        rows = np.where(rows < 0, -1, renumber[rows])
+        rows = rows[rng.permutation(outputs)]
+    return rows
+
+
+class Shared(Problem):
+    def __init__(self, tokens, inputs, outputs, slots, dtype, sets, group, scattered, seed=0):
+        from graphchallenge21_b200 import SparseTopology
+        super().__init__(tokens, inputs, outputs, slots, dtype, sets)
+        self.top = SparseTopology.from_rows(shared_rows(inputs, outputs, slots, group, scattered, seed), inputs)
+        self.rows = self.top.rows()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("sets", [1, 2])
+@pytest.mark.parametrize("tokens, inputs, outputs, slots, group, scattered", [
+    (17, 256, 320, 32, 16, False), (64, 256, 320, 32, 16, True), (65, 512, 100, 48, 16, False), (200, 128, 96, 20, 10, True),
+    (130, 1024, 1024, 32, 16, True), (77, 300, 333, 45, 15, False), (64, 64, 33, 32, 32, False), (31, 96, 1600, 8, 8, False),
+])
+def test_steps_of_neurons_that_share_their_inputs(tokens, inputs, outputs, slots, group, scattered, sets, dtype):
+    check_step(Shared(tokens, inputs, outputs, slots, dtype, sets, group, scattered), "gelu")
+
+
+def test_the_challenge_networks_butterfly():
+    from graphchallenge21_b200 import SparseTopology, mx4_quantize
+    from graphchallenge21_b200.generator import SyntheticNetwork
+    p = Problem(150, 1024, 1024, 32, BF16, 2)
+    cp, ri, _ = SyntheticNetwork(1024, 3, "radix16").layer_csc(2)
+    p.top = SparseTopology(1024, 1024, cp, ri)
+    p.rows = p.top.rows()
+    check_step(p, "silu")
+    q = [mx4_quantize(w) for w in p.w]
+    x4 = mx4_quantize(p.x)
+    for x, t in ((p.x, BF16), (x4, F32)):
+        f = p.reference("silu", x=x if x is p.x else x4.dequantize(), w=[m.dequantize() for m in q], out_dtype=t)
+        check(p.forward("silu", x=x, w=q, out_dtype=t), f.y, f.bound, "y")
+    out = torch.full((150, 1030), 5.0, dtype=BF16, device="cuda")
+    p.forward("silu", out=out[:, 1:1025])
+    assert torch.equal(out[:, 1:1025], p.forward("silu")) and (out[:, 0] == 5).all() and (out[:, 1025:] == 5).all()
