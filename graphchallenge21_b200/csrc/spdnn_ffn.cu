@@ -302,18 +302,18 @@ cudaError_t launch_prepare(const PrepareArgs &args, int x_blocks, int sets, bool
 
 // The part of it that orders a table.
 void order_part(PrepareArgs &args, const GatherPlan &g, const Matrix &w0, const Matrix &w1, const DeviceTable &t, const DeviceBlocks &b, int slots,
-                int sets, int values, int image_type, void *weights, void *index) {
+                int values, int image_type, void *weights, void *index) {
     if (g.blocks) {
         args.by_blocks = 1;
         args.blocks = OrderBlocksArgs{w0, w1, b.src, b.chunks, slots, weights};
-        args.order_blocks = (unsigned)((b.chunks * 512 * sets + kPackThreads - 1) / kPackThreads);
+        args.order_blocks = (unsigned)((b.chunks * 64 + kPackThreads - 1) / kPackThreads);
         return;
     }
     OrderArgs &a = args.order;
     a.w0 = w0; a.w1 = w1; a.idx = t.idx; a.src = t.src; a.entries = t.entries; a.slots = slots; a.values = values; a.p = g.p;
     a.whole = g.v * type_size(image_type) == 16; a.wide = g.global;
     a.weights = weights; a.index = index;
-    args.order_blocks = (unsigned)((t.entries + kPackThreads - 1) / kPackThreads);
+    args.order_blocks = (unsigned)((t.entries / 4 + kPackThreads - 1) / kPackThreads);
 }
 
 // The type activations have in an image, and weights in a gather table's order.  Microscaled values are exact in bf16 (two bits of
@@ -503,10 +503,10 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     if (guard.status != cudaSuccess) return fail_cuda(c.err, c.err_len, guard.status);
     char *base = (char *)c.workspace;
     PrepareArgs prep{};
-    order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->forward_blocks, h.slots, c.sets, 1, it, base + ws.weights, base + ws.index);
+    order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->forward_blocks, h.slots, 1, it, base + ws.weights, base + ws.index);
     PackArgs &p = prep.main;
     p.x = matrix(c.x); p.image = base + ws.image; p.image_bytes = g.image_bytes;
-    p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x);
+    p.rows = h.inputs; p.tokens = c.tokens; p.v = g.v; p.p = g.p; p.vector = on_16_bytes(c.x); p.same = p.vector && c.x->type == it;
     prep.main_blocks = pack_blocks(p);
     cudaError_t e = launch_prepare(prep, 0, c.sets, false, it, wt, c.stream);
     if (e == cudaSuccess) {
@@ -559,7 +559,7 @@ int run_backward(const Call &c, const Gradients &d) {
     const int64_t stride = ((int64_t)c.tokens + 63) / 64 * 64;
     if (c.tokens > 0 && e == cudaSuccess) {
         PrepareArgs prep{};
-        if (d.dx) order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->backward_blocks, h.slots, c.sets, c.sets, type, base + ws.weights, base + ws.index);
+        if (d.dx) order_part(prep, g, matrix(c.w[0]), matrix(c.w[1]), t, c.top->backward_blocks, h.slots, c.sets, type, base + ws.weights, base + ws.index);
         PackArgs &p = prep.main;
         p.x = matrix(d.dy);
         if (c.z[0]) { p.z0 = (const float *)c.z[0]->data; p.z_stride = c.z[0]->stride; }
@@ -570,7 +570,7 @@ int run_backward(const Call &c, const Gradients &d) {
         p.columns = d.dw[0] ? base + ws.d_columns : nullptr; p.token_stride = stride;
         prep.main_blocks = p.image || p.columns ? pack_blocks(p) : 0;
         PackArgs &x = prep.x;
-        x.x = matrix(c.x); x.rows = h.inputs; x.tokens = c.tokens; x.v = x.p = 1; x.vector = on_16_bytes(c.x);
+        x.x = matrix(c.x); x.rows = h.inputs; x.tokens = c.tokens; x.v = x.p = 1; x.vector = on_16_bytes(c.x); x.same = x.vector;
         x.columns = base + ws.x_columns; x.token_stride = stride;
         e = launch_prepare(prep, d.dw[0] ? pack_blocks(x) : 0, c.sets, true, type, type, c.stream);
     }

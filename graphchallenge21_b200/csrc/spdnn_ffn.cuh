@@ -96,13 +96,34 @@ template <bool FAST> __device__ __forceinline__ float sigmoid_times(float v, flo
     return v * r;
 }
 
+// The normal distribution at v and its density, FAST: the tail by formula 7.1.26 of Abramowitz and Stegun (erf off by 1.5e-7 at most), whose
+// exponential is the density's.
+template <bool FAST> __device__ __forceinline__ void normal(float v, float &phi, float &density) {
+    if (!FAST) {
+        phi = 0.5f * (1.0f + erff(v * kInvSqrt2));
+        density = kInvSqrt2Pi * expf(-0.5f * v * v);
+        return;
+    }
+    float e, t;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * v * (-0.5f * 1.44269504088896341f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fabsf(v), 0.3275911f * kInvSqrt2, 1.0f)));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * e;
+    phi = v >= 0.0f ? 1.0f - tail : tail;
+    density = kInvSqrt2Pi * e;
+}
+
 // A NaN stays one (v < 0 is false for it).
 template <bool FAST> __device__ __forceinline__ float activate(float v, int act, float clip) {
     switch (act) {
         case RELU: return v < 0.0f ? 0.0f : v;
         case CLIP: return v < 0.0f ? 0.0f : v > clip ? clip : v;
         case SILU: return sigmoid_times<FAST>(v, v);
-        case GELU: return 0.5f * v * (1.0f + erff(v * kInvSqrt2));
+        case GELU: {
+            float phi, density;
+            normal<FAST>(v, phi, density);
+            return v * phi;
+        }
         case GELU_TANH: return sigmoid_times<FAST>(v, 2.0f * kGeluA * (v + kGeluB * v * v * v));
         default: return v;
     }
@@ -125,8 +146,9 @@ template <bool FAST> __device__ __forceinline__ void activate_both(float v, int 
             return;
         }
         case GELU: {
-            const float h = 0.5f * (1.0f + erff(v * kInvSqrt2));
-            value = v * h; slope = h + v * kInvSqrt2Pi * expf(-0.5f * v * v);
+            float phi, density;
+            normal<FAST>(v, phi, density);
+            value = v * phi; slope = phi + v * density;
             return;
         }
         case GELU_TANH: {
@@ -135,6 +157,18 @@ template <bool FAST> __device__ __forceinline__ void activate_both(float v, int 
             return;
         }
         default: value = v; slope = 1.0f;
+    }
+}
+
+// Calls f with the activation as a constant; not at all for NONE.
+template <class F> __device__ __forceinline__ void with_activation(int act, const F &f) {
+    switch (act) {
+        case RELU: f(std::integral_constant<int, RELU>()); return;
+        case CLIP: f(std::integral_constant<int, CLIP>()); return;
+        case SILU: f(std::integral_constant<int, SILU>()); return;
+        case GELU: f(std::integral_constant<int, GELU>()); return;
+        case GELU_TANH: f(std::integral_constant<int, GELU_TANH>()); return;
+        default: return;
     }
 }
 
@@ -281,6 +315,7 @@ struct PackArgs {
     int rows, tokens;
     int v, p;              // the image's unit and units per neuron (powers of two)
     int vector;            // every row of every operand begins on 16 bytes
+    int same;              // x has the image's type, its rows begin on 16 bytes
     int act;
     float clip;
 };
@@ -290,7 +325,7 @@ constexpr int kPackThreads = 256;
 // The tile of a block: a row of 64 tokens and 16 bytes for every set and neuron; of gradients in float32.
 template <class E, int SETS, bool GRADIENT> __host__ __device__ constexpr int pack_tile_bytes() {
     using Tile = typename std::conditional<GRADIENT, float, E>::type;
-    return SETS * 64 * (64 + 16 / (int)sizeof(Tile)) * (int)sizeof(Tile);
+    return SETS * 64 * (64 + 16 / (int)sizeof(Tile)) * (int)sizeof(Tile) + (sizeof(E) == 2 && !GRADIENT ? 64 * 128 : 0);
 }
 
 // `COUNT` neighbours of a row as floats, from column `col` on; zeros behind `cols`.
@@ -330,23 +365,58 @@ __device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int6
     for (int k = 0; k < COUNT; ++k) v[k] = col + k < cols ? load_as_float(x.data, x.type, row * x.stride + col + k) : 0.0f;
 }
 
+template <class E> __device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {
+    if constexpr (std::is_same<E, bf16>::value) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    } else {
+        const __half2 p = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    }
+}
+
+// COUNT neighbours of the tile (on their natural alignment) as values of type E, in words; one 16-bit value: in the low half.
+template <class E, int COUNT, class Tile> __device__ __forceinline__ void tile_words(const Tile *p, uint32_t *w) {
+    if constexpr (sizeof(Tile) == sizeof(E)) {
+        Raw<E, COUNT> r;
+        r.load(p);
+#pragma unroll
+        for (int i = 0; i < (COUNT * (int)sizeof(E) + 3) / 4; ++i) w[i] = r.w[i];
+    } else if constexpr (COUNT == 1) {
+        w[0] = pair_bits<E>(*p, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; i += 2) {
+            const float2 v = *(const float2 *)(p + i);
+            w[i / 2] = pair_bits<E>(v.x, v.y);
+        }
+    }
+}
+
 // The units of fewer than 16 bytes of a block's neurons: 16 bytes at a time.  (An image is whole groups of 16 bytes, and so is what the
 // 64 neurons before n0 take.)
 template <class E, int SETS, int V, class Tile, class At>
 __device__ __forceinline__ void small_units(char *image, int64_t image_bytes, int parts, const Tile &tile, const At &at, int n0, int n_end,
                                             uint32_t units, int rows) {
-    constexpr int N = 16 / (int)sizeof(E);
+    constexpr int N = 16 / (int)sizeof(E), PIECES = N / V;
     const int first = (int)((uint32_t)n0 * SETS * V / N);
     const int here = (int)(min((uint32_t)(n0 + n_end) * SETS, units) * V / N) - first;
+    const int log_here = n_end == 64 ? 31 - __clz(here) : 0;              // 64 neurons: a power of two
     for (int i = threadIdx.x; i < parts * here; i += kPackThreads) {
-        const int part = i / here, g = first + i - part * here;
-        E e[N];
+        const int part = log_here ? i >> log_here : i / here, g = i - part * here;
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int q = (g * N + k) / V, n = q / SETS - n0, s = q % SETS;
-            e[k] = from_float<E>(n < 64 && n0 + n < rows ? to_float(tile[s][n & 63][at(n & 63, part * V + k % V)]) : 0.0f);
+        for (int k = 0; k < PIECES; ++k) {
+            const int q = g * PIECES + k, n = q / SETS, s = q % SETS;
+            uint32_t v[2] = {0, 0};
+            if (n < 64 && n0 + n < rows) tile_words<E, V>(&tile[s][n][at(n, part * V)], v);
+            constexpr int WORDS = V * (int)sizeof(E) / 4;
+            if constexpr (WORDS == 0) w[k / 2] |= v[0] << (16 * (k & 1)) & (k & 1 ? 0xffff0000u : 0xffffu);
+            else
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) w[k * WORDS + j] = v[j];
         }
-        ((uint4 *)(image + part * image_bytes))[g] = *(const uint4 *)e;
+        ((uint4 *)(image + part * image_bytes))[first + g] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -358,13 +428,47 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
     constexpr int N = 16 / (int)sizeof(E);            // neurons a thread loads at a time
     constexpr int G = 16 / (int)sizeof(Tile);         // tokens of a permuted group
     constexpr int ROW = 64 + G;
-    static_assert(sizeof(Tile[SETS][64][ROW]) == pack_tile_bytes<E, SETS, GRADIENT>(), "the tile");
+    static_assert(sizeof(Tile[SETS][64][ROW]) <= pack_tile_bytes<E, SETS, GRADIENT>(), "the tile");
     Tile (&tile)[SETS][64][ROW] = *reinterpret_cast<Tile (*)[SETS][64][ROW]>(shared);
     const auto at = [](int n, int t) { return t ^ (((n / N) & (64 / G - 1)) * G); };
     const int blocks_n = (a.rows + 63) / 64;
     const int n0 = (int)(block % blocks_n) * 64;
     const int t0 = (int)(block / blocks_n) * 64;
-    for (int i = threadIdx.x; i < 64 * 64 / N; i += kPackThreads) {
+    bool loaded = false;
+    if constexpr (sizeof(E) == 2 && !GRADIENT) {
+        // 16-bit values that stay as they are: rows come in with cp.async (behind the tile) and are turned by ldmatrix.trans, eight
+        // tokens x eight neurons at a time, without a value passing through the ALU
+        if (a.same && n0 + 64 <= a.rows) {
+            loaded = true;
+            const uint32_t rows = (uint32_t)__cvta_generic_to_shared(shared + sizeof(Tile[SETS][64][ROW]));
+            const uint16_t *x = (const uint16_t *)a.x.data;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = i * 32 + threadIdx.x / 8, q = threadIdx.x & 7;
+                const int64_t row = min(t0 + t, a.tokens - 1);
+                const int bytes = t0 + t < a.tokens ? 16 : 0;         // zeros behind the last token
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(rows + t * 128 + ((q ^ (t & 7)) * 16)),
+                             "l"(x + row * a.x.stride + n0 + q * 8), "r"(bytes) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();
+            const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;      // of eight tokens
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w[4];
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(rows + (group * 8 + (lane & 7)) * 128 + (((i * 4 + lane / 8) ^ (lane & 7)) * 16)) : "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int n = (i * 4 + k) * 8 + lane / 4;
+                    *(uint32_t *)&tile[0][n][at(n, group * 8) + (lane & 3) * 2] = w[k];
+                }
+            }
+        }
+    }
+    for (int i = loaded ? 64 * 64 : threadIdx.x; i < 64 * 64 / N; i += kPackThreads) {
         const int t = i / (64 / N), n = i % (64 / N) * N;
         float d0[N], d1[N];
 #pragma unroll
@@ -374,20 +478,27 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
             const int col = n0 + n;
             load_row_part<N>(a.x, a.vector, row, col, a.rows, d0);
             if constexpr (GRADIENT) {
-                float g[N], u[N];
+                float g[N], u[N], dy[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) dy[k] = d0[k];
                 const bool saved = SETS == 2 || a.act != NONE;
                 if (saved) load_row_part<N>(Matrix{a.z0, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, g);
                 if (SETS == 2) load_row_part<N>(Matrix{a.z1, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, u);
-                if (saved) {
+                if (SETS == 2) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) { d1[k] = d0[k] * g[k]; u[k] *= d0[k]; d0[k] = u[k]; }       // NONE
+                }
+                with_activation(a.act, [&](auto act) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
                         float value, slope;
-                        activate_both<sizeof(E) == 2>(g[k], a.act, a.clip, value, slope);
-                        if (SETS == 2) { d1[k] = d0[k] * value; slope *= u[k]; }
+                        activate_both<sizeof(E) == 2>(g[k], act.value, a.clip, value, slope);
+                        if (SETS == 2) d1[k] = dy[k] * value;
                         d0[k] *= slope;
-                        if (col + k >= a.rows) d0[k] = d1[k] = 0.0f;
                     }
-                }
+                });
+                // behind the last neuron there is nothing to be read but zeros
+
             }
         }
 #pragma unroll
@@ -407,21 +518,21 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
         const int parts = (int)min((int64_t)(64 / T), tiles - tile0);
         if (a.v == N) {
             const int units_here = min(n_end * per_row, (int)(units - (uint32_t)n0 * per_row));
+            const int log_units = n_end == 64 ? 31 - __clz(units_here) : 0;        // 64 neurons: a power of two
             for (int i = threadIdx.x; i < parts * units_here; i += kPackThreads) {
-                const int part = i / units_here, u = i - part * units_here;
+                const int part = log_units ? i >> log_units : i / units_here, u = i - part * units_here;
                 const int p = u & (a.p - 1), s = (u >> log_p) & (SETS - 1), n = (u >> log_p) / SETS;
                 const int t = part * T + p * N;
-                uint4 r = make_uint4(0, 0, 0, 0);
+                uint32_t w[4] = {0, 0, 0, 0};
                 if (n < 64 && n0 + n < a.rows) {
-                    if constexpr (!GRADIENT || sizeof(E) == 4) {
-                        r = *(const uint4 *)&tile[s][n][at(n, t)];
+                    if constexpr (sizeof(Tile) == sizeof(E)) {
+                        tile_words<E, N>(&tile[s][n][at(n, t)], w);
                     } else {
-                        const float4 lo = *(const float4 *)&tile[s][n][at(n, t)], hi = *(const float4 *)&tile[s][n][at(n, t + 4)];
-                        E e[8] = {from_float<E>(lo.x), from_float<E>(lo.y), from_float<E>(lo.z), from_float<E>(lo.w),
-                                  from_float<E>(hi.x), from_float<E>(hi.y), from_float<E>(hi.z), from_float<E>(hi.w)};
-                        r = *(const uint4 *)e;
+                        tile_words<E, 4>(&tile[s][n][at(n, t)], w);
+                        tile_words<E, 4>(&tile[s][n][at(n, t + 4)], w + 2);
                     }
                 }
+                const uint4 r = make_uint4(w[0], w[1], w[2], w[3]);
                 ((uint4 *)((char *)a.image + (tile0 + part) * a.image_bytes))[unit_place(n0 + n, per_row) ^ (uint32_t)(s * a.p + p)] = r;
             }
         } else {
@@ -432,11 +543,14 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
         }
     }
     if (a.columns) {
-        for (int i = threadIdx.x; i < SETS * 64 * (64 / G); i += kPackThreads) {
-            const int t = i % (64 / G) * G, n = i / (64 / G) % 64, s = i / (64 / G) / 64;
-            if (n0 + n >= a.rows) continue;
-            Tile *to = (Tile *)a.columns + ((int64_t)(n0 + n) * SETS + s) * a.token_stride + t0 + t;
-            *(uint4 *)to = *(const uint4 *)&tile[s][n][at(n, t)];
+        // columns (n, s) are rows of token_stride one after another
+        constexpr int STEP = kPackThreads / (64 / G);
+        const int t = threadIdx.x % (64 / G) * G, q0 = threadIdx.x / (64 / G);
+        Tile *to = (Tile *)a.columns + ((int64_t)n0 * SETS + q0) * a.token_stride + t0 + t;
+#pragma unroll
+        for (int q = 0; q < SETS * 64; q += STEP, to += STEP * a.token_stride) {
+            const int n = (q + q0) / SETS, s = (q + q0) % SETS;
+            if (n0 + n < a.rows) *(uint4 *)to = *(const uint4 *)&tile[s][n][at(n, t)];
         }
     }
 }
@@ -451,26 +565,50 @@ struct OrderArgs {
     void *weights, *index;      // [quads][32][4][sets], [quads][32][4]
 };
 
+// Bits of the weight at canonical position s, as W.  A caller's matrix has W's type or is microscaled.  Where its rows follow one another
+// without gaps the position is the address; the division is for the others.
+template <class W> __device__ __forceinline__ uint32_t weight_bits(const Matrix &m, uint32_t s, int slots) {
+    if (s == 0xffffffffu) return 0u;
+    if (m.type == MX4) {
+        uint32_t c = s / (uint32_t)slots, j = s - c * (uint32_t)slots;
+        const float v = mx4_value((const uint8_t *)m.data, m.scales, m.stride, c, (int)j);
+        if constexpr (sizeof(W) == 4) return __float_as_uint(v);
+        else return pair_bits<W>(v, 0.0f) & 0xffffu;
+    }
+    int64_t at = s;
+    if (m.stride != slots) {
+        const uint32_t c = s / (uint32_t)slots;
+        at = (int64_t)c * m.stride + (s - c * (uint32_t)slots);
+    }
+    if constexpr (sizeof(W) == 4) return __ldg((const uint32_t *)m.data + at);
+    else return __ldg((const uint16_t *)m.data + at);
+}
+
 // The gather table as a call's gather reads it: the weights in its order, and the place of every gathered neuron in the image.  Padding
-// gets the weight zero, whatever the caller's matrix holds where a neuron has no connection.
+// gets the weight zero, whatever the caller's matrix holds where a neuron has no connection.  A thread has the four connections of a quad.
 template <class W, int SETS>
 __device__ __forceinline__ void order_block(const OrderArgs &a, unsigned block) {
-    const int64_t e = (int64_t)block * kPackThreads + threadIdx.x;
-    if (e >= a.entries) return;
-    const uint32_t s = __ldg(a.src + e), n = __ldg(a.idx + e);
-    const uint32_t c = s / (uint32_t)a.slots, j = s % (uint32_t)a.slots;
+    const int64_t quad = (int64_t)block * kPackThreads + threadIdx.x;
+    if (quad * 4 >= a.entries) return;
+    const uint4 src4 = __ldg((const uint4 *)a.src + quad), idx4 = __ldg((const uint4 *)a.idx + quad);
+    const uint32_t src[4] = {src4.x, src4.y, src4.z, src4.w}, idx[4] = {idx4.x, idx4.y, idx4.z, idx4.w};
+    uint32_t w[4 * SETS], place[4];
 #pragma unroll
-    for (int k = 0; k < SETS; ++k) {
-        const Matrix &w = k ? a.w1 : a.w0;
-        float v = 0.0f;
-        if (s != 0xffffffffu)
-            v = w.type == MX4 ? mx4_value((const uint8_t *)w.data, w.scales, w.stride, c, (int)j)
-                              : load_as_float(w.data, w.type, (int64_t)c * w.stride + j);
-        ((W *)a.weights)[e * SETS + k] = from_float<W>(v);
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) w[k * SETS + s] = weight_bits<W>(s ? a.w1 : a.w0, src[k], a.slots);
+        place[k] = a.whole ? unit_place(idx[k], (uint32_t)(a.values * a.p)) : idx[k];
     }
-    const uint32_t place = a.whole ? unit_place(n, (uint32_t)(a.values * a.p)) : n;
-    if (a.wide) ((uint32_t *)a.index)[e] = place;
-    else ((uint16_t *)a.index)[e] = (uint16_t)place;
+    if constexpr (sizeof(W) == 4) {
+#pragma unroll
+        for (int k = 0; k < SETS; ++k) ((uint4 *)a.weights)[quad * SETS + k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    } else if constexpr (SETS == 2) {
+        ((uint4 *)a.weights)[quad] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    } else {
+        ((uint2 *)a.weights)[quad] = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    }
+    if (a.wide) ((uint4 *)a.index)[quad] = make_uint4(place[0], place[1], place[2], place[3]);
+    else ((uint2 *)a.index)[quad] = make_uint2(place[0] | place[1] << 16, place[2] | place[3] << 16);
 }
 
 struct OrderBlocksArgs {
@@ -482,28 +620,22 @@ struct OrderBlocksArgs {
 };
 
 // The weights of a block table as mma.m16n8k16 takes them for its second operand: of a chunk, per step of 16 rows and per set 16 bytes a
-// lane, the fragments of the block's neurons 0-7 and 8-15.  SPREAD (backward): the sets are planes of their own.
+// lane, the fragments of the block's neurons 0-7 and 8-15; the table's sources are in that order.  SPREAD (backward): the sets are
+// planes of their own.
 template <class W, int SETS, bool SPREAD>
 __device__ __forceinline__ void order_blocks_block(const OrderBlocksArgs &a, unsigned block) {
-    const int64_t e = (int64_t)block * kPackThreads + threadIdx.x;
-    if (e >= a.chunks * 512 * SETS) return;
-    const int v = (int)(e & 3), half = (int)(e >> 2 & 1), lane = (int)(e >> 3 & 31);
-    int64_t chunk = e >> 8;                            // [chunk][step][set] or [set][chunk][step]
-    int set = 0;
-    if (!SPREAD) { set = (int)(chunk % SETS); chunk /= SETS; }
-    const int step = (int)(chunk & 1);
-    chunk >>= 1;
-    if (SPREAD) { set = (int)(chunk / a.chunks); chunk -= set * a.chunks; }
-    const int row = step * 16 + (lane & 3) * 2 + (v & 1) + (v >> 1) * 8, neuron = half * 8 + lane / 4;
-    const uint32_t s = __ldg(a.src + (chunk * 32 + row) * 16 + neuron);
-    const Matrix &w = set ? a.w1 : a.w0;
-    float value = 0.0f;
-    if (s != 0xffffffffu) {
-        const uint32_t c = s / (uint32_t)a.slots, j = s % (uint32_t)a.slots;
-        value = w.type == MX4 ? mx4_value((const uint8_t *)w.data, w.scales, w.stride, c, (int)j)
-                              : load_as_float(w.data, w.type, (int64_t)c * w.stride + j);
+    const int64_t e = (int64_t)block * kPackThreads + threadIdx.x;        // lane of a step
+    if (e >= a.chunks * 64) return;
+    const uint4 lo = __ldg((const uint4 *)a.src + e * 2), hi = __ldg((const uint4 *)a.src + e * 2 + 1);
+    const uint32_t src[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = weight_bits<W>(set ? a.w1 : a.w0, src[k], a.slots);
+        const int64_t to = SPREAD ? set * a.chunks * 64 + e : ((e >> 5) * SETS + set) * 32 + (e & 31);
+        ((uint4 *)a.weights)[to] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
-    ((W *)a.weights)[e] = from_float<W>(value);
 }
 
 // Everything that a call lays out, in one launch (a launch takes longer than most of these blocks): the table, then image and columns
@@ -597,17 +729,6 @@ template <class W, int SETS, bool WIDE> struct Quad {
         else return e & 1 ? weight[e >> 1] >> 16 : weight[e >> 1] & 0xffffu;
     }
 };
-
-template <class F> __device__ __forceinline__ void with_activation(int act, const F &f) {
-    switch (act) {
-        case RELU: f(std::integral_constant<int, RELU>()); return;
-        case CLIP: f(std::integral_constant<int, CLIP>()); return;
-        case SILU: f(std::integral_constant<int, SILU>()); return;
-        case GELU: f(std::integral_constant<int, GELU>()); return;
-        case GELU_TANH: f(std::integral_constant<int, GELU_TANH>()); return;
-        default: return;
-    }
-}
 
 // One block: the image of one tile of T = V P tokens, and a range of the gathering neurons.  Unit of work of a warp: 32 / L neurons, L
 // lanes each with NV units of V tokens.  S = 1: one gathered value for G sums (forward).  S = 2: two gathered values for one

@@ -37,9 +37,16 @@ struct BlockTable {
     int blocks = 0;                    // 0: not worth it (too few neurons share their rows)
     std::vector<uint32_t> chunk_ptr;   // [blocks + 1] first chunk of a block
     std::vector<uint32_t> rows;        // [chunks][32] gathered row, padding = the row of zeros
-    std::vector<uint32_t> src;         // [chunks][32][16] position in the canonical weights, kNoSource = padding
+    std::vector<uint32_t> src;         // [chunks][2][32][8] position in the canonical weights, kNoSource = padding: see fragment()
     std::vector<int32_t> members;      // [blocks][16] gathering neuron, -1 = none
 };
+
+// Where the weight of row `k` and neuron `j` of a chunk is: in the order of the tensor cores' second operand (16 rows x 8 neurons: lane 4 (j mod 8) +
+// (k mod 8) / 2 holds the rows 2 (lane mod 4) + {0, 1, 8, 9}), a lane's eight for the neurons 0-7 and 8-15 together.
+inline size_t fragment(int k, int j) {
+    const int lane = j % 8 * 4 + k % 8 / 2, v = k % 2 + k % 16 / 8 * 2;
+    return (size_t)((k / 16 * 32 + lane) * 8 + j / 8 * 4 + v);
+}
 
 struct Topology {
     int inputs = 0, outputs = 0;
@@ -260,7 +267,7 @@ inline void build_block_table(int outs, int rows, const std::vector<size_t> &sta
             for (size_t k = 0; k < n; ++k) {
                 t.rows[chunk * 32 + k] = row_of(start[first[c]] + k);
                 for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j)
-                    t.src[(chunk * 32 + k) * 16 + (j - m)] = source_of(start[members[c][j]] + k);
+                    t.src[(chunk + k / 32) * 512 + fragment((int)(k % 32), (int)(j - m))] = source_of(start[members[c][j]] + k);
             }
             for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j) t.members[block * 16 + (j - m)] = members[c][j];
             chunk += (n + 31) / 32;
