@@ -30,7 +30,7 @@ struct DeviceTable {
 };
 
 struct DeviceBlocks {
-    uint32_t *chunk_ptr = nullptr, *rows = nullptr, *src = nullptr;
+    uint32_t *chunk_ptr = nullptr, *rows = nullptr, *src = nullptr, *chunk_block = nullptr;
     int32_t *members = nullptr;
     int blocks = 0;                 // 0: this direction has none
     int64_t chunks = 0;
@@ -106,11 +106,12 @@ cudaError_t upload(DeviceBlocks &d, const BlockTable &t) {
     if (e == cudaSuccess) e = upload(&d.rows, t.rows);
     if (e == cudaSuccess) e = upload(&d.src, t.src);
     if (e == cudaSuccess) e = upload(&d.members, t.members);
+    if (e == cudaSuccess) e = upload(&d.chunk_block, t.chunk_block);
     return e;
 }
 
 void release(DeviceBlocks &d) {
-    cudaFree(d.chunk_ptr); cudaFree(d.rows); cudaFree(d.src); cudaFree(d.members);
+    cudaFree(d.chunk_ptr); cudaFree(d.rows); cudaFree(d.src); cudaFree(d.members); cudaFree(d.chunk_block);
     d = DeviceBlocks();
 }
 
@@ -528,6 +529,39 @@ struct Gradients {
     float *dw[2], *db[2];
 };
 
+cudaError_t launch_dw(const Call &c, const Gradients &d, int type, const void *x_columns, const float *d_columns, int64_t stride) {
+    const Topology &h = c.top->host;
+    DwArgs a{};
+    a.x = x_columns; a.d = d_columns; a.rows = c.top->rows; a.token_stride = stride;
+    a.outputs = h.outputs; a.slots = h.slots; a.chunks = (h.slots + kDwSlots - 1) / kDwSlots;
+    a.dw0 = d.dw[0]; a.dw1 = d.dw[1]; a.db0 = d.db[0]; a.db1 = d.db[1];
+    const int per_block = kDwThreads / 32;
+    const unsigned grid = (unsigned)(((int64_t)a.outputs * a.chunks + per_block - 1) / per_block);
+    const auto run = [&](auto v) {
+        using E = decltype(v);
+        return c.sets == 2 ? launch(dw_kernel<E, 2>, grid, kDwThreads, c.stream, a) : launch(dw_kernel<E, 1>, grid, kDwThreads, c.stream, a);
+    };
+    return type == F32 ? run(float()) : type == F16 ? run(__half()) : run(bf16());
+}
+
+cudaError_t launch_dw_blocks(const Call &c, const Gradients &d, const DeviceBlocks &b, int type, const void *x_columns, const float *d_columns, int64_t stride) {
+    const Topology &h = c.top->host;
+    cudaError_t e = cudaSuccess;
+    // the kernel writes the connections there are
+    if (h.connections < (int64_t)h.outputs * h.slots)
+        for (int s = 0; s < c.sets && e == cudaSuccess; ++s) e = cudaMemsetAsync(d.dw[s], 0, sizeof(float) * (size_t)h.outputs * h.slots, c.stream);
+    if (e != cudaSuccess) return e;
+    DwBlockArgs a{};
+    a.x = x_columns; a.d = d_columns; a.chunk_ptr = b.chunk_ptr; a.rows = b.rows; a.src = b.src; a.members = b.members; a.chunk_block = b.chunk_block;
+    a.token_stride = stride; a.inputs = h.inputs; a.dw0 = d.dw[0]; a.dw1 = d.dw[1]; a.db0 = d.db[0]; a.db1 = d.db[1];
+    const auto run = [&](auto v) {
+        using E = decltype(v);
+        return c.sets == 2 ? launch(dw_block_kernel<E, 2>, (unsigned)b.chunks, kDwBlockThreads, c.stream, a)
+                           : launch(dw_block_kernel<E, 1>, (unsigned)b.chunks, kDwBlockThreads, c.stream, a);
+    };
+    return type == F16 ? run(__half()) : run(bf16());
+}
+
 int run_backward(const Call &c, const Gradients &d) {
     int rc = check_call(c, true);
     if (rc) return rc;
@@ -582,19 +616,9 @@ int run_backward(const Call &c, const Gradients &d) {
         e = g.blocks ? launch_blocks(*c.top, g, c.top->backward_blocks, a, type, c.sets, 1, c.stream) : launch_gather(g, a, type, type, c.sets, 1, c.stream);
     }
     if (d.dw[0] && e == cudaSuccess) {
-        if (e == cudaSuccess) {
-            DwArgs a{};
-            a.x = base + ws.x_columns; a.d = (const float *)(base + ws.d_columns); a.rows = c.top->rows; a.token_stride = stride;
-            a.outputs = h.outputs; a.slots = h.slots; a.chunks = (h.slots + kDwSlots - 1) / kDwSlots;
-            a.dw0 = d.dw[0]; a.dw1 = d.dw[1]; a.db0 = d.db[0]; a.db1 = d.db[1];
-            const int per_block = kDwThreads / 32;
-            const unsigned grid = (unsigned)(((int64_t)a.outputs * a.chunks + per_block - 1) / per_block);
-            const auto run = [&](auto v) {
-                using E = decltype(v);
-                return c.sets == 2 ? launch(dw_kernel<E, 2>, grid, kDwThreads, c.stream, a) : launch(dw_kernel<E, 1>, grid, kDwThreads, c.stream, a);
-            };
-            e = type == F32 ? run(float()) : type == F16 ? run(__half()) : run(bf16());
-        }
+        const DeviceBlocks &b = c.top->forward_blocks;
+        if (e == cudaSuccess && go_by_blocks(b, c.tokens, type, type)) e = launch_dw_blocks(c, d, b, type, base + ws.x_columns, (const float *)(base + ws.d_columns), stride);
+        else if (e == cudaSuccess) e = launch_dw(c, d, type, base + ws.x_columns, (const float *)(base + ws.d_columns), stride);
     }
     if (e != cudaSuccess) return fail_cuda(c.err, c.err_len, e);
     return SPDNN_OK;

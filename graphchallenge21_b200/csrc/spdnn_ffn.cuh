@@ -857,6 +857,142 @@ __global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_
     }
 }
 
+// ---- gradients of the weights by blocks ----------------------------------------------------------------
+
+struct DwBlockArgs {
+    const void *x;               // [inputs][token_stride]
+    const float *d;              // [outputs][sets][token_stride]
+    const uint32_t *chunk_ptr, *rows, *src;   // the forward direction's block table
+    const int32_t *members;
+    const uint32_t *chunk_block; // block of every chunk
+    int64_t token_stride;
+    int inputs;
+    float *dw0, *dw1;            // [outputs][slots]
+    float *db0, *db1;            // or nullptr
+};
+
+constexpr int kDwBlockThreads = 256;
+
+__device__ __forceinline__ void mma_16x8x8_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One block of threads: a chunk (16 outputs over 32 inputs); its warps take 32 tokens each in turn and are joined at the end, in a fixed
+// order.  dw[j][k] = sum_t d[j][t] x[k][t]: both factors lie along tokens, so a lane's 16 bytes of a row are its part of four steps of eight
+// tokens (which tokens make a step is free as long as both factors agree), and no shared memory is needed to feed the tensor cores.  x (16
+// bits) is exact in tf32; d is the sum of two tf32 numbers, 22 bits, and takes two products.  The tensor cores cut sums off instead
+// of rounding them: they add up 32 tokens only, the rest is added in float32.
+template <class E, int G>
+__global__ void __launch_bounds__(kDwBlockThreads, 2) dw_block_kernel(const __grid_constant__ DwBlockArgs a) {
+    constexpr int WARPS = kDwBlockThreads / 32;
+    __shared__ float sums[WARPS][G][16][33];
+    __shared__ float bias_sums[WARPS][G][16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t chunk = blockIdx.x, block = __ldg(a.chunk_block + chunk);
+    // rows g, g + 8, ...; outputs g and g + 8.  What is not there reads row or output 0, and its sum is dropped.
+    const E *x[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const uint32_t row = __ldg(a.rows + (size_t)chunk * 32 + n * 8 + g);
+        x[n] = (const E *)a.x + (row < (uint32_t)a.inputs ? row : 0u) * a.token_stride + t * 8;
+    }
+    const float *d[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) d[h] = a.d + (int64_t)max(__ldg(a.members + (size_t)block * 16 + h * 8 + g), 0) * G * a.token_stride + t * 8;
+    float total[G][4][4], bias[G][2];
+#pragma unroll
+    for (int s = 0; s < G; ++s) {
+        bias[s][0] = bias[s][1] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[s][n][i] = 0.0f;
+    }
+    for (int64_t at = warp * 32; at < a.token_stride; at += WARPS * 32) {
+        Raw<E, 8> xv[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) xv[n].load(x[n] + at);
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+            float4 dv[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    dv[h][i] = __ldg((const float4 *)(d[h] + s * a.token_stride + at) + i);
+                    bias[s][h] += (dv[h][i].x + dv[h][i].y) + (dv[h][i].z + dv[h][i].w);
+                }
+            float part[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[n][i] = 0.0f;
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {         // tokens 8 t + 2 step and the next
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 &q = dv[k & 1][step >> 1];
+                    const float v = step & 1 ? (k < 2 ? q.z : q.w) : (k < 2 ? q.x : q.y);
+                    hi[k] = __float_as_uint(v) & 0xffffe000u;
+                    lo[k] = __float_as_uint(v - __uint_as_float(hi[k]));
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t b0 = __float_as_uint(bits_to_float<E>(xv[n].bits(2 * step))), b1 = __float_as_uint(bits_to_float<E>(xv[n].bits(2 * step + 1)));
+                    mma_16x8x8_tf32(part[n], hi, b0, b1);
+                    mma_16x8x8_tf32(part[n], lo, b0, b1);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) total[s][n][i] += part[n][i];
+        }
+    }
+    // total[s][n][i]: output g + 8 (i / 2), row 8 n + 2 t + i % 2
+#pragma unroll
+    for (int s = 0; s < G; ++s)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[warp][s][g + 8 * (i >> 1)][n * 8 + 2 * t + (i & 1)] = total[s][n][i];
+#pragma unroll
+    for (int s = 0; s < G; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v = bias[s][h];
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            if (t == 0) bias_sums[warp][s][g + 8 * h] = v;
+        }
+    __syncthreads();
+    // every block has a first chunk: there the biases' gradients, the sums of d, are written
+    if (chunk == __ldg(a.chunk_ptr + block) && threadIdx.x < 16 * G) {
+        const int s = threadIdx.x >> 4, j = threadIdx.x & 15, c = __ldg(a.members + (size_t)block * 16 + j);
+        float *db = s ? a.db1 : a.db0;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) sum += bias_sums[w][s][j];
+        if (c >= 0 && db) db[c] = sum;
+    }
+    for (int e = threadIdx.x; e < 512; e += kDwBlockThreads) {
+        // e counts the table's order: lane, half, v of a step (topology.h, fragment)
+        const int v = e & 3, half = e >> 2 & 1, l = e >> 3 & 31, step = e >> 8;
+        const int k = step * 16 + (l & 3) * 2 + (v & 1) + (v >> 1) * 8, j = half * 8 + (l >> 2);
+        const uint32_t to = __ldg(a.src + (size_t)chunk * 512 + e);
+        if (to == 0xffffffffu) continue;
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum += sums[w][s][j][k];
+            (s ? a.dw1 : a.dw0)[to] = sum;
+        }
+    }
+}
+
 // ---- a few tokens ----------------------------------------------------------------------------------
 
 struct FewArgs {

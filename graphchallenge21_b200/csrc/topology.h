@@ -39,6 +39,7 @@ struct BlockTable {
     std::vector<uint32_t> rows;        // [chunks][32] gathered row, padding = the row of zeros
     std::vector<uint32_t> src;         // [chunks][2][32][8] position in the canonical weights, kNoSource = padding: see fragment()
     std::vector<int32_t> members;      // [blocks][16] gathering neuron, -1 = none
+    std::vector<uint32_t> chunk_block; // [chunks]
 };
 
 // Where the weight of row `k` and neuron `j` of a chunk is: in the order of the tensor cores' second operand (16 rows x 8 neurons: lane 4 (j mod 8) +
@@ -250,7 +251,7 @@ inline void build_block_table(int outs, int rows, const std::vector<size_t> &sta
     for (size_t c = 0; c < first.size(); ++c) {
         const int64_t b = ((int64_t)members[c].size() + 15) / 16;
         blocks += b;
-        chunks += b * (int64_t)((length(first[c]) + 31) / 32);
+        chunks += b * (int64_t)std::max<size_t>(1, (length(first[c]) + 31) / 32);
     }
     const int64_t entries = (int64_t)start[outs];
     if (!entries || chunks * 512 > entries * kBlockWaste) return;
@@ -270,7 +271,8 @@ inline void build_block_table(int outs, int rows, const std::vector<size_t> &sta
                     t.src[(chunk + k / 32) * 512 + fragment((int)(k % 32), (int)(j - m))] = source_of(start[members[c][j]] + k);
             }
             for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j) t.members[block * 16 + (j - m)] = members[c][j];
-            chunk += (n + 31) / 32;
+            chunk += std::max<size_t>(1, (n + 31) / 32);        // neurons without connections have a chunk of padding
+            t.chunk_block.resize(chunk, (uint32_t)block);
             t.chunk_ptr.push_back((uint32_t)chunk);
         }
 }
