@@ -5,7 +5,11 @@
 // stream, so calls on one topology may overlap, from several threads too.
 #include "../../include/spdnn_b200.h"
 
+#include <array>
+#include <cmath>
 #include <cstdio>
+#include <map>
+#include <mutex>
 #include <new>
 #include <string>
 #include <tuple>
@@ -36,6 +40,14 @@ struct DeviceBlocks {
     int64_t chunks = 0;
 };
 
+// How a gather runs: the image's unit (v tokens) and units per neuron (p), and how many blocks share a tile.
+struct GatherPlan {
+    int v = 1, p = 1, splits = 1;
+    int64_t tiles = 0, image_bytes = 0;
+    bool global = false;
+    bool blocks = false;            // by blocks, on the tensor cores: 64 tokens per tile
+};
+
 }  // namespace
 
 struct spdnn_topology {
@@ -46,6 +58,9 @@ struct spdnn_topology {
     DeviceBlocks forward_blocks, backward_blocks;
     int32_t *rows = nullptr;        // canonical
     void *few_rows = nullptr;       // canonical as few_kernel reads them
+    // plans made so far: functions of the topology and the key, kept because a call may come every few microseconds
+    mutable std::mutex plans_lock;
+    mutable std::map<std::array<int, 5>, GatherPlan> plans;
 };
 
 namespace {
@@ -55,6 +70,18 @@ int fail(char *err, int err_len, int code, const char *msg) {
     return code;
 }
 int fail(char *err, int err_len, int code, const std::string &msg) { return fail(err, err_len, code, msg.c_str()); }
+
+// No exception leaves a C entry point.
+template <class F>
+int guarded(char *err, int err_len, const F &f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return fail(err, err_len, SPDNN_ERR_MEMORY, "host allocation failed");
+    } catch (const std::exception &e) {
+        return fail(err, err_len, SPDNN_ERR_MEMORY, e.what());
+    }
+}
 
 // A failed runtime call: its message, and nothing left for the next caller of cudaGetLastError to find.
 int fail_cuda(char *err, int err_len, cudaError_t e) {
@@ -141,14 +168,6 @@ int type_size(int type) { return type == F32 ? 4 : 2; }
 bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
 int64_t aligned(int64_t n) { return (n + 255) & ~255ll; }
 
-// How a gather runs: the image's unit (v tokens) and units per neuron (p), and how many blocks share a tile.
-struct GatherPlan {
-    int v = 1, p = 1, splits = 1;
-    int64_t tiles = 0, image_bytes = 0;
-    bool global = false;
-    bool blocks = false;            // by blocks, on the tensor cores: 64 tokens per tile
-};
-
 constexpr int64_t kSharedLimit = 227 * 1024;
 #ifndef SPDNN_BLOCK_TOKENS
 #define SPDNN_BLOCK_TOKENS 17
@@ -158,53 +177,6 @@ int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
 }
 
-// Blocks take 16-bit operands of one type and whole tiles of 64 tokens.
-bool go_by_blocks(const DeviceBlocks &b, int tokens, int image_type, int weight_type) {
-    return b.blocks && tokens >= SPDNN_BLOCK_TOKENS && image_type != F32 && image_type == weight_type;
-}
-
-GatherPlan plan_gather(const spdnn_topology &top, bool forward, int tokens, int sets, int image_type, int weight_type) {
-    const DeviceTable &t = forward ? top.forward : top.backward;
-    GatherPlan g;
-    const int size = type_size(image_type), full = 16 / size;
-    if (go_by_blocks(forward ? top.forward_blocks : top.backward_blocks, tokens, image_type, weight_type)) {
-        g.blocks = true;
-        g.v = 8; g.p = 8;
-        g.image_bytes = image_size(t.rows, sets, 8, 8, 2);
-        g.tiles = ((int64_t)tokens + 63) / 64;
-        return g;
-    }
-    bool found = false;
-    for (int T = full * 8; T >= 1 && !found; T /= 2) {
-        const int v = T < full ? T : full, p = T / v;
-        if (T > 1 && T / 2 >= tokens) continue;
-        const int64_t bytes = image_size(t.rows, sets, v, p, size);
-        if (t.rows >= 65536 || bytes > kSharedLimit) continue;
-        g.v = v; g.p = p; g.image_bytes = bytes;
-        found = true;
-    }
-    if (!found) {
-        g.global = true;
-        g.v = full; g.p = tokens > full ? 8 : 1;
-        g.image_bytes = image_size(t.rows, sets, g.v, g.p, size);
-    }
-    const int T = g.v * g.p;
-    g.tiles = (tokens + T - 1) / T;
-    const int64_t per_sm = g.global ? 2 : std::max<int64_t>(1, std::min<int64_t>(2, kSharedLimit / (g.image_bytes + 1024)));
-    const int64_t slots = per_sm * top.sm_count, units = (int64_t)((t.outs + 31) / 32) * (g.p / lane_units(g.p));
-    // Blocks of a tile: clocks of a wave of blocks are those of the image (about 40 bytes a clock) and of the block's units (a
-    // connection of 32 lanes about 8 clocks of the SM); the fewest in all waves, of the splits that fill 1 to 16 waves.
-    const double per_unit = 8.0 * lane_units(g.p) * std::max<double>(1.0, (double)t.entries / 32.0 / std::max<int64_t>(1, (t.outs + 31) / 32)) / per_sm;
-    double best = 0.0;
-    for (int64_t w = 0; w <= 16; ++w) {
-        const int64_t s = std::max<int64_t>(1, std::min<int64_t>(w * slots / g.tiles, units / 16));
-        const int64_t waves = (g.tiles * s + slots - 1) / slots;
-        const double cost = waves * ((g.global ? 0.0 : g.image_bytes / 40.0) + 1000.0 + (double)((units + s - 1) / s) * per_unit);
-        if (w == 0 || cost < best) { best = cost; g.splits = (int)s; }
-    }
-    return g;
-}
-
 // How many neurons are read at a time by the gather that many tokens of `rows` neurons get (plan_gather), for the order of connections: the
 // image's bytes per neuron, and with them the lanes per neuron, do not depend on the type.  Fewer tokens may read more at a time.
 int neurons_at_a_time(int rows, int sets) {
@@ -212,6 +184,72 @@ int neurons_at_a_time(int rows, int sets) {
     while (p > 1 && image_size(rows, sets, 8, p, 2) > kSharedLimit) p /= 2;
     if (image_size(rows, sets, 8, p, 2) > kSharedLimit) return 16;
     return 8 / (p / lane_units(p));
+}
+
+// Blocks take 16-bit operands of one type and whole tiles of 64 tokens.
+bool go_by_blocks(const DeviceBlocks &b, int tokens, int image_type, int weight_type) {
+    return b.blocks && tokens >= SPDNN_BLOCK_TOKENS && image_type != F32 && image_type == weight_type;
+}
+
+GatherPlan make_plan(const spdnn_topology &top, bool forward, int tokens, int sets, int image_type, int weight_type) {
+    const DeviceTable &t = forward ? top.forward : top.backward;
+    GatherPlan g;
+    const int size = type_size(image_type), full = 16 / size;
+    if (go_by_blocks(forward ? top.forward_blocks : top.backward_blocks, tokens, image_type, weight_type)) {
+        g.blocks = true;
+        g.v = 8; g.p = 8;
+        g.image_bytes = image_size(t.rows, forward ? 1 : sets, 8, 8, 2);
+        g.tiles = ((int64_t)tokens + 63) / 64;
+        return g;
+    }
+    const int slices = (t.outs + 31) / 32;
+    const double quads = std::max(1.0, (double)t.entries / 128.0 / slices);       // of a slice
+    const int s_values = forward ? 1 : sets, sums = forward ? sets : 1;
+    double best = 0.0;
+    const auto consider = [&](int T, bool global) {
+        const int v = std::min(T, full), p = T / v, nv = lane_units(p), lanes = p / nv;
+        const int64_t bytes = image_size(t.rows, s_values, v, p, size), tiles = ((int64_t)tokens + T - 1) / T, units = (int64_t)slices * lanes;
+        const int warps = gather_threads(v * nv * sums) / 32;
+        // Clocks, fitted to a sweep of T and splits over 15 sizes (33 to 4096 tokens, 300 to 16384 neurons; the choice is 1 % off the best of the
+        // sweep in the mean).  A connection of a warp takes the shared memory's wavefronts (1.3 per 128 bytes in the order of topology.h,
+        // more where more neurons are read at a time than it was made for) with those of the table, or its instructions on four
+        // schedulers; a quad that a warp works on alone, the latency of its loads and instructions.
+        const int at_a_time = v * size < 16 ? 16 : 8 / lanes;
+        const double conflicts = 1.3 + 0.35 * std::max(0.0, std::log2((double)at_a_time / neurons_at_a_time(t.rows, s_values)));
+        const double wavefronts = nv * s_values * v * size * 32 / 128.0 * conflicts + (2 + sets * type_size(weight_type)) / 4.0;
+        const double issue = (nv * s_values * (v * sums + 1.5) + 6 + sets) / 4.0;
+        const double busy = 4.0 * std::max(wavefronts, issue) * 1.25, alone = 600.0 + 6.0 * (nv * s_values * (v * sums + 4) + 6);
+        int64_t tried = 0;
+        for (int64_t w = 0; w <= 24; ++w) {
+            // splits that fill w waves, and a few between
+            const int64_t n = std::max<int64_t>(1, std::min<int64_t>(w * top.sm_count / tiles, (units + 3) / 4));
+            if (n == tried) continue;
+            tried = n;
+            const int64_t waves = (tiles * n + top.sm_count - 1) / top.sm_count, here = (units + n - 1) / n;
+            const double work = std::max((double)((here + warps - 1) / warps) * quads * alone, here * quads * busy);
+            const double cost = waves * (1500.0 + (global ? 0.0 : bytes / 45.0) + work * (global ? 3.0 : 1.0));
+            if (best == 0.0 || cost < best) {
+                best = cost;
+                g.v = v; g.p = p; g.image_bytes = bytes; g.tiles = tiles; g.splits = (int)n; g.global = global;
+            }
+        }
+    };
+    for (int T = full * 8; T >= 1; T /= 2)
+        if ((T == 1 || T / 2 < tokens) && t.rows < 65536 && image_size(t.rows, s_values, std::min(T, full), std::max(T / full, 1), size) <= kSharedLimit)
+            consider(T, false);
+    if (best == 0.0) consider(tokens > full ? full * 8 : full, true);     // nothing fits: the image stays in global memory
+    return g;
+}
+
+GatherPlan plan_gather(const spdnn_topology &top, bool forward, int tokens, int sets, int image_type, int weight_type) {
+    const std::array<int, 5> key{forward, tokens, sets, image_type, weight_type};
+    std::lock_guard<std::mutex> lock(top.plans_lock);
+    const auto found = top.plans.find(key);
+    if (found != top.plans.end()) return found->second;
+    const GatherPlan g = make_plan(top, forward, tokens, sets, image_type, weight_type);
+    if (top.plans.size() >= 4096) top.plans.clear();
+    top.plans.emplace(key, g);
+    return g;
 }
 
 template <class E, class W, int S, int G>
@@ -497,7 +535,7 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     }
     const DeviceTable &t = c.top->forward;
     const int it = image_type(c.x->type), wt = ordered_type(c.x->type, c.w[0]->type);
-    const GatherPlan g = plan_gather(*c.top, true, std::max(c.tokens, 1), 1, it, wt);
+    const GatherPlan g = plan_gather(*c.top, true, std::max(c.tokens, 1), c.sets, it, wt);
     const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, it, wt, false);
     if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
     OnDevice guard(c.top->device);
@@ -712,14 +750,16 @@ extern "C" int spdnn_layer_workspace(const spdnn_topology_t *top, int tokens, in
     if (check_types(x_type, w_type, backward != 0)) return SPDNN_ERR_ARG;
     if (top->device < 0) return SPDNN_ERR_STATE;
     const int it = image_type(x_type), wt = ordered_type(x_type, w_type);
-    if (!backward && few_tokens(*top, tokens, x_type)) {
-        *bytes = 0;
-        return SPDNN_OK;
-    }
-    const DeviceTable &t = backward ? top->backward : top->forward;
-    const GatherPlan g = plan_gather(*top, !backward, std::max(tokens, 1), backward ? sets : 1, it, wt);
-    *bytes = layout(*top, g, t, tokens, sets, it, wt, backward != 0).total;
-    return SPDNN_OK;
+    return guarded(nullptr, 0, [&] {
+        if (!backward && few_tokens(*top, tokens, x_type)) {
+            *bytes = 0;
+            return (int)SPDNN_OK;
+        }
+        const DeviceTable &t = backward ? top->backward : top->forward;
+        const GatherPlan g = plan_gather(*top, !backward, std::max(tokens, 1), sets, it, wt);
+        *bytes = layout(*top, g, t, tokens, sets, it, wt, backward != 0).total;
+        return (int)SPDNN_OK;
+    });
 }
 
 extern "C" int spdnn_linear(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w, const float *bias,
@@ -727,7 +767,7 @@ extern "C" int spdnn_linear(const spdnn_topology_t *top, int tokens, const spdnn
                             int64_t workspace_bytes, void *cuda_stream, char *err, int err_len) {
     const Call c{top, tokens, 1, activation, clip, x, {w, nullptr}, y, {z, nullptr}, workspace, workspace_bytes,
                  static_cast<cudaStream_t>(cuda_stream), err, err_len};
-    return run_forward(c, bias, nullptr);
+    return guarded(err, err_len, [&] { return run_forward(c, bias, nullptr); });
 }
 
 extern "C" int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *x, const spdnn_operand_t *w_gate,
@@ -736,7 +776,7 @@ extern "C" int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_
                            int64_t workspace_bytes, void *cuda_stream, char *err, int err_len) {
     const Call c{top, tokens, 2, activation, clip, x, {w_gate, w_up}, y, {z_gate, z_up}, workspace, workspace_bytes,
                  static_cast<cudaStream_t>(cuda_stream), err, err_len};
-    return run_forward(c, bias_gate, bias_up);
+    return guarded(err, err_len, [&] { return run_forward(c, bias_gate, bias_up); });
 }
 
 extern "C" int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
@@ -745,7 +785,7 @@ extern "C" int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, co
                                      int err_len) {
     const Call c{top, tokens, 1, activation, clip, x, {w, nullptr}, nullptr, {z, nullptr}, workspace, workspace_bytes,
                  static_cast<cudaStream_t>(cuda_stream), err, err_len};
-    return run_backward(c, Gradients{dy, dx, {dw, nullptr}, {dbias, nullptr}});
+    return guarded(err, err_len, [&] { return run_backward(c, Gradients{dy, dx, {dw, nullptr}, {dbias, nullptr}}); });
 }
 
 extern "C" int spdnn_gated_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
@@ -755,7 +795,7 @@ extern "C" int spdnn_gated_backward(const spdnn_topology_t *top, int tokens, con
                                     void *cuda_stream, char *err, int err_len) {
     const Call c{top, tokens, 2, activation, clip, x, {w_gate, w_up}, nullptr, {z_gate, z_up}, workspace, workspace_bytes,
                  static_cast<cudaStream_t>(cuda_stream), err, err_len};
-    return run_backward(c, Gradients{dy, dx, {dw_gate, dw_up}, {dbias_gate, dbias_up}});
+    return guarded(err, err_len, [&] { return run_backward(c, Gradients{dy, dx, {dw_gate, dw_up}, {dbias_gate, dbias_up}}); });
 }
 
 // ---- microscaled matrices ------------------------------------------------------------------------------

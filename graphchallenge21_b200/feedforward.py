@@ -33,8 +33,11 @@ def _torch():
     return torch
 
 
+_Error = C.c_char * _ERR_LEN
+
+
 def _call(fn, *args):
-    err = C.create_string_buffer(_ERR_LEN)
+    err = _Error()
     rc = fn(*args, err, _ERR_LEN)
     if rc != 0:
         raise SpDNNError(rc, err.value.decode())
@@ -71,28 +74,21 @@ class MX4:
         torch = _torch()
         device = self.codes.get_device()
         if out is None:
-            out = torch.empty(self.shape, dtype=dtype or torch.float32, device=self.device)
+            out = self.codes.new_empty(self.shape, dtype=dtype or torch.float32)
         operand = _operand(out, *self.shape, device, "out")
-        with _On(device):
-            _call(_lib.load().spdnn_mx4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
-                  _byref(operand), _stream(device))
+        _on(device, _lib.load().spdnn_mx4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
+            _byref(operand), _stream(device))
         return out
 
 
-class _On:
-    """``torch.cuda.device`` where the current device is another one."""
-
-    def __init__(self, device):
-        cuda = _torch().cuda
-        self._guard = None if cuda.current_device() == device else cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _on(device, fn, *args):
+    """``_call`` with ``device`` as the current one."""
+    cuda = _torch().cuda
+    if cuda.current_device() == device:
+        _call(fn, *args)
+    else:
+        with cuda.device(device):
+            _call(fn, *args)
 
 
 def _operand(t, rows, cols, device, name):
@@ -102,7 +98,7 @@ def _operand(t, rows, cols, device, name):
             raise SpDNNError(-1, f"{name} must be {(rows, cols)}, not {t.shape}")
         on, operand = t.codes.get_device(), _Operand(t.codes.data_ptr(), t.scales.data_ptr(), (cols + 31) // 32, MX4_TYPE, 0)
     else:
-        if not hasattr(t, "is_cuda") or not t.is_cuda:
+        if not getattr(t, "is_cuda", False):
             raise SpDNNError(-1, f"{name} must be a CUDA tensor")
         if t.shape != (rows, cols):
             raise SpDNNError(-1, f"{name} must be {(rows, cols)}, not {tuple(t.shape)}")
@@ -129,9 +125,10 @@ def mx4_quantize(x) -> MX4:
     codes = x.new_empty((rows, blocks, 16), dtype=torch.uint8)
     scales = x.new_empty((rows, blocks), dtype=torch.uint8)
     device = x.get_device()
-    with _On(device):
-        _call(_lib.load().spdnn_mx4_quantize, _byref(operand), rows, cols, codes.data_ptr(), scales.data_ptr(), _stream(device))
-    return MX4(codes, scales, cols)
+    _on(device, _lib.load().spdnn_mx4_quantize, _byref(operand), rows, cols, codes.data_ptr(), scales.data_ptr(), _stream(device))
+    q = MX4.__new__(MX4)                 # what __init__ would check holds
+    q.codes, q.scales, q.cols, q.shape = codes, scales, cols, (rows, cols)
+    return q
 
 
 class Saved:
