@@ -14,17 +14,32 @@ namespace ffn {
 
 constexpr int kMx4Threads = 256;
 
-// Two values as one byte of E2M1, `lo` in the low half.
-__device__ __forceinline__ uint32_t to_e2m1x2(float lo, float hi) {
+// Eight values as a word of E2M1, the first in the lowest half-byte.
+__device__ __forceinline__ uint32_t to_e2m1x8(const float (&v)[8]) {
     uint32_t r;
-    asm("{ .reg .b8 b, z; mov.b16 {b, z}, 0; cvt.rn.satfinite.e2m1x2.f32 b, %1, %2; mov.b32 %0, {b, z, z, z}; }" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("{ .reg .b8 b0, b1, b2, b3; cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;"
+        " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5; cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7; mov.b32 %0, {b0, b1, b2, b3}; }"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
 
-// i / n, in 32 bits where both fit (a division of 64 bits takes longer than the rest of the loop).
-__device__ __forceinline__ int64_t quotient(int64_t i, uint32_t n) {
-    return i >> 32 ? i / n : (int64_t)((uint32_t)i / n);
-}
+// Where group `i` of a matrix with `per_row` groups a row is, and then those a block of threads further on: one division for a thread's whole
+// batch (a division takes longer than the rest of a group's work).
+struct Walk {
+    int64_t row;
+    uint32_t at;
+    __device__ __forceinline__ Walk(int64_t i, uint32_t per_row) {
+        row = i >> 32 ? i / per_row : (int64_t)((uint32_t)i / per_row);
+        at = (uint32_t)(i - row * per_row);
+    }
+    __device__ __forceinline__ void step(uint32_t by, uint32_t per_row) {
+        at += by;
+        if (at < per_row) return;
+        const uint32_t rows = per_row >= by ? 1u : at / per_row;
+        row += rows;
+        at -= rows * per_row;
+    }
+};
 
 constexpr int kMx4Batch = 4;      // groups of a thread whose loads are in flight together
 
@@ -38,36 +53,40 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_quantize_kernel(const E *__re
     for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * BATCH + (threadIdx.x & ~31); first < groups; first += step) {
         constexpr int PER = BYTES / (int)sizeof(E);
         Raw<E, PER> part[BATCH][8 / PER];
+        Walk walk(first + (threadIdx.x & 31), (uint32_t)blocks * 4);
 #pragma unroll
         for (int m = 0; m < BATCH; ++m) {
             const int64_t i = first + m * kMx4Threads + (threadIdx.x & 31);
+            if (m) walk.step(kMx4Threads, (uint32_t)blocks * 4);
 #pragma unroll
             for (int h = 0; h < 8 / PER; ++h) part[m][h].clear();
             if (i >= groups) continue;
-            const int64_t row = quotient(i, (uint32_t)blocks * 4);
-            const int col = (int)(i - row * (blocks * 4)) * 8;
-            const E *from = x + row * stride + col;
+            const int col = (int)walk.at * 8;
+            const E *from = x + walk.row * stride + col;
+            if (col + 8 <= cols) {
 #pragma unroll
-            for (int h = 0; h < 8 / PER; ++h) {
-                if (col + (h + 1) * PER <= cols) {
-                    part[m][h].load(from + h * PER);
-                } else {
+                for (int h = 0; h < 8 / PER; ++h) part[m][h].load(from + h * PER);
+            } else {
 #pragma unroll
-                    for (int k = 0; k < PER; ++k)
-                        if (col + h * PER + k < cols) part[m][h].set(k, from[h * PER + k]);
-                }
+                for (int k = 0; k < 8; ++k)
+                    if (col + k < cols) part[m][k / PER].set(k % PER, from[k]);
             }
         }
 #pragma unroll
         for (int m = 0; m < BATCH; ++m) {
             const int64_t i = first + m * kMx4Threads + (threadIdx.x & 31);
-            float v[8];
-            // the largest magnitude as bits: they are ordered as the values are, and NaN and infinity are the largest
+            // the largest magnitude as bits: they are ordered as the values are, and NaN and infinity are the largest; 16-bit ones in pairs
             uint32_t top = 0;
+            if constexpr (sizeof(E) == 2 && PER > 1) {
+                uint32_t pair = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[k] = bits_to_float<E>(part[m][k / PER].bits(k % PER));
-                top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+                for (int k = 0; k < 8 / PER; ++k)
+#pragma unroll
+                    for (int j = 0; j < PER / 2; ++j) pair = __vmaxu2(pair, part[m][k].w[j] & 0x7fff7fffu);
+                top = __float_as_uint(bits_to_float<E>(max(pair & 0xffffu, pair >> 16)));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(bits_to_float<E>(part[m][k / PER].bits(k % PER))) & 0x7fffffffu);
             }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -77,12 +96,10 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_quantize_kernel(const E *__re
             const int e = max((int)(top >> 23) - 2, 0);
             // 2^-(e - 127), between 2^-125 and 2^127: a normal number, and the product is exact
             const float inverse = __uint_as_float((uint32_t)(254 - e) << 23);
-            uint32_t word = 0;
-            if (finite) {
+            float v[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) word |= to_e2m1x2(v[2 * k] * inverse, v[2 * k + 1] * inverse) << (8 * k);
-            }
-            codes[i] = word;
+            for (int k = 0; k < 8; ++k) v[k] = bits_to_float<E>(part[m][k / PER].bits(k % PER)) * inverse;
+            codes[i] = finite ? to_e2m1x8(v) : 0u;
             if ((i & 3) == 0) scales[i >> 2] = finite ? (uint8_t)e : (uint8_t)255;
         }
     }
@@ -97,15 +114,19 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_dequantize_kernel(const uint8
     const int64_t step = (int64_t)gridDim.x * kMx4Threads * BATCH;
     for (int64_t first = (int64_t)blockIdx.x * kMx4Threads * BATCH + threadIdx.x; first < groups; first += step) {
         uint32_t word[BATCH], scale[BATCH];
-        int64_t row[BATCH];
-        int col[BATCH];
+        int64_t to_at[BATCH];
+        int left[BATCH];
+        Walk walk(first, per_row);
 #pragma unroll
         for (int m = 0; m < BATCH; ++m) {
-            const int64_t i = min(first + m * kMx4Threads, groups - 1);
-            row[m] = quotient(i, per_row);
-            col[m] = (int)(i - row[m] * per_row) * 4;
-            const int64_t block = row[m] * blocks + (col[m] >> 5);
-            word[m] = __ldg((const uint16_t *)(codes + block * 16 + ((col[m] & 31) >> 1)));
+            if (m) walk.step(kMx4Threads, per_row);
+            word[m] = scale[m] = 0;
+            const int col = (int)walk.at * 4;
+            to_at[m] = walk.row * stride + col;
+            left[m] = cols - col;
+            if (first + m * kMx4Threads >= groups) continue;
+            const int64_t block = walk.row * blocks + (col >> 5);
+            word[m] = __ldg((const uint16_t *)(codes + block * 16 + ((col & 31) >> 1)));
             scale[m] = __ldg(scales + block);
         }
 #pragma unroll
@@ -117,14 +138,14 @@ __global__ void __launch_bounds__(kMx4Threads) mx4_dequantize_kernel(const uint8
             __align__(16) E e[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) e[k] = from_float<E>(v[k] * factor);
-            E *to = y + row[m] * stride + col[m];
-            if (VECTOR && col[m] + 4 <= cols) {
+            E *to = y + to_at[m];
+            if (VECTOR && left[m] >= 4) {
                 if constexpr (sizeof(E) == 4) *(uint4 *)to = *(const uint4 *)e;
                 else *(uint2 *)to = *(const uint2 *)e;
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (col[m] + k < cols) to[k] = e[k];
+                    if (k < left[m]) to[k] = e[k];
             }
         }
     }
