@@ -423,9 +423,11 @@ const char *check_operand(const spdnn_operand_t *o, int64_t rows, int64_t cols, 
     const int64_t least = o->type == MX4 ? (cols + 31) / 32 : cols;
     if (o->stride < least) return "an operand's stride is less than its row";
     if (o->stride > (1ll << 40)) return "an operand's stride is out of range";
-    if (o->type != MX4 && reinterpret_cast<uintptr_t>(o->data) % type_size(o->type)) return "an operand is not aligned to its type";
+    if (reinterpret_cast<uintptr_t>(o->data) % (o->type == MX4 ? 4 : type_size(o->type))) return "an operand is not aligned to its type (codes: 4 bytes)";
     return nullptr;
 }
+
+bool off_4_bytes(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
 
 int check_call(const Call &c, bool backward) {
     if (!c.top) return fail(c.err, c.err_len, SPDNN_ERR_ARG, "null topology");
@@ -525,6 +527,7 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
         }
     if (!bad && c.sets == 2 && !c.z[0] != !c.z[1]) bad = "save both pre-activations or none";
     if (!bad && c.sets == 2 && c.z[0] && c.z[0]->stride != c.z[1]->stride) bad = "both pre-activations must have one stride";
+    if (!bad && (off_4_bytes(b0) || off_4_bytes(b1))) bad = "a bias is not aligned to 4 bytes";
     if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
     if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, kAnalysisOnly);
     if (c.tokens == 0) return SPDNN_OK;
@@ -618,6 +621,8 @@ int run_backward(const Call &c, const Gradients &d) {
         if (!bad && d.dx->type != type) bad = "dx must have the activations' type";
     }
     if (!bad && c.sets == 2 && !d.dw[0] != !d.dw[1]) bad = "ask for the gradients of both sets of weights or of none";
+    for (int s = 0; s < 2 && !bad; ++s)
+        if (off_4_bytes(d.dw[s]) || off_4_bytes(d.db[s])) bad = "a gradient is not aligned to 4 bytes";
     if (!bad && !d.dw[0] && (d.db[0] || d.db[1])) bad = "the gradients of the biases come with those of the weights";
     if (bad) return fail(c.err, c.err_len, SPDNN_ERR_ARG, bad);
     if (c.top->device < 0) return fail(c.err, c.err_len, SPDNN_ERR_STATE, kAnalysisOnly);

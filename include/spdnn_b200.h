@@ -239,7 +239,7 @@ enum {
 #define SPDNN_MAX_TOKENS (1 << 26)   /* of one call */
 
 /* A matrix in device memory.  F32, F16, BF16: row i begins at data + i * stride elements; any stride not less than a row, any
- * alignment of the type.  MX4: data = codes [rows][stride][16], scales [rows][stride] (stride in blocks of 32 columns). */
+ * alignment of the type.  MX4: data = codes [rows][stride][16] on 4 bytes, scales [rows][stride] (stride in blocks of 32 columns). */
 typedef struct spdnn_operand {
     const void *data;         /* written where the call says so */
     const uint8_t *scales;    /* MX4 only */

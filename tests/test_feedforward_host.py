@@ -97,6 +97,7 @@ def linear(top, tokens=2, x=operand(), w=operand(), act=0, clip=32.0, y=operand(
     (dict(x=operand(data=None)), "no data"), (dict(w=operand(data=None)), "no data"), (dict(y=operand(data=None)), "no data"),
     (dict(x=operand(stride=3)), "stride"), (dict(w=operand(stride=1)), "stride"), (dict(y=operand(stride=2)), "stride"),
     (dict(x=operand(data=4098)), "aligned"), (dict(x=operand(type=1, data=4097), w=operand(type=1)), "aligned"),
+    (dict(x=operand(type=3, scales=4096, data=4098), w=operand(type=3, scales=4096)), "aligned"),
     (dict(w=operand(type=2)), "activations' type"), (dict(x=operand(type=3, scales=4096)), "activations' type"),
     (dict(w=operand(type=3)), "scales"), (dict(z=operand(type=1)), "pre-activations are saved as fp32"),
     (dict(), "analysis only"),
@@ -123,6 +124,8 @@ def test_refusals_of_the_gated_block_and_of_backward_calls(analysis):
     assert "null" in back(o, o, o, None, None, None, None)[1]
     assert "dx must have" in back(o, o, o, r(o), r(f16), None, None)[1]
     assert "biases" in back(o, o, o, r(o), r(o), None, 4096)[1]
+    assert "aligned" in back(o, o, o, r(o), r(o), 4098, None)[1] and "aligned" in back(o, o, o, r(o), r(o), 4096, 4097)[1]
+    assert "aligned" in err_of(lib.spdnn_linear, analysis._top, 2, r(o), r(o), 4097, 0, 32.0, r(o), None, *tail)[1]
     assert back(o, o, o, None, r(o), 4096, 4096, act=0)[0] == -4        # nothing saved is needed without an activation
     rc, msg = err_of(lib.spdnn_gated_backward, analysis._top, 2, r(o), r(o), r(o), r(o), r(o), r(o), 3, 32.0, None, 4096, None, None, None,
                      *tail)

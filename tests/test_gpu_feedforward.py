@@ -507,3 +507,82 @@ def test_the_challenge_networks_butterfly():
     out = torch.full((150, 1030), 5.0, dtype=BF16, device="cuda")
     p.forward("silu", out=out[:, 1:1025])
     assert torch.equal(out[:, 1:1025], p.forward("silu")) and (out[:, 0] == 5).all() and (out[:, 1025:] == 5).all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_holes_and_infinities_of_many_tokens(shared):
+    """As test_weights_without_connection_and_infinities, for the images' and the blocks' way."""
+    p = Shared(200, 256, 320, 32, F16, 2, 16, False) if shared else Problem(200, 256, 320, 32, F16, 2, "ragged")
+    want, saved = p.forward("silu", save=True)
+    grads = p.backward(saved, "silu")
+    hole = torch.as_tensor(p.rows < 0).cuda()
+    assert hole.any()
+    p.w = [w.masked_fill(hole, float("nan")) for w in p.w]
+    y, saved = p.forward("silu", save=True)
+    again = p.backward(saved, "silu")
+    assert torch.equal(y, want) and torch.equal(again[0], grads[0])
+    assert all(torch.equal(a, b) for a, b in zip(again[1] + again[2], grads[1] + grads[2]))
+    assert all((d[hole] == 0).all() for d in again[1])
+    p.x[150, 7] = float("nan")
+    y = p.forward("silu")
+    touched = torch.zeros_like(y, dtype=torch.bool)
+    touched[150] = torch.as_tensor((p.rows == 7).any(1)).cuda()
+    assert touched.any() and torch.isnan(y[touched]).all() and torch.equal(y[~touched], want[~touched])
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_large_images_captured_and_replayed(shared):
+    """Kernels with more shared memory than a launch has by default, and a gradient that is cleared first, inside a capture that is
+    the first call on its topology."""
+    make = lambda: Shared(150, 4096, 4100, 32, BF16, 2, 16, False) if shared else Problem(150, 4096, 4100, 32, BF16, 2, "ragged")  # noqa: E731
+    p, q = make(), make()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, saved = p.forward("silu", save=True)
+        grads = p.backward(saved, "silu")
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    want, kept = q.forward("silu", save=True)
+    wants = q.backward(kept, "silu")
+    assert torch.equal(y, want) and torch.equal(grads[0], wants[0])
+    assert all(torch.equal(a, b) for a, b in zip(grads[1] + grads[2], wants[1] + wants[2]))
+    del graph
+
+
+def test_two_graphs_of_one_topology_replayed_in_turn():
+    """Each graph has a workspace of its own: replays of one do not disturb the other's results."""
+    p = Problem(300, 500, 400, 20, BF16, 2)
+    x2 = (p.x.float() * -0.5).to(BF16)
+    want = [p.forward("silu").clone(), p.forward("silu", x=x2).clone()]
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, x in zip(graphs, (p.x, x2)):
+        with torch.cuda.graph(g):
+            outs.append(p.forward("silu", x=x))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    del graphs
+
+
+def test_large_values():
+    """Pre-activations far out: the activations' limits, no overflow on the way."""
+    p = Problem(40, 64, 48, 8, F32, 1, bias=False)
+    p.x *= 1e3
+    for kind in ("silu", "gelu", "gelu_tanh"):
+        y, saved = p.forward(kind, save=True)
+        f = p.reference(kind)
+        check(y, f.y, f.bound, kind)
+        assert all(torch.isfinite(t).all() for t in p.backward(saved, kind)[1])
+    h = Problem(300, 64, 48, 8, BF16, 1, bias=False)
+    h.x = (h.x.float() * 1e3).to(BF16)
+    for kind in ("silu", "gelu", "gelu_tanh"):
+        y, saved = h.forward(kind, save=True)
+        f = h.reference(kind)
+        check(y, f.y, f.bound, kind)
+        assert all(torch.isfinite(t).all() for t in h.backward(saved, kind)[1])
