@@ -22,13 +22,18 @@ F32, F16, BF16, MX4_TYPE = 0, 1, 2, 3
 _ERR_LEN = 256
 
 
-_TYPES = {}          # torch type -> SPDNN_F32 ..., filled when torch is first needed
+_TYPES = {}          # torch type -> SPDNN_F32 ..., filled with what follows when torch is first needed
+_F32 = _U8 = _raw_stream = None
 _byref, _Operand = C.byref, _lib.Operand
 
 
 def _torch():
     import torch
+    global _F32, _U8, _raw_stream
     if not _TYPES:
+        _F32, _U8 = torch.float32, torch.uint8
+        # torch.cuda.current_stream makes an object for the handle, in twenty times the time
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
     return torch
 
@@ -44,10 +49,10 @@ def _call(fn, *args):
 
 
 def _stream(device: int) -> int:
-    """The handle of torch's current stream; ``torch.cuda.current_stream`` makes an object for it, in twenty times the time."""
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+    """The handle of torch's current stream."""
+    if not _TYPES:
+        _torch()
+    return _raw_stream(device)
 
 
 class MX4:
@@ -55,15 +60,18 @@ class MX4:
     of its ``cols`` columns (include/spdnn_b200.h says what the bytes mean)."""
 
     def __init__(self, codes, scales, cols: int):
-        import torch
-        blocks = (int(cols) + 31) // 32
-        if (codes.dim() != 3 or codes.dtype != torch.uint8 or codes.shape[2] != 16 or codes.shape[1] != blocks or cols < 1
-                or scales.dtype != torch.uint8 or tuple(scales.shape) != tuple(codes.shape[:2])):
+        if not _TYPES:
+            _torch()
+        cols = int(cols)
+        blocks = (cols + 31) // 32
+        shape = codes.shape
+        if len(shape) != 3 or shape[1] != blocks or shape[2] != 16 or scales.shape != shape[:2] or cols < 1 or not (
+                codes.dtype is _U8 and scales.dtype is _U8):
             raise SpDNNError(-1, f"codes must be uint8 [rows, {blocks}, 16] and scales uint8 [rows, {blocks}]")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device or not codes.is_cuda:
+        if not codes.is_cuda or codes.get_device() != scales.get_device() or not codes.is_contiguous() or not scales.is_contiguous():
             raise SpDNNError(-1, "codes and scales must be contiguous and on one GPU")
-        self.codes, self.scales, self.cols = codes, scales, int(cols)
-        self.shape = (int(codes.shape[0]), self.cols)
+        self.codes, self.scales, self.cols = codes, scales, cols
+        self.shape = (shape[0], cols)
 
     @property
     def device(self):
@@ -213,27 +221,30 @@ class SparseTopology:
         return out
 
     # -- calls -----------------------------------------------------------------------
-    def _prepare(self, x, weights, biases, activation):
-        """(tokens, operands of x and the weights, the activation's number) of a call, checked as far as the C side cannot."""
-        if not self._top:
-            raise SpDNNError(-4, "the topology is closed")
-        if self.device is None:
-            raise SpDNNError(-4, "the topology was created for analysis only (device None)")
+    def _begin(self, x, weights, activation):
+        """(tokens, the activation's number, operands of x and the weights, their types) of a call."""
+        if self.device is None or not self._top:
+            raise SpDNNError(-4, "the topology was created for analysis only (device None)" if self._top else "the topology is closed")
         kind = ACTIVATIONS.get(activation)
         if kind is None:
             raise SpDNNError(-1, f"activation must be one of {sorted(ACTIVATIONS)}")
-        torch = _torch()
+        if not _TYPES:
+            _torch()
         if len(x.shape) != 2:
             raise SpDNNError(-1, f"x must be [tokens, {self.inputs}]")
-        tokens = x.shape[0]
-        ops = [_operand(x, tokens, self.inputs, self.device, "x")]
+        tokens, device = x.shape[0], self.device
+        xo = _operand(x, tokens, self.inputs, device, "x")
+        ops = [xo]
         for w in weights:
-            ops.append(_operand(w, self.outputs, self.slots, self.device, "weights"))
-        for b in biases:
-            if b is not None and (b.dtype != torch.float32 or b.shape != (self.outputs,) or b.get_device() != self.device
-                                  or not b.is_contiguous()):
-                raise SpDNNError(-1, f"a bias must be contiguous float32 [{self.outputs}] on the topology's device")
-        return tokens, ops, kind
+            ops.append(_operand(w, self.outputs, self.slots, device, "weights"))
+        return tokens, kind, [_byref(o) for o in ops], xo.type, ops[1].type
+
+    def _bias(self, b):
+        if b is None:
+            return None
+        if b.dtype is not _F32 or b.get_device() != self.device or b.shape != (self.outputs,) or not b.is_contiguous():
+            raise SpDNNError(-1, f"a bias must be contiguous float32 [{self.outputs}] on the topology's device")
+        return b.data_ptr()
 
     def _workspace(self, x, *key):
         """(pointer, bytes, what keeps it alive) of a call's workspace; ``key``: tokens, sets, types of x and w, backward."""
@@ -248,7 +259,7 @@ class SparseTopology:
             size = self._sizes[key] = n.value
         if not size:
             return None, 0, None
-        ws = x.new_empty(size, dtype=_torch().uint8)
+        ws = x.new_empty(size, dtype=_U8)
         return ws.data_ptr(), size, ws
 
     def _saved_operands(self, z, tokens):
@@ -256,8 +267,9 @@ class SparseTopology:
         return [_byref(_Operand(at + s * step, None, self.outputs, F32, 0)) for s in range(z.shape[0])]
 
     def _forward(self, fn, x, weights, biases, activation, clip, save, out_dtype, out):
-        tokens, ops, kind = self._prepare(x, weights, biases, activation)
-        like = x.codes if isinstance(x, MX4) else x
+        tokens, kind, refs, x_type, w_type = self._begin(x, weights, activation)
+        refs += [self._bias(b) for b in biases]
+        like = x.codes if x_type == MX4_TYPE else x
         if out is None:
             if out_dtype is None and like is not x:
                 raise SpDNNError(-1, "out_dtype is needed for microscaled activations")
@@ -266,13 +278,12 @@ class SparseTopology:
         if save:
             if like is not x:
                 raise SpDNNError(-1, "microscaled activations have no backward pass: nothing to save")
-            saved = Saved(x.new_empty((len(weights), tokens, self.outputs), dtype=_torch().float32))
+            saved = Saved(x.new_empty((len(weights), tokens, self.outputs), dtype=_F32))
             z = self._saved_operands(saved.z, tokens)
         else:
-            z = [None] * len(weights)
-        ws, size, keep = self._workspace(like, tokens, len(weights), ops[0].type, ops[1].type, 0)
-        _call(fn, self._top, tokens, *map(_byref, ops), *[None if b is None else b.data_ptr() for b in biases], kind, clip, _byref(y), *z,
-              ws, size, _stream(self.device))
+            z = (None,) * len(weights)
+        ws, size, keep = self._workspace(like, tokens, len(weights), x_type, w_type, 0)
+        _call(fn, self._top, tokens, *refs, kind, clip, _byref(y), *z, ws, size, _stream(self.device))
         return (out, saved) if save else out
 
     def linear(self, x, w, bias=None, activation: str = "none", clip: float = 32.0, save: bool = False, out_dtype=None, out=None):
@@ -286,24 +297,24 @@ class SparseTopology:
         return self._forward(self._lib.spdnn_gated, x, [w_gate, w_up], [bias_gate, bias_up], activation, clip, save, out_dtype, out)
 
     def _backward(self, fn, dy, x, weights, saved, activation, clip, need_dx, need_dw):
-        tokens, ops, kind = self._prepare(x, weights, (), activation)
-        if isinstance(x, MX4):
+        tokens, kind, refs, x_type, w_type = self._begin(x, weights, activation)
+        if x_type == MX4_TYPE:
             raise SpDNNError(-1, "microscaled activations have no backward pass")
         z = getattr(saved, "z", None)
         if z is None or z.shape != (len(weights), tokens, self.outputs) or z.get_device() != self.device:
             raise SpDNNError(-1, "saved must be what the forward call returned")
-        dy_op = _byref(_operand(dy, tokens, self.outputs, self.device, "dy"))
-        dx = dx_op = None
+        dy_ref = _byref(_operand(dy, tokens, self.outputs, self.device, "dy"))
+        dx = dx_ref = None
         if need_dx:
             dx = x.new_empty((tokens, self.inputs))
-            dx_op = _byref(_operand(dx, tokens, self.inputs, self.device, "dx"))
-        f32 = _torch().float32
-        grads = [None] * (2 * len(weights))
+            dx_ref = _byref(_Operand(dx.data_ptr(), None, self.inputs, x_type, 0))
+        grads = pointers = (None,) * (2 * len(weights))
         if need_dw:
-            grads = [x.new_empty((self.outputs, self.slots), dtype=f32) for _ in weights] + [x.new_empty(self.outputs, dtype=f32) for _ in weights]
-        ws, size, keep = self._workspace(x, tokens, len(weights), ops[0].type, ops[1].type, 1)
-        _call(fn, self._top, tokens, dy_op, *map(_byref, ops), *self._saved_operands(z, tokens), kind, clip, dx_op,
-              *[None if t is None else t.data_ptr() for t in grads], ws, size, _stream(self.device))
+            grads = [x.new_empty((self.outputs, self.slots), dtype=_F32) for _ in weights] + [x.new_empty(self.outputs, dtype=_F32) for _ in weights]
+            pointers = [t.data_ptr() for t in grads]
+        ws, size, keep = self._workspace(x, tokens, len(weights), x_type, w_type, 1)
+        _call(fn, self._top, tokens, dy_ref, *refs, *self._saved_operands(z, tokens), kind, clip, dx_ref, *pointers, ws, size,
+              _stream(self.device))
         return (dx, *grads)
 
     def linear_backward(self, dy, x, w, saved, activation: str = "none", clip: float = 32.0, need_dx: bool = True, need_dw: bool = True):
