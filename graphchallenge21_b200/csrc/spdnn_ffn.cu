@@ -169,9 +169,6 @@ bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
 int64_t aligned(int64_t n) { return (n + 255) & ~255ll; }
 
 constexpr int64_t kSharedLimit = 227 * 1024;
-#ifndef SPDNN_BLOCK_TOKENS
-#define SPDNN_BLOCK_TOKENS 17
-#endif
 
 int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
@@ -186,9 +183,11 @@ int neurons_at_a_time(int rows, int sets) {
     return 8 / (p / lane_units(p));
 }
 
-// Blocks take 16-bit operands of one type and whole tiles of 64 tokens.
+// Blocks take 16-bit operands of one type and whole tiles of 64 tokens.  From 17 tokens on they are no more than a microsecond or four slower
+// than the gather by connections (1024 neurons, 256 tokens, forward / backward 9.1 / 21.5 and 8.1 / 17.5 us), and soon faster
+// (4096 neurons, 256 tokens 9.8 / 27.9 and 11.6 / 36.4).
 bool go_by_blocks(const DeviceBlocks &b, int tokens, int image_type, int weight_type) {
-    return b.blocks && tokens >= SPDNN_BLOCK_TOKENS && image_type != F32 && image_type == weight_type;
+    return b.blocks && tokens >= 17 && image_type != F32 && image_type == weight_type;
 }
 
 GatherPlan make_plan(const spdnn_topology &top, bool forward, int tokens, int sets, int image_type, int weight_type) {
@@ -459,12 +458,12 @@ int check_blocks(const Call &c, const GatherPlan &g) {
     return SPDNN_OK;
 }
 
-// Tokens that one launch of few_kernel takes at a time, or 0: the images' way.  It wins up to about 2^22 multiply-adds a set (us, few_kernel
-// against the images: 4096 -> 16384, 32 connections, bf16, 8 tokens 11.1 and 12.4, 12 tokens 19.5 and 14.8; 1024 -> 4096, 24 tokens
-// 11.8 and 13.2), in at most four groups of tokens.
+// Tokens that one launch of few_kernel takes at a time, or 0: the images' way.  Up to about 2^21 multiply-adds a set its one launch takes no
+// longer than their two (us on the GPU, few_kernel and images: 4096 -> 16384, 32 connections, 4 tokens 7 and 11, 8 tokens 11 and 11;
+// 4096 -> 4096, 17 tokens 14 and 8), in at most four groups of tokens.
 int few_tokens(const spdnn_topology &top, int tokens, int x_type) {
     const int64_t row = (int64_t)(top.host.inputs + 1) * type_size(image_type(x_type));
-    if (tokens * (int64_t)top.host.outputs * top.host.slots > 1ll << 22 && tokens > 1) return 0;
+    if (tokens * (int64_t)top.host.outputs * top.host.slots > 1ll << 21 && tokens > 1) return 0;
     int T = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
     if (x_type == F32) T = std::min(T, 4);
     while (T > 1 && row * T > kSharedLimit / 2) T /= 2;

@@ -679,14 +679,9 @@ struct GatherArgs {
 
 // Units a lane reads per gathered value, and threads per block.  Two units halve what index, weights and the loop cost per fma; with more sums
 // than 16 in registers a block of 1024 threads would spill.
-#ifndef SPDNN_NV
-#define SPDNN_NV 2
-#endif
-#ifndef SPDNN_BIG
-#define SPDNN_BIG 768
-#endif
-__host__ __device__ constexpr int lane_units(int P) { return P < SPDNN_NV ? P : SPDNN_NV; }
-__host__ __device__ constexpr int gather_threads(int sums) { return sums <= 16 ? 1024 : SPDNN_BIG; }
+// (4096 tokens 1024 -> 4096, gated: two units 90 us, one 129; 768 threads 90, 1024 97).
+__host__ __device__ constexpr int lane_units(int P) { return P < 2 ? P : 2; }
+__host__ __device__ constexpr int gather_threads(int sums) { return sums <= 16 ? 1024 : 768; }
 
 // Brings `bytes` (a multiple of 16) from global to shared memory, 16 bytes per thread and copy, none of them through registers.
 __device__ __forceinline__ void copy_in(void *dst, const void *src, uint32_t bytes) {
@@ -1142,41 +1137,30 @@ struct BlockArgs {
     int whole_y, whole_z;        // rows of y, of z begin on 16 bytes: blocks of 16 neighbours are stored in whole sectors
 };
 
-#ifndef SPDNN_BW
-#define SPDNN_BW 16
-#define SPDNN_BS 2
-#endif
-constexpr int kBlockWarps = SPDNN_BW, kBlockStages = SPDNN_BS;
+// 16 warps of two stages (1024 tokens of the butterfly 16384, gated: 32 us) rather than 12 of three (38) or 8 of four (43).
+constexpr int kBlockWarps = 16, kBlockStages = 2;
 __host__ __device__ constexpr int block_stage_bytes(int G) { return 32 * 128 + 1024 * G; }
 
-// Stores 64 tokens x 16 neighbouring neurons of a warp's fragments (value(m, half, i), laid out as block_kernel's accumulators) through 4 KB of
-// shared memory of its own, 16 bytes a lane: fragments hold two neighbours of eight tokens, an eighth of a sector each.
+// Stores 64 tokens x 16 neighbouring neurons of a warp's fragments (value(m, half, i), laid out as block_kernel's accumulators) in a 16-bit type
+// through 2 KB of shared memory of its own, 16 bytes a lane: fragments hold two neighbours of eight tokens, an eighth of a sector each.
 template <class T, class F>
 __device__ __forceinline__ void store_block(unsigned char *stage, T *to, int64_t stride, int tokens, const F &value) {
     const int lane = threadIdx.x & 31;
-    constexpr int PIECES = (int)sizeof(T);             // of 16 bytes in a row of 16 neurons (4 or 2), turned against each other by token
-    const auto place = [](int token, int piece) { return token * (16 * PIECES) + ((piece ^ (PIECES == 4 ? token >> 1 & 3 : token >> 2 & 1)) * 16); };
+    // halves of a token's 32 bytes, turned against each other for neighbouring tokens to meet on fewer banks
+    const auto place = [](int token, int half) { return token * 32 + ((half ^ (token >> 2 & 1)) * 16); };
     __syncwarp();
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int token = m * 16 + i * 8 + lane / 4;
-                const float lo = value(m, half, 2 * i), hi = value(m, half, 2 * i + 1);
-                if constexpr (sizeof(T) == 4) {
-                    *(float2 *)(stage + place(token, half * 2 + (lane >> 1 & 1)) + (lane & 1) * 8) = make_float2(lo, hi);
-                } else {
-                    T both[2] = {from_float<T>(lo), from_float<T>(hi)};
-                    *(uint32_t *)(stage + place(token, half) + (lane & 3) * 4) = *(const uint32_t *)both;
-                }
-            }
+            for (int i = 0; i < 2; ++i)
+                *(uint32_t *)(stage + place(m * 16 + i * 8 + lane / 4, half) + (lane & 3) * 4) = pair_bits<T>(value(m, half, 2 * i), value(m, half, 2 * i + 1));
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 2 * PIECES; ++i) {
-        const int token = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
-        if (token < tokens) *(uint4 *)((char *)(to + token * stride) + piece * 16) = *(const uint4 *)(stage + place(token, piece));
+    for (int i = 0; i < 4; ++i) {
+        const int token = i * 16 + lane / 2, half = lane & 1;
+        if (token < tokens) *(uint4 *)((char *)(to + token * stride) + half * 16) = *(const uint4 *)(stage + place(token, half));
     }
 }
 
@@ -1194,7 +1178,7 @@ __device__ __forceinline__ void copy_16(uint32_t to, const void *from) {
 }
 
 // A warp takes 64 tokens of a block (16 neurons over the same rows) at a time: a chunk of 32 rows x 64 tokens and its weights come into the warp's
-// own stages with cp.async, three chunks ahead; ldmatrix.trans turns 16 rows x 16 tokens into a fragment of tokens x rows, wherever the rows
+// own stages with cp.async, a chunk ahead; ldmatrix.trans turns 16 rows x 16 tokens into a fragment of tokens x rows, wherever the rows
 // came from, and the products (16 tokens x 8 neurons x 16 rows) run on the tensor cores.  One gathered value serves 16 neurons and
 // both sets, where gather_kernel's serves one: what is left is bringing the rows in (each is used by as many blocks as list it) and the results
 // out.  The contraction is 16 wide: mma.sync, not tcgen05, whose tile of 128 tokens and its round trip through tensor memory would have the
@@ -1312,9 +1296,24 @@ __global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_co
                 }
         }
         const auto store = [&](auto *to, int64_t stride, bool whole, const auto &value) {
+            using T = typename std::remove_pointer<decltype(to)>::type;
             to += tile0 * stride;
             if (whole && neighbours) {
-                store_block(scratch, to + head, stride, tokens, value);
+                if constexpr (sizeof(T) == 4) {
+                    // four lanes' pairs fill a sector as they are
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int token = m * 16 + i * 8 + lane / 4;
+                            if (token >= tokens) continue;
+                            T *row = to + token * stride + head + (lane & 3) * 2;
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) *(float2 *)(row + half * 8) = make_float2(value(m, half, 2 * i), value(m, half, 2 * i + 1));
+                        }
+                } else {
+                    store_block(scratch, to + head, stride, tokens, value);
+                }
                 return;
             }
 #pragma unroll
@@ -1324,7 +1323,7 @@ __global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int token = m * 16 + i / 2 * 8 + lane / 4, neuron = i & 1 ? c[half].y : c[half].x;
-                        if (token < tokens && neuron >= 0) to[token * stride + neuron] = from_float<typename std::remove_pointer<decltype(to)>::type>(value(m, half, i));
+                        if (token < tokens && neuron >= 0) to[token * stride + neuron] = from_float<T>(value(m, half, i));
                     }
         };
         if (a.z0) {

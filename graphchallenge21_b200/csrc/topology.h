@@ -62,11 +62,9 @@ struct Topology {
 // Most entries of a gather table (4 bytes of index, 4 of source): a slice is as long as its longest neuron.
 constexpr int64_t kMostEntries = 1ll << 30;
 constexpr int kMostSlots = 4096;       // as canonicalize_layer
-// Blocks are used where their products have at most this many times the connections.
-#ifndef SPDNN_BLOCK_WASTE
-#define SPDNN_BLOCK_WASTE 4
-#endif
-constexpr int64_t kBlockWaste = SPDNN_BLOCK_WASTE;
+// Blocks are used where their products have at most this many times the connections (1024 tokens, 4096 neurons, 32 connections, bf16, gated, us
+// forward / backward by blocks: 15 / 66 where 16 neurons share their rows, 27 / 88 where 8 do, 44 / 129 where 4 do; by connections 27 / 97).
+constexpr int64_t kBlockWaste = 2;
 
 // Orders the connections of `lanes` (2, 4, 8 or 16) neighbouring neurons, whose lanes read their k-th connections at the same time, so
 // that those fall on different banks: into steps in which the gathered rows belong to different CLASSES, row mod `lanes` (spdnn_ffn.cuh

@@ -486,6 +486,7 @@ class Shared(Problem):
 @pytest.mark.parametrize("tokens, inputs, outputs, slots, group, scattered", [
     (17, 256, 320, 32, 16, False), (64, 256, 320, 32, 16, True), (65, 512, 100, 48, 16, False), (200, 128, 96, 20, 10, True),
     (130, 1024, 1024, 32, 16, True), (77, 300, 333, 45, 15, False), (64, 64, 33, 32, 32, False), (31, 96, 1600, 8, 8, False),
+    (130, 360, 350, 30, 12, True), (18, 640, 77, 64, 16, True),
 ])
 def test_steps_of_neurons_that_share_their_inputs(tokens, inputs, outputs, slots, group, scattered, sets, dtype):
     check_step(Shared(tokens, inputs, outputs, slots, dtype, sets, group, scattered), "gelu")
