@@ -215,22 +215,21 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
     return "";
 }
 
-// The blocks of a gather.  start[i]: where the entries of neuron i begin in row_of / source_of (start has outs + 1 entries).
-template <class Row, class Source>
-inline void build_block_table(int outs, int rows, const std::vector<size_t> &start, const Row &row_of, const Source &source_of, BlockTable &t) {
-    const auto length = [&](int i) { return start[i + 1] - start[i]; };
+// The blocks of a gather: neuron i gathers row(i, k) for k < length(i), with the weight at source(i, k).
+template <class Length, class Row, class Source>
+inline void build_block_table(int outs, int rows, int64_t entries, const Length &length, const Row &row, const Source &source, BlockTable &t) {
     std::unordered_map<uint64_t, int> newest;          // hash of a list -> the class that was opened last for it
     std::vector<int> first, older;                     // of a class: its first neuron; the class before it with the same hash
     std::vector<std::vector<int32_t>> members;
     const auto same = [&](int i, int j) {
         if (length(i) != length(j)) return false;
         for (size_t k = 0; k < length(i); ++k)
-            if (row_of(start[i] + k) != row_of(start[j] + k)) return false;
+            if (row(i, k) != row(j, k)) return false;
         return true;
     };
     for (int i = 0; i < outs; ++i) {
         uint64_t h = 0x9E3779B97F4A7C15ull ^ length(i);
-        for (size_t k = start[i]; k < start[i + 1]; ++k) h = (h ^ row_of(k)) * 0xBF58476D1CE4E5B9ull, h ^= h >> 29;
+        for (size_t k = 0; k < length(i); ++k) h = (h ^ row(i, k)) * 0xBF58476D1CE4E5B9ull, h ^= h >> 29;
         const auto found = newest.find(h);
         int c = found == newest.end() ? -1 : found->second;
         while (c >= 0 && !same(first[c], i)) c = older[c];
@@ -251,7 +250,6 @@ inline void build_block_table(int outs, int rows, const std::vector<size_t> &sta
         blocks += b;
         chunks += b * (int64_t)std::max<size_t>(1, (length(first[c]) + 31) / 32);
     }
-    const int64_t entries = (int64_t)start[outs];
     if (!entries || chunks * 512 > entries * kBlockWaste) return;
     t.blocks = (int)blocks;
     t.chunk_ptr.assign(1, 0);
@@ -264,9 +262,9 @@ inline void build_block_table(int outs, int rows, const std::vector<size_t> &sta
         for (size_t m = 0; m < members[c].size(); m += 16, ++block) {
             const size_t n = length(first[c]);
             for (size_t k = 0; k < n; ++k) {
-                t.rows[chunk * 32 + k] = row_of(start[first[c]] + k);
+                t.rows[chunk * 32 + k] = row(first[c], k);
                 for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j)
-                    t.src[(chunk + k / 32) * 512 + fragment((int)(k % 32), (int)(j - m))] = source_of(start[members[c][j]] + k);
+                    t.src[(chunk + k / 32) * 512 + fragment((int)(k % 32), (int)(j - m))] = source(members[c][j], k);
             }
             for (size_t j = m; j < std::min(m + 16, members[c].size()); ++j) t.members[block * 16 + (j - m)] = members[c][j];
             chunk += std::max<size_t>(1, (n + 31) / 32);        // neurons without connections have a chunk of padding
@@ -315,23 +313,22 @@ inline std::string build_topology(int inputs, int outputs, const int32_t *col_pt
         for (uint32_t k = 0; k < in_count[c]; ++k) emit((uint32_t)r[k], (uint32_t)((size_t)c * most + k));
     }, forward_lanes, t.forward);
     if (!why.empty()) return why;
-    std::vector<size_t> in_start((size_t)outputs + 1, 0);
-    for (int c = 0; c < outputs; ++c) in_start[c + 1] = (size_t)col_ptr[c + 1];
     // the transposed lists, outputs ascending
     std::vector<size_t> start((size_t)inputs + 1, 0);
     for (int i = 0; i < inputs; ++i) start[i + 1] = start[i] + out_count[i];
-    std::vector<uint32_t> by_input((size_t)nnz), flat((size_t)nnz);
+    std::vector<uint32_t> by_input((size_t)nnz);
     std::vector<size_t> at(start.begin(), start.end() - 1);
     for (int c = 0; c < outputs; ++c)
         for (uint32_t k = 0; k < in_count[c]; ++k) {
             const size_t p = (size_t)c * most + k;
             by_input[at[t.rows[p]]++] = (uint32_t)p;
-            flat[in_start[c] + k] = (uint32_t)p;
         }
-    build_block_table(outputs, inputs, in_start, [&](size_t e) { return (uint32_t)t.rows[flat[e]]; }, [&](size_t e) { return flat[e]; },
-                      t.forward_blocks);
-    build_block_table(inputs, outputs, start, [&](size_t e) { return by_input[e] / (uint32_t)most; }, [&](size_t e) { return by_input[e]; },
-                      t.backward_blocks);
+    build_block_table(outputs, inputs, nnz, [&](int c) { return (size_t)in_count[c]; },
+                      [&](int c, size_t k) { return (uint32_t)t.rows[(size_t)c * most + k]; },
+                      [&](int c, size_t k) { return (uint32_t)((size_t)c * most + k); }, t.forward_blocks);
+    build_block_table(inputs, outputs, nnz, [&](int i) { return (size_t)out_count[i]; },
+                      [&](int i, size_t k) { return by_input[start[i] + k] / (uint32_t)most; },
+                      [&](int i, size_t k) { return by_input[start[i] + k]; }, t.backward_blocks);
     return build_gather_table(inputs, outputs, out_count, [&](int i, auto emit) {
         for (size_t e = start[i]; e < start[i + 1]; ++e) emit(by_input[e] / (uint32_t)most, by_input[e]);
     }, backward_lanes, t.backward);

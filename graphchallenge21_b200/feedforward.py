@@ -179,6 +179,8 @@ class SparseTopology:
     def from_rows(cls, rows, inputs: int, device: int | None = 0):
         """``rows`` int [outputs, K]: the inputs of every output (entries < 0 are skipped), as ``SpDNN.set_layer_rows``."""
         rows = np.asarray(rows)
+        if rows.size and rows.min() >= 0:
+            return cls(inputs, rows.shape[0], np.arange(rows.shape[0] + 1, dtype=np.int64) * rows.shape[1], rows.reshape(-1), device)
         keep = rows >= 0
         col_ptr = np.concatenate([[0], np.cumsum(keep.sum(axis=1))])
         return cls(inputs, rows.shape[0], col_ptr, rows[keep], device)
