@@ -99,6 +99,14 @@ cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, cudaStre
     }, values);
 }
 
+constexpr int64_t kSharedLimit = 227 * 1024;
+
+// Lets a kernel have more shared memory than a launch has by default: always as much as there is, never the size of this launch, since another
+// thread may be about to launch the same kernel with more.
+cudaError_t allow_shared(const void *kernel, size_t shared) {
+    return shared > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedLimit) : cudaSuccess;
+}
+
 // The device of the topology for the length of a call.
 struct OnDevice {
     int before = -1;
@@ -168,7 +176,6 @@ int type_size(int type) { return type == F32 ? 4 : 2; }
 bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
 int64_t aligned(int64_t n) { return (n + 255) & ~255ll; }
 
-constexpr int64_t kSharedLimit = 227 * 1024;
 
 int64_t image_size(int rows, int sets, int v, int p, int size) {
     return ((int64_t)image_units(rows, p * sets) * v * size + 127) / 128 * 128;
@@ -284,10 +291,7 @@ cudaError_t launch_gather(const GatherPlan &g, GatherArgs a, int image_type, int
     a.splits = g.splits;
     a.image_bytes = g.image_bytes;
     const size_t shared = g.global ? 0 : (size_t)g.image_bytes;
-    if (shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-        if (e != cudaSuccess) return e;
-    }
+    if (const cudaError_t e = allow_shared(kernel, shared)) return e;
     void *args[] = {&a};
     const int threads = gather_threads(g.v * lane_units(g.p) * (s == 2 ? 1 : sets));
     return cudaLaunchKernel(kernel, dim3((unsigned)(g.tiles * g.splits)), dim3(threads), args, shared, stream);
@@ -308,8 +312,7 @@ cudaError_t launch_blocks(const spdnn_topology &top, const GatherPlan &g, const 
     };
     const auto kernel = image_type == BF16 ? of(bf16()) : of(__half());
     const int shared = kBlockWarps * kBlockStages * block_stage_bytes(s == 2 ? 1 : sets);
-    const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-    if (e != cudaSuccess) return e;
+    if (const cudaError_t e = allow_shared((const void *)kernel, (size_t)shared)) return e;
     const int64_t want = ((int64_t)b.blocks * g.tiles + kBlockWarps - 1) / kBlockWarps;
     void *args[] = {&k};
     return cudaLaunchKernel((const void *)kernel, dim3((unsigned)std::min<int64_t>(want, top.sm_count)), dim3(kBlockWarps * 32), args, (size_t)shared, stream);
@@ -503,10 +506,7 @@ cudaError_t launch_few(const Call &c, int T, const float *b0, const float *b1) {
     };
     const void *kernel = it == F32 ? of(float()) : it == F16 ? of(__half()) : of(bf16());
     const size_t shared = (size_t)(h.inputs + 1) * T * type_size(it);
-    if (shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-        if (e != cudaSuccess) return e;
-    }
+    if (const cudaError_t e = allow_shared(kernel, shared)) return e;
     const int64_t want = (h.outputs + kFewThreads / 8 - 1) / (kFewThreads / 8);
     const int per_sm = shared > (size_t)kSharedLimit / 4 ? 1 : 4;
     void *args[] = {&a};

@@ -497,8 +497,6 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
                         d0[k] *= slope;
                     }
                 });
-                // behind the last neuron there is nothing to be read but zeros
-
             }
         }
 #pragma unroll
@@ -665,7 +663,7 @@ struct GatherArgs {
     const void *image;          // tiles of image_bytes
     int64_t image_bytes;
     const uint32_t *slice_ptr;  // the gather table (topology.h)
-    const void *index;          // order_kernel's: uint16_t (image in shared memory) or uint32_t
+    const void *index;          // order_block's: uint16_t (image in shared memory) or uint32_t
     const void *weights;
     int outs, tokens, splits;
     const float *bias0, *bias1; // or nullptr
@@ -678,8 +676,7 @@ struct GatherArgs {
 };
 
 // Units a lane reads per gathered value, and threads per block.  Two units halve what index, weights and the loop cost per fma; with more sums
-// than 16 in registers a block of 1024 threads would spill.
-// (4096 tokens 1024 -> 4096, gated: two units 90 us, one 129; 768 threads 90, 1024 97).
+// than 16 in registers a block of 1024 threads would spill (4096 tokens 1024 -> 4096, gated: two units 90 us, one 129; 768 threads 90, 1024 97).
 __host__ __device__ constexpr int lane_units(int P) { return P < 2 ? P : 2; }
 __host__ __device__ constexpr int gather_threads(int sums) { return sums <= 16 ? 1024 : 768; }
 

@@ -222,7 +222,7 @@ int spdnn_layer_static(const float *yin, float *yout, int neurons, int live_in, 
  *
  * A TOPOLOGY says which inputs every output neuron is connected to; the weights are arguments of the calls.  It does not change
  * once created: calls on one topology may overlap, on several streams and from several threads, each with a workspace of
- * its own.  Destroy it when no call on it is in flight.
+ * its own.  Destroy it when no call on it is in flight and no graph that holds one will be replayed.
  *
  * A set of weights is a matrix [outputs][slots] in CANONICAL order: connection j of a neuron is its j-th smallest input
  * (spdnn_topology_rows).  What a matrix holds where a neuron has no j-th connection is never read; gradients are zero there.

@@ -587,3 +587,30 @@ def test_large_values():
         f = h.reference(kind)
         check(y, f.y, f.bound, kind)
         assert all(torch.isfinite(t).all() for t in h.backward(saved, kind)[1])
+
+
+def test_two_threads_with_images_of_different_sizes():
+    """The same kernel launched from two threads with different amounts of shared memory."""
+    import threading
+    a = Problem(40, 4000, 300, 16, BF16, 2)
+    b = Problem(60, 6900, 300, 16, BF16, 2)
+    want = [p.forward("silu", save=True) for p in (a, b)]
+    grads = [p.backward(s, "silu")[0] for p, (_, s) in zip((a, b), want)]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(p, y, g):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(150):
+                    got, saved = p.forward("silu", save=True)
+                    dx = p.backward(saved, "silu", need_dw=False)[0]
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(got, y) and torch.equal(dx, g)
+        except Exception as e:                             # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(p, y, g)) for p, (y, _), g in zip((a, b), want, grads)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
