@@ -614,3 +614,35 @@ def test_two_threads_with_images_of_different_sizes():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not errors, errors
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_offsets_beyond_32_bits(shared):
+    """More than 2^31 activations in one call: its last tokens as a call of their own gives them."""
+    tokens, inputs, outputs = 140001, 16384, 32
+    p = (Shared(1, inputs, outputs, 16, BF16, 1, 16, False) if shared else Problem(1, inputs, outputs, 16, BF16, 1))
+    x = torch.zeros(tokens, inputs, dtype=BF16, device="cuda")
+    assert x.numel() > 2 ** 31
+    g = torch.Generator("cuda").manual_seed(5)
+    tail = torch.randn(500, inputs, device="cuda", generator=g).to(BF16)
+    x[-500:] = tail
+    dy = torch.zeros(tokens, outputs, dtype=BF16, device="cuda")
+    dy[-500:] = torch.randn(500, outputs, device="cuda", generator=g).to(BF16)
+    y, saved = p.top.linear(x, p.w[0], p.b[0], activation="silu", save=True)
+    small, kept = p.top.linear(tail, p.w[0], p.b[0], activation="silu", save=True)
+    assert torch.equal(y[-500:], small) and torch.equal(y[0], y[70000])
+    dx, dw, db = p.top.linear_backward(dy, x, p.w[0], saved, activation="silu")
+    dx2, dw2, db2 = p.top.linear_backward(dy[-500:], tail, p.w[0], kept, activation="silu")
+    assert torch.equal(dx[-500:], dx2) and not dx[:-500].any()
+    # the same products, added up in another order: 500 terms and their zeros
+    bound = 2 * 510 * ref.U * (tail.double().abs().t() @ dy[-500:].double().abs()).max()
+    assert float((dw - dw2).abs().max()) <= bound and float((db - db2).abs().max()) <= bound
+    del x, dx, y, saved
+    from graphchallenge21_b200 import mx4_quantize
+    big = torch.zeros(70000, 33000, dtype=BF16, device="cuda")
+    big[-3:] = torch.randn(3, 33000, device="cuda", generator=g).to(BF16)
+    q = mx4_quantize(big)
+    last = mx4_quantize(big[-3:])
+    assert torch.equal(q.codes[-3:], last.codes) and torch.equal(q.scales[-3:], last.scales) and not q.codes[:-3].any()
+    values = q.dequantize(BF16)
+    assert torch.equal(values[-3:], last.dequantize(BF16)) and not values[:-3].any()
