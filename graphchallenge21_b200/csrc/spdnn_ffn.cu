@@ -670,14 +670,14 @@ int run_backward(const Call &c, const Gradients &d) {
 
 // ---- topologies ------------------------------------------------------------------------------------
 
-extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inputs, int outputs, const int32_t *col_ptr,
+extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inputs, int outputs, int slots, const int32_t *col_ptr,
                                      const int32_t *row_idx, char *err, int err_len) {
     if (!out) return fail(err, err_len, SPDNN_ERR_ARG, "null handle pointer");
     *out = nullptr;
     spdnn_topology *t = nullptr;
     try {
         t = new spdnn_topology();
-        const std::string why = build_topology(inputs, outputs, col_ptr, row_idx, neurons_at_a_time(std::max(inputs, 1), 1),
+        const std::string why = build_topology(inputs, outputs, slots, col_ptr, row_idx, neurons_at_a_time(std::max(inputs, 1), 1),
                                                neurons_at_a_time(std::max(outputs, 1), 2), t->host);
         if (!why.empty()) {
             delete t;

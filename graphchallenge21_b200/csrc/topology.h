@@ -273,9 +273,9 @@ inline void build_block_table(int outs, int rows, int64_t entries, const Length 
         }
 }
 
-// Returns an empty string on success, else the reason the topology is rejected.
-// forward_lanes, backward_lanes: see BankOrder.
-inline std::string build_topology(int inputs, int outputs, const int32_t *col_ptr, const int32_t *row_idx, int forward_lanes, int backward_lanes,
+// Returns an empty string on success, else the reason the topology is rejected.  slots: width of a weight matrix, 0 = as many as the output with
+// most connections has.  forward_lanes, backward_lanes: see BankOrder.
+inline std::string build_topology(int inputs, int outputs, int slots, const int32_t *col_ptr, const int32_t *row_idx, int forward_lanes, int backward_lanes,
                                   Topology &t) {
     if (inputs <= 0 || outputs <= 0 || inputs >= (1 << 26) || outputs >= (1 << 26)) return "inputs and outputs must be in [1, 2^26)";
     if (!col_ptr) return "col_ptr is null";
@@ -289,6 +289,8 @@ inline std::string build_topology(int inputs, int outputs, const int32_t *col_pt
     }
     const int64_t nnz = col_ptr[outputs];
     if (nnz && !row_idx) return "row_idx is null";
+    if (slots < 0 || slots > kMostSlots || (slots > 0 && slots < most)) return "slots must be 0, or at least an output's connections and at most 4096";
+    if (slots) most = slots;
     if ((int64_t)outputs * most >= (1ll << 31)) return "outputs times connections per output must stay below 2^31";
     t.inputs = inputs; t.outputs = outputs; t.slots = most; t.connections = nnz;
     t.rows.assign((size_t)outputs * most, -1);

@@ -154,9 +154,10 @@ class Saved:
 
 class SparseTopology:
     """The connections between ``inputs`` and ``outputs`` neurons, as CSC: output c is connected to inputs
-    ``row_idx[col_ptr[c]:col_ptr[c + 1]]``.  ``device=None``: analysis only (``rows``, ``pack``), no GPU needed."""
+    ``row_idx[col_ptr[c]:col_ptr[c + 1]]``.  ``slots``: columns of a weight matrix (0: as many as the output with most
+    connections has).  ``device=None``: analysis only (``rows``, ``pack``), no GPU needed."""
 
-    def __init__(self, inputs: int, outputs: int, col_ptr, row_idx, device: int | None = 0):
+    def __init__(self, inputs: int, outputs: int, col_ptr, row_idx, device: int | None = 0, slots: int = 0):
         self._top = C.c_void_p()
         self._lib = _lib.load()
         self._sizes = {}                 # workspaces: a function of these arguments and the topology
@@ -168,7 +169,7 @@ class SparseTopology:
             raise SpDNNError(-1, "row_idx size must equal col_ptr[-1]")
         self._col_ptr, self._row_idx = col_ptr, row_idx
         self.device = None if device is None else int(device)
-        _call(self._lib.spdnn_topology_create, C.byref(self._top), -1 if device is None else self.device, inputs, outputs,
+        _call(self._lib.spdnn_topology_create, C.byref(self._top), -1 if device is None else self.device, inputs, outputs, slots,
               C.c_void_p(col_ptr.ctypes.data), C.c_void_p(row_idx.ctypes.data))
         slots, fan_out, connections = C.c_int(), C.c_int(), C.c_int64()
         self._lib.spdnn_topology_info(self._top, None, None, C.byref(slots), C.byref(fan_out), C.byref(connections))
@@ -177,13 +178,15 @@ class SparseTopology:
 
     @classmethod
     def from_rows(cls, rows, inputs: int, device: int | None = 0):
-        """``rows`` int [outputs, K]: the inputs of every output (entries < 0 are skipped), as ``SpDNN.set_layer_rows``."""
+        """``rows`` int [outputs, K]: the inputs of every output (entries < 0 are skipped), as ``SpDNN.set_layer_rows``; weight
+        matrices are [outputs, K]."""
         rows = np.asarray(rows)
         if rows.size and rows.min() >= 0:
-            return cls(inputs, rows.shape[0], np.arange(rows.shape[0] + 1, dtype=np.int64) * rows.shape[1], rows.reshape(-1), device)
+            return cls(inputs, rows.shape[0], np.arange(rows.shape[0] + 1, dtype=np.int64) * rows.shape[1], rows.reshape(-1), device,
+                       rows.shape[1])
         keep = rows >= 0
         col_ptr = np.concatenate([[0], np.cumsum(keep.sum(axis=1))])
-        return cls(inputs, rows.shape[0], col_ptr, rows[keep], device)
+        return cls(inputs, rows.shape[0], col_ptr, rows[keep], device, rows.shape[1])
 
     def close(self):
         """Frees the device tables.  No call on the topology may be in flight."""

@@ -249,13 +249,14 @@ typedef struct spdnn_operand {
 } spdnn_operand_t;
 
 /* Topology as CSC: output c is connected to inputs row_idx[col_ptr[c] .. col_ptr[c+1]), in any order (at most 4096; repeated
- * entries stay separate connections).  Host arrays, borrowed for the call.  device -1: analysis only, for
+ * entries stay separate connections).  slots: columns of a weight matrix, at least the connections of every output; 0 = as many as
+ * the output with most has (1 if none has any).  Host arrays, borrowed for the call.  device -1: analysis only, for
  * spdnn_topology_info and _rows, without a GPU.  Call it outside stream captures (it allocates). */
-int spdnn_topology_create(spdnn_topology_t **top, int device, int inputs, int outputs, const int32_t *col_ptr,
+int spdnn_topology_create(spdnn_topology_t **top, int device, int inputs, int outputs, int slots, const int32_t *col_ptr,
                           const int32_t *row_idx, char *err, int err_len);
 void spdnn_topology_destroy(spdnn_topology_t *top);
 
-/* slots: connections of the output that has most, at least 1; fan_out: most outputs that one input feeds.  Pointers may be NULL. */
+/* slots: columns of a weight matrix; fan_out: most outputs that one input feeds.  Pointers may be NULL. */
 int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int *outputs, int *slots, int *fan_out, int64_t *connections);
 
 /* The canonical order, to host memory: rows[outputs][slots] = inputs of every output ascending, -1 behind the last one. */

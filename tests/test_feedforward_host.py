@@ -54,17 +54,17 @@ def test_malformed_topologies_are_refused(inputs, outputs, col_ptr, row_idx, say
     lib = _lib.load()
     cp, ri = np.array(col_ptr, np.int32), np.array(row_idx, np.int32)
     top = C.c_void_p(1)
-    rc, msg = err_of(lib.spdnn_topology_create, C.byref(top), -1, inputs, outputs, cp.ctypes.data, ri.ctypes.data)
+    rc, msg = err_of(lib.spdnn_topology_create, C.byref(top), -1, inputs, outputs, 0, cp.ctypes.data, ri.ctypes.data)
     assert rc == -1 and says in msg and not top.value
 
 
 def test_null_arguments_are_refused():
     lib = _lib.load()
     top = C.c_void_p()
-    assert err_of(lib.spdnn_topology_create, None, -1, 4, 4, None, None)[0] == -1
-    assert err_of(lib.spdnn_topology_create, C.byref(top), -1, 4, 4, None, None)[0] == -1
+    assert err_of(lib.spdnn_topology_create, None, -1, 4, 4, 0, None, None)[0] == -1
+    assert err_of(lib.spdnn_topology_create, C.byref(top), -1, 4, 4, 0, None, None)[0] == -1
     cp = np.array([0, 1], np.int32)
-    rc, msg = err_of(lib.spdnn_topology_create, C.byref(top), -1, 4, 1, cp.ctypes.data, None)
+    rc, msg = err_of(lib.spdnn_topology_create, C.byref(top), -1, 4, 1, 0, cp.ctypes.data, None)
     assert rc == -1 and "row_idx" in msg
     assert lib.spdnn_topology_info(None, None, None, None, None, None) == -1
     assert lib.spdnn_topology_rows(None, None, 0) == -1
@@ -181,3 +181,16 @@ def test_microscaled_reference_of_the_tests():
     assert scales[:, 0].tolist() == [127, 0, 255, 0, 0] and scales[3, 1] == 126
     assert np.isnan(values[2, :32]).all() and values[2, 32] == 0 and values[3, 32] == 3.0 and codes[3, 1, 0] == 7
     assert codes[0, 0, 0] == 7 | 6 << 4 and codes[0, 0, 1] == (8 | 7) | 4 << 4
+
+
+def test_slots_are_the_width_that_was_asked_for():
+    """A table of rows keeps its width where no neuron uses all of it; CSC takes the longest, or what it is given."""
+    rows = np.array([[3, -1, 1], [2, -1, -1]])
+    top = SparseTopology.from_rows(rows, 4, device=None)
+    assert top.slots == 3 and np.array_equal(top.rows(), [[1, 3, -1], [2, -1, -1]])
+    assert np.array_equal(top.pack([5, 6, 7]), [[6, 5, 0], [7, 0, 0]])
+    csc = ([0, 2, 3], [3, 1, 2])
+    assert SparseTopology(4, 2, *csc, device=None).slots == 2 and SparseTopology(4, 2, *csc, device=None, slots=7).slots == 7
+    for bad in (1, -1, 4097):
+        with pytest.raises(SpDNNError, match="slots"):
+            SparseTopology(4, 2, *csc, device=None, slots=bad)

@@ -646,3 +646,15 @@ def test_offsets_beyond_32_bits(shared):
     assert torch.equal(q.codes[-3:], last.codes) and torch.equal(q.scales[-3:], last.scales) and not q.codes[:-3].any()
     values = q.dequantize(BF16)
     assert torch.equal(values[-3:], last.dequantize(BF16)) and not values[:-3].any()
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_weights_wider_than_any_neuron(tokens):
+    p = Problem(tokens, 90, 40, 12, BF16, 2, "random")
+    from graphchallenge21_b200 import SparseTopology
+    rows = p.rows_given.copy()
+    rows[:, -3:] = -1                                      # nine of twelve are used
+    p.top = SparseTopology.from_rows(rows, 90)
+    assert p.top.slots == 12
+    p.rows = p.top.rows()
+    check_step(p, "silu")
