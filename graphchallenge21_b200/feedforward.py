@@ -140,7 +140,8 @@ def mx4_quantize(x) -> MX4:
 
 
 class Saved:
-    """What a forward call with ``save=True`` keeps for its backward call: the pre-activations, float32 [sets, tokens, outputs]."""
+    """What a forward call with ``save=True`` keeps for its backward call: the pre-activations, float32 [sets, tokens, outputs]
+    without gaps (a backward call refuses any other type or layout)."""
 
     def __init__(self, z):
         self.z = z
@@ -267,6 +268,15 @@ class SparseTopology:
         ws = x.new_empty(size, dtype=_U8)
         return ws.data_ptr(), size, ws
 
+    def _pre_activations(self, saved, sets, tokens):
+        """The tensor of ``saved``, which the kernels read as float32 without gaps."""
+        z = getattr(saved, "z", None)
+        if z is None or z.shape != (sets, tokens, self.outputs) or z.get_device() != self.device:
+            raise SpDNNError(-1, "saved must be what the forward call returned")
+        if z.dtype is not _F32 or not z.is_contiguous():
+            raise SpDNNError(-1, "saved pre-activations must be contiguous float32, as the forward call returned them")
+        return z
+
     def _saved_operands(self, z, tokens):
         at, step = z.data_ptr(), tokens * self.outputs * 4
         return [_byref(_Operand(at + s * step, None, self.outputs, F32, 0)) for s in range(z.shape[0])]
@@ -305,9 +315,7 @@ class SparseTopology:
         tokens, kind, refs, x_type, w_type = self._begin(x, weights, activation)
         if x_type == MX4_TYPE:
             raise SpDNNError(-1, "microscaled activations have no backward pass")
-        z = getattr(saved, "z", None)
-        if z is None or z.shape != (len(weights), tokens, self.outputs) or z.get_device() != self.device:
-            raise SpDNNError(-1, "saved must be what the forward call returned")
+        z = self._pre_activations(saved, len(weights), tokens)
         dy_ref = _byref(_operand(dy, tokens, self.outputs, self.device, "dy"))
         dx = dx_ref = None
         if need_dx:
