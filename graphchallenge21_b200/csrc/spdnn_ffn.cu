@@ -1,5 +1,6 @@
 // C ABI of the feed-forward operators: topologies, sparse layers on row-major activations (plain and gated, forward and
-// backward) and microscaled 4-bit matrices.  Kernels: spdnn_ffn.cuh, spdnn_mx4.cuh; host analysis: topology.h.
+// backward) and microscaled 4-bit matrices.  Kernels: spdnn_ffn.cuh, spdnn_mx4.cuh; host analysis: topology.h; its tables on the GPU:
+// topology_device.h.
 //
 // A topology is immutable once created, and every call works on buffers of its caller (operands and workspace) on the caller's
 // stream, so calls on one topology may overlap, from several threads too.
@@ -16,7 +17,7 @@
 
 #include "spdnn_ffn.cuh"
 #include "spdnn_mx4.cuh"
-#include "topology.h"
+#include "topology_device.h"
 
 using namespace spdnn_impl;
 using namespace spdnn_impl::ffn;
@@ -26,19 +27,6 @@ static_assert((int)SPDNN_ACT_NONE == NONE && (int)SPDNN_ACT_RELU == RELU && (int
                   (int)SPDNN_ACT_GELU == GELU && (int)SPDNN_ACT_GELU_TANH == GELU_TANH, "activations of the header");
 
 namespace {
-
-struct DeviceTable {
-    uint32_t *slice_ptr = nullptr, *idx = nullptr, *src = nullptr;
-    int64_t entries = 0;
-    int outs = 0, rows = 0;
-};
-
-struct DeviceBlocks {
-    uint32_t *chunk_ptr = nullptr, *rows = nullptr, *src = nullptr, *chunk_block = nullptr;
-    int32_t *members = nullptr;
-    int blocks = 0;                 // 0: this direction has none
-    int64_t chunks = 0;
-};
 
 // How a gather runs: the image's unit (v tokens) and units per neuron (p), and how many blocks share a tile.
 struct GatherPlan {
@@ -50,14 +38,10 @@ struct GatherPlan {
 
 }  // namespace
 
-struct spdnn_topology {
+struct spdnn_topology : DeviceTopology {
     Topology host;
     int device = -1;                // -1: analysis only
     int sm_count = 0;
-    DeviceTable forward, backward;
-    DeviceBlocks forward_blocks, backward_blocks;
-    int32_t *rows = nullptr;        // canonical
-    void *few_rows = nullptr;       // canonical as few_kernel reads them
     // plans made so far: functions of the topology and the key, kept because a call may come every few microseconds
     mutable std::mutex plans_lock;
     mutable std::map<std::array<int, 5>, GatherPlan> plans;
@@ -118,59 +102,6 @@ struct OnDevice {
     }
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
-
-template <class T>
-cudaError_t upload(T **to, const std::vector<T> &from) {
-    cudaError_t e = cudaMalloc((void **)to, std::max<size_t>(from.size(), 1) * sizeof(T));
-    if (e != cudaSuccess) return e;
-    return cudaMemcpy(*to, from.data(), from.size() * sizeof(T), cudaMemcpyHostToDevice);
-}
-
-cudaError_t upload(DeviceTable &d, const GatherTable &t) {
-    d.outs = t.outs; d.rows = t.rows; d.entries = (int64_t)t.idx.size();
-    cudaError_t e = upload(&d.slice_ptr, t.slice_ptr);
-    if (e == cudaSuccess) e = upload(&d.idx, t.idx);
-    if (e == cudaSuccess) e = upload(&d.src, t.src);
-    return e;
-}
-
-cudaError_t upload(DeviceBlocks &d, const BlockTable &t) {
-    if (!t.blocks) return cudaSuccess;
-    d.blocks = t.blocks; d.chunks = (int64_t)t.chunk_ptr.back();
-    cudaError_t e = upload(&d.chunk_ptr, t.chunk_ptr);
-    if (e == cudaSuccess) e = upload(&d.rows, t.rows);
-    if (e == cudaSuccess) e = upload(&d.src, t.src);
-    if (e == cudaSuccess) e = upload(&d.members, t.members);
-    if (e == cudaSuccess) e = upload(&d.chunk_block, t.chunk_block);
-    return e;
-}
-
-void release(DeviceBlocks &d) {
-    cudaFree(d.chunk_ptr); cudaFree(d.rows); cudaFree(d.src); cudaFree(d.members); cudaFree(d.chunk_block);
-    d = DeviceBlocks();
-}
-
-void release(DeviceTable &d) {
-    cudaFree(d.slice_ptr); cudaFree(d.idx); cudaFree(d.src);
-    d = DeviceTable();
-}
-
-int few_stride(int slots) { return (slots + 3) / 4 * 4; }
-
-template <class T>
-cudaError_t upload_few_rows(spdnn_topology &top, T **to) {
-    const int stride = few_stride(top.host.slots);
-    std::vector<T> rows((size_t)top.host.outputs * stride, (T)top.host.inputs);
-    for (int c = 0; c < top.host.outputs; ++c)
-        for (int k = 0; k < top.host.slots; ++k) {
-            const int32_t r = top.host.rows[(size_t)c * top.host.slots + k];
-            if (r >= 0) rows[(size_t)c * stride + k] = (T)r;
-        }
-    return upload(to, rows);
-}
-cudaError_t upload_few_rows(spdnn_topology &top) {
-    return top.host.inputs < 65536 ? upload_few_rows(top, (uint16_t **)&top.few_rows) : upload_few_rows(top, (int32_t **)&top.few_rows);
-}
 
 int type_size(int type) { return type == F32 ? 4 : 2; }
 bool is_float(int type) { return type == F32 || type == F16 || type == BF16; }
@@ -690,12 +621,7 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
         OnDevice guard(device);
         cudaError_t e = guard.status;
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&t->sm_count, cudaDevAttrMultiProcessorCount, device);
-        if (e == cudaSuccess) e = upload(t->forward, t->host.forward);
-        if (e == cudaSuccess) e = upload(t->backward, t->host.backward);
-        if (e == cudaSuccess) e = upload(t->forward_blocks, t->host.forward_blocks);
-        if (e == cudaSuccess) e = upload(t->backward_blocks, t->host.backward_blocks);
-        if (e == cudaSuccess) e = upload(&t->rows, t->host.rows);
-        if (e == cudaSuccess) e = upload_few_rows(*t);
+        if (e == cudaSuccess) e = upload(*t, t->host);
         t->device = device;
         if (e != cudaSuccess) {
             spdnn_topology_destroy(t);
@@ -721,12 +647,7 @@ extern "C" void spdnn_topology_destroy(spdnn_topology_t *top) {
     if (!top) return;
     if (top->device >= 0) {
         OnDevice guard(top->device);
-        release(top->forward);
-        release(top->backward);
-        release(top->forward_blocks);
-        release(top->backward_blocks);
-        cudaFree(top->rows);
-        cudaFree(top->few_rows);
+        release(*top);
     }
     delete top;
 }

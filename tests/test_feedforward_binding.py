@@ -1,8 +1,11 @@
 """CPU tests of what the binding of the feed-forward operators checks before a pointer reaches the library."""
+import os
+import subprocess
+
 import pytest
 
 from graphchallenge21_b200 import Saved, SparseTopology, SpDNNError
-from graphchallenge21_b200 import feedforward
+from graphchallenge21_b200 import build, feedforward
 
 torch = pytest.importorskip("torch")
 
@@ -32,3 +35,19 @@ def test_saved_pre_activations_of_another_type_or_layout_are_refused():
     for wrong in (None, Saved(z[:1]), Saved(torch.zeros(2, 5, 7)), Saved(torch.zeros(2, 4, 6))):
         with pytest.raises(SpDNNError, match="what the forward call returned"):
             top._pre_activations(wrong, 2, 5)
+
+
+@pytest.fixture(scope="module")
+def harness(tmp_path_factory):
+    """tests/topology_device_harness.cpp, built with the host compiler against the headers of the CUDA runtime."""
+    cxx, nvcc = build._host_cxx()[1:] or ["g++"], build._nvcc()
+    exe = str(tmp_path_factory.mktemp("harness") / "topology_device")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
+    subprocess.run([*cxx, "-std=c++17", "-O1", "-pthread", "-I", build.CSRC, "-I", include, "-o", exe,
+                    os.path.join(os.path.dirname(os.path.abspath(__file__)), "topology_device_harness.cpp")], check=True)
+    return lambda *args: subprocess.run([exe, *map(str, args)], check=True, capture_output=True, text=True, timeout=120).stdout.split()
+
+
+def test_a_topology_is_on_the_gpu_when_its_creation_returns(harness):
+    """Copies from pageable memory may return before they are done, and a call on another stream than theirs does not wait for them."""
+    assert harness("ordered") == ["0"]

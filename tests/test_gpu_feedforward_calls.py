@@ -17,3 +17,18 @@ def test_saved_pre_activations_of_another_type_or_layout_are_refused():
             p.backward(Saved(z), "silu")
     got = p.backward(Saved(saved.z.clone()), "silu")
     assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1] + got[2], want[1] + want[2]))
+
+
+@pytest.mark.parametrize("tokens", [1, 200])
+def test_the_first_call_comes_from_another_stream_at_once(tokens):
+    from graphchallenge21_b200 import SparseTopology
+    p = Problem(tokens, 4000, 5000, 48, BF16, 1)
+    want = p.forward("none")
+    torch.cuda.synchronize()
+    for _ in range(8):
+        top = SparseTopology.from_rows(p.rows_given, 4000)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            y = top.linear(p.x, p.w[0], p.b[0])
+            torch.cuda.current_stream().synchronize()
+        assert torch.equal(y, want)
+        top.close()
