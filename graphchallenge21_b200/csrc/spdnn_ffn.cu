@@ -622,11 +622,11 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
         cudaError_t e = guard.status;
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&t->sm_count, cudaDevAttrMultiProcessorCount, device);
         if (e == cudaSuccess) e = upload(*t, t->host);
-        t->device = device;
         if (e != cudaSuccess) {
-            spdnn_topology_destroy(t);
+            delete t;
             return fail_cuda(err, err_len, e);
         }
+        t->device = device;
         // the tables are on the device: only the canonical rows are asked for again
         t->host.forward = GatherTable();
         t->host.backward = GatherTable();

@@ -77,8 +77,17 @@ inline cudaError_t upload_few_rows(const Topology &host, T **to) {
     return upload(to, rows);
 }
 
-// On the current device.
-inline cudaError_t upload(DeviceTopology &d, const Topology &host) {
+inline void release(DeviceTopology &d) {
+    release(d.forward);
+    release(d.backward);
+    release(d.forward_blocks);
+    release(d.backward_blocks);
+    cudaFree(d.rows);
+    cudaFree(d.few_rows);
+    d = DeviceTopology();
+}
+
+inline cudaError_t upload_all(DeviceTopology &d, const Topology &host) {
     cudaError_t e = upload(d.forward, host.forward);
     if (e == cudaSuccess) e = upload(d.backward, host.backward);
     if (e == cudaSuccess) e = upload(d.forward_blocks, host.forward_blocks);
@@ -91,14 +100,17 @@ inline cudaError_t upload(DeviceTopology &d, const Topology &host) {
     return e;
 }
 
-inline void release(DeviceTopology &d) {
-    release(d.forward);
-    release(d.backward);
-    release(d.forward_blocks);
-    release(d.backward_blocks);
-    cudaFree(d.rows);
-    cudaFree(d.few_rows);
-    d = DeviceTopology();
+// On the current device.  What fails, with a status or an exception, leaves nothing behind.
+inline cudaError_t upload(DeviceTopology &d, const Topology &host) {
+    cudaError_t e;
+    try {
+        e = upload_all(d, host);
+    } catch (...) {
+        release(d);
+        throw;
+    }
+    if (e != cudaSuccess) release(d);
+    return e;
 }
 
 }  // namespace spdnn_impl

@@ -51,3 +51,11 @@ def harness(tmp_path_factory):
 def test_a_topology_is_on_the_gpu_when_its_creation_returns(harness):
     """Copies from pageable memory may return before they are done, and a call on another stream than theirs does not wait for them."""
     assert harness("ordered") == ["0"]
+
+
+def test_a_topology_that_cannot_be_created_leaves_no_device_memory(harness):
+    device, host = map(int, harness("calls"))
+    assert device == 18 and host >= 1
+    for where, times in (("device", device), ("host", host)):
+        for n in range(1, times + 1):
+            assert harness(where, n) == ["1", "0"], (where, n)
