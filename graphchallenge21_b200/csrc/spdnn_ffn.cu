@@ -234,7 +234,7 @@ cudaError_t launch_blocks(const spdnn_topology &top, const GatherPlan &g, const 
     BlockArgs k{};
     k.image = a.image; k.image_bytes = g.image_bytes; k.chunk_ptr = b.chunk_ptr; k.rows = b.rows; k.members = b.members; k.weights = a.weights;
     k.chunks = b.chunks; k.blocks = b.blocks; k.tokens = a.tokens; k.bias0 = a.bias0; k.bias1 = a.bias1;
-    k.y = a.y; k.z0 = a.z0; k.z1 = a.z1; k.y_stride = a.y_stride; k.z_stride = a.z_stride; k.y_type = a.y_type; k.act = a.act; k.clip = a.clip;
+    k.y = a.y; k.z0 = a.z0; k.z1 = a.z1; k.y_stride = a.y_stride; k.z_stride = a.z_stride; k.y_type = a.y_type; k.act = a.act; k.clip = a.clip; k.scale = a.scale;
     k.whole_y = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * type_size(a.y_type) % 16 == 0;
     k.whole_z = (reinterpret_cast<uintptr_t>(a.z0) | reinterpret_cast<uintptr_t>(a.z1)) % 16 == 0 && a.z_stride % 4 == 0;
     const auto of = [&](auto e) {
@@ -303,7 +303,7 @@ const char *check_types(int x_type, int w_type, bool backward) {
 }
 
 struct Workspace {
-    int64_t weights = 0, index = 0, image = 0, x_columns = 0, d_columns = 0, total = 0;
+    int64_t weights = 0, index = 0, image = 0, x_columns = 0, d_columns = 0, scale = 0, total = 0;
 };
 
 // Layout of a call's workspace.  The plan is a function of the topology, the device and the arguments.
@@ -318,6 +318,7 @@ Workspace layout(const spdnn_topology &top, const GatherPlan &g, const DeviceTab
         const int64_t stride = (tokens + 63) / 64 * 64;
         w.x_columns = at; at += aligned(stride * top.host.inputs * type_size(image));
         w.d_columns = at; at += aligned(stride * top.host.outputs * sets * 4);
+        w.scale = at; at += image == F16 ? aligned(stride * 4) : 0;
     }
     w.total = std::max<int64_t>(at, 256);
     return w;
@@ -495,6 +496,9 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     return SPDNN_OK;
 }
 
+// Whether dL/dz of fp16 operands may leave fp16's range or be rounded: not where it is dy or zero.
+bool needs_scale(const Call &c) { return c.x->type == F16 && (c.sets == 2 || (c.act != NONE && c.act != RELU && c.act != CLIP)); }
+
 struct Gradients {
     const spdnn_operand_t *dy, *dx;
     float *dw[2], *db[2];
@@ -576,16 +580,21 @@ int run_backward(const Call &c, const Gradients &d) {
         p.image = d.dx ? base + ws.image : nullptr; p.image_bytes = g.image_bytes;
         p.columns = d.dw[0] ? base + ws.d_columns : nullptr; p.token_stride = stride;
         prep.main_blocks = p.image || p.columns ? pack_blocks(p) : 0;
+        if (p.image && needs_scale(c)) {
+            e = launch(c.sets == 2 ? token_scale_kernel<2> : token_scale_kernel<1>, (unsigned)stride, kScaleThreads, c.stream, p, (float *)(base + ws.scale));
+            p.scale = (const float *)(base + ws.scale);
+        }
         PackArgs &x = prep.x;
         x.x = matrix(c.x); x.rows = h.inputs; x.tokens = c.tokens; x.v = x.p = 1; x.vector = on_16_bytes(c.x); x.same = x.vector;
         x.columns = base + ws.x_columns; x.token_stride = stride;
-        e = launch_prepare(prep, d.dw[0] ? pack_blocks(x) : 0, c.sets, true, type, type, c.stream);
+        if (e == cudaSuccess) e = launch_prepare(prep, d.dw[0] ? pack_blocks(x) : 0, c.sets, true, type, type, c.stream);
     }
     if (c.tokens > 0 && d.dx && e == cudaSuccess) {
         GatherArgs a{};
         a.image = base + ws.image; a.slice_ptr = t.slice_ptr; a.index = base + ws.index;
         a.weights = base + ws.weights; a.outs = t.outs; a.tokens = c.tokens;
         a.y = const_cast<void *>(d.dx->data); a.y_stride = d.dx->stride; a.y_type = type;
+        if (needs_scale(c)) a.scale = (const float *)(base + ws.scale);
         e = g.blocks ? launch_blocks(*c.top, g, c.top->backward_blocks, a, type, c.sets, 1, c.stream) : launch_gather(g, a, type, type, c.sets, 1, c.stream);
     }
     if (d.dw[0] && e == cudaSuccess) {

@@ -15,7 +15,8 @@
 //
 // Roundings: all sums, the pre-activations kept for the backward pass and the d that the weights' gradients are made of are in 32 bits.  The
 // d that dx gathers is rounded to the activations' type: a gathered value costs what it is wide, in shared memory and in tokens per
-// image, and the error (half a step of every term) is that of rounding dx itself.
+// image, and the error is half a step of every term.  fp16 does not hold d's range (a product of two or three factors of the operands' order), so a
+// token's d are gathered at a power of two of their own (token_scale_kernel), which the sums are divided by again.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -312,6 +313,7 @@ struct PackArgs {
     int64_t image_bytes;
     void *columns;         // [rows][sets][token_stride], or nullptr: what dw_kernel reads (gradients as float)
     int64_t token_stride;
+    const float *scale;    // [token_stride] what a token's values in the image are multiplied by, or nullptr: see token_scale_kernel
     int rows, tokens;
     int v, p;              // the image's unit and units per neuron (powers of two)
     int vector;            // every row of every operand begins on 16 bytes
@@ -350,16 +352,14 @@ __device__ __forceinline__ void load_row_part(const Matrix &x, bool vector, int6
             }
             return;
         }
-        if constexpr (COUNT == 8) {
-            const uint4 r = __ldg((const uint4 *)((const uint16_t *)x.data + row * x.stride + col));
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        Raw<bf16, COUNT> r;
+        r.load((const uint16_t *)x.data + row * x.stride + col);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const f32x2 two = x.type == F16 ? widen<__half>(w[k]) : widen<bf16>(w[k]);
-                unpack2(two, v[2 * k], v[2 * k + 1]);
-            }
-            return;
+        for (int k = 0; k < COUNT / 2; ++k) {
+            const f32x2 two = x.type == F16 ? widen<__half>(r.w[k]) : widen<bf16>(r.w[k]);
+            unpack2(two, v[2 * k], v[2 * k + 1]);
         }
+        return;
     }
 #pragma unroll
     for (int k = 0; k < COUNT; ++k) v[k] = col + k < cols ? load_as_float(x.data, x.type, row * x.stride + col + k) : 0.0f;
@@ -375,19 +375,24 @@ template <class E> __device__ __forceinline__ uint32_t pair_bits(float lo, float
     }
 }
 
-// COUNT neighbours of the tile (on their natural alignment) as values of type E, in words; one 16-bit value: in the low half.
-template <class E, int COUNT, class Tile> __device__ __forceinline__ void tile_words(const Tile *p, uint32_t *w) {
+// COUNT neighbours of the tile (on their natural alignment) as values of type E, in words; one 16-bit value: in the low half.  scale: of these
+// tokens, or nullptr (a tile of gradients in fp16 only).
+template <class E, int COUNT, class Tile> __device__ __forceinline__ void tile_words(const Tile *p, uint32_t *w, const float *scale) {
     if constexpr (sizeof(Tile) == sizeof(E)) {
         Raw<E, COUNT> r;
         r.load(p);
 #pragma unroll
         for (int i = 0; i < (COUNT * (int)sizeof(E) + 3) / 4; ++i) w[i] = r.w[i];
     } else if constexpr (COUNT == 1) {
-        w[0] = pair_bits<E>(*p, 0.0f);
+        w[0] = pair_bits<E>(std::is_same<E, __half>::value && scale ? *p * __ldg(scale) : *p, 0.0f);
     } else {
 #pragma unroll
         for (int i = 0; i < COUNT; i += 2) {
-            const float2 v = *(const float2 *)(p + i);
+            float2 v = *(const float2 *)(p + i);
+            if (std::is_same<E, __half>::value && scale) {
+                const float2 f = __ldg((const float2 *)(scale + i));
+                v.x *= f.x; v.y *= f.y;
+            }
             w[i / 2] = pair_bits<E>(v.x, v.y);
         }
     }
@@ -397,7 +402,7 @@ template <class E, int COUNT, class Tile> __device__ __forceinline__ void tile_w
 // 64 neurons before n0 take.)
 template <class E, int SETS, int V, class Tile, class At>
 __device__ __forceinline__ void small_units(char *image, int64_t image_bytes, int parts, const Tile &tile, const At &at, int n0, int n_end,
-                                            uint32_t units, int rows) {
+                                            uint32_t units, int rows, const float *scale) {
     constexpr int N = 16 / (int)sizeof(E), PIECES = N / V;
     const int first = (int)((uint32_t)n0 * SETS * V / N);
     const int here = (int)(min((uint32_t)(n0 + n_end) * SETS, units) * V / N) - first;
@@ -409,7 +414,7 @@ __device__ __forceinline__ void small_units(char *image, int64_t image_bytes, in
         for (int k = 0; k < PIECES; ++k) {
             const int q = g * PIECES + k, n = q / SETS, s = q % SETS;
             uint32_t v[2] = {0, 0};
-            if (n < 64 && n0 + n < rows) tile_words<E, V>(&tile[s][n][at(n, part * V)], v);
+            if (n < 64 && n0 + n < rows) tile_words<E, V>(&tile[s][n][at(n, part * V)], v, scale ? scale + part * V : nullptr);
             constexpr int WORDS = V * (int)sizeof(E) / 4;
             if constexpr (WORDS == 0) w[k / 2] |= v[0] << (16 * (k & 1)) & (k & 1 ? 0xffff0000u : 0xffffu);
             else
@@ -418,6 +423,31 @@ __device__ __forceinline__ void small_units(char *image, int64_t image_bytes, in
         }
         ((uint4 *)(image + part * image_bytes))[first + g] = make_uint4(w[0], w[1], w[2], w[3]);
     }
+}
+
+// dL/dz of N neurons of a token, from neuron `col` on; zeros behind the last.
+template <class E, int SETS, int N>
+__device__ __forceinline__ void gradient_part(const PackArgs &a, int64_t row, int col, float (&d0)[N], float (&d1)[N]) {
+    float g[N], u[N], dy[N];
+    load_row_part<N>(a.x, a.vector, row, col, a.rows, d0);
+#pragma unroll
+    for (int k = 0; k < N; ++k) dy[k] = d0[k];
+    const bool saved = SETS == 2 || a.act != NONE;
+    if (saved) load_row_part<N>(Matrix{a.z0, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, g);
+    if (SETS == 2) load_row_part<N>(Matrix{a.z1, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, u);
+    if (SETS == 2) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) { d1[k] = d0[k] * g[k]; u[k] *= d0[k]; d0[k] = u[k]; }       // NONE
+    }
+    with_activation(a.act, [&](auto act) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float value, slope;
+            activate_both<sizeof(E) == 2>(g[k], act.value, a.clip, value, slope);
+            if (SETS == 2) d1[k] = dy[k] * value;
+            d0[k] *= slope;
+        }
+    });
 }
 
 // One block: 64 neurons x 64 tokens, through shared memory so that reads run along neurons and writes along tokens.  The tokens of a
@@ -474,30 +504,8 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
 #pragma unroll
         for (int k = 0; k < N; ++k) d0[k] = d1[k] = 0.0f;
         if (t0 + t < a.tokens && n0 + n < a.rows) {
-            const int64_t row = t0 + t;
-            const int col = n0 + n;
-            load_row_part<N>(a.x, a.vector, row, col, a.rows, d0);
-            if constexpr (GRADIENT) {
-                float g[N], u[N], dy[N];
-#pragma unroll
-                for (int k = 0; k < N; ++k) dy[k] = d0[k];
-                const bool saved = SETS == 2 || a.act != NONE;
-                if (saved) load_row_part<N>(Matrix{a.z0, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, g);
-                if (SETS == 2) load_row_part<N>(Matrix{a.z1, nullptr, a.z_stride, F32}, a.vector, row, col, a.rows, u);
-                if (SETS == 2) {
-#pragma unroll
-                    for (int k = 0; k < N; ++k) { d1[k] = d0[k] * g[k]; u[k] *= d0[k]; d0[k] = u[k]; }       // NONE
-                }
-                with_activation(a.act, [&](auto act) {
-#pragma unroll
-                    for (int k = 0; k < N; ++k) {
-                        float value, slope;
-                        activate_both<sizeof(E) == 2>(g[k], act.value, a.clip, value, slope);
-                        if (SETS == 2) d1[k] = dy[k] * value;
-                        d0[k] *= slope;
-                    }
-                });
-            }
+            if constexpr (GRADIENT) gradient_part<E, SETS, N>(a, t0 + t, n0 + n, d0, d1);
+            else load_row_part<N>(a.x, a.vector, t0 + t, n0 + n, a.rows, d0);
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -507,6 +515,7 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
     }
     __syncthreads();
     if (a.image) {
+        const float *scale = GRADIENT && a.scale ? a.scale + t0 : nullptr;
         const int log_p = 31 - __clz(a.p), T = a.v * a.p, per_row = a.p * SETS;
         const uint32_t units = image_units(a.rows, per_row);
         const int64_t tiles = ((int64_t)a.tokens + T - 1) / T;
@@ -524,10 +533,10 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
                 uint32_t w[4] = {0, 0, 0, 0};
                 if (n < 64 && n0 + n < a.rows) {
                     if constexpr (sizeof(Tile) == sizeof(E)) {
-                        tile_words<E, N>(&tile[s][n][at(n, t)], w);
+                        tile_words<E, N>(&tile[s][n][at(n, t)], w, nullptr);
                     } else {
-                        tile_words<E, 4>(&tile[s][n][at(n, t)], w);
-                        tile_words<E, 4>(&tile[s][n][at(n, t + 4)], w + 2);
+                        tile_words<E, 4>(&tile[s][n][at(n, t)], w, scale ? scale + t : nullptr);
+                        tile_words<E, 4>(&tile[s][n][at(n, t + 4)], w + 2, scale ? scale + t + 4 : nullptr);
                     }
                 }
                 const uint4 r = make_uint4(w[0], w[1], w[2], w[3]);
@@ -535,9 +544,9 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
             }
         } else {
             char *image = (char *)a.image + tile0 * a.image_bytes;
-            if (a.v == 1) small_units<E, SETS, 1>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
-            else if (a.v == 2) small_units<E, SETS, 2>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
-            else small_units<E, SETS, (N > 4 ? 4 : 2)>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows);
+            if (a.v == 1) small_units<E, SETS, 1>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows, scale);
+            else if (a.v == 2) small_units<E, SETS, 2>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows, scale);
+            else small_units<E, SETS, (N > 4 ? 4 : 2)>(image, a.image_bytes, parts, tile, at, n0, n_end, units, a.rows, scale);
         }
     }
     if (a.columns) {
@@ -552,6 +561,41 @@ __device__ __forceinline__ void pack_block(const PackArgs &a, unsigned block, un
         }
     }
 }
+
+constexpr int kScaleThreads = 512;
+
+// The power of two that brings the largest finite |d| of a token into [2^14, 2^15): what fp16 holds of it is off by half a step, or by 2^-39 of the
+// largest where that is more.  2^126 at most, whose reciprocal is a normal number.  One block per token; bringing in what the image is made of, once
+// more, is what bounds it (1024 tokens x 16384, both sets: 39 us for 168 MB with four neurons a lane, 43 with eight; 97 tokens: 12 us with 512 threads, 16 with
+// 256).
+template <int SETS>
+__global__ void __launch_bounds__(kScaleThreads) token_scale_kernel(const __grid_constant__ PackArgs a, float *scales) {
+    __shared__ uint32_t tops[kScaleThreads / 32];
+    const int t = gridDim.x - 1 - blockIdx.x;         // the tokens that prepare_kernel begins with come last, and are still in L2 then
+    uint32_t top = 0;           // bits of magnitudes are ordered as they are
+    if (t < a.tokens)
+        for (int col = threadIdx.x * 4; col < a.rows; col += kScaleThreads * 4) {
+            float d[2][4];
+            gradient_part<__half, SETS, 4>(a, t, col, d[0], d[1]);
+#pragma unroll
+            for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t m = __float_as_uint(d[s][k]) & 0x7fffffffu;
+                    top = max(top, m < 0x7f800000u ? m : 0u);
+                }
+        }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int w = 1; w < kScaleThreads / 32; ++w) top = max(top, tops[w]);
+    scales[t] = __uint_as_float((127 + 14 + 127 - max(top >> 23, 15u)) << 23);
+}
+
+// 1 / a power of two between 2^-126 and 2^126
+__device__ __forceinline__ float reciprocal(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
 
 struct OrderArgs {
     Matrix w0, w1;
@@ -674,6 +718,7 @@ struct GatherArgs {
     int y_type;
     int act;
     float clip;
+    const float *scale;         // of the image's tokens (PackArgs), or nullptr; fp16 only
 };
 
 // Units a lane reads per gathered value, and threads per block.  Two units halve what index, weights and the loop cost per fma; with more sums
@@ -750,6 +795,13 @@ __global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_
     uint32_t q0 = 0, q1 = 0;
     if (unit < last) { q0 = __ldg(a.slice_ptr + unit / L); q1 = __ldg(a.slice_ptr + unit / L + 1); }
     const auto in_slice = [&](int64_t u) { return (int)(u % L) * (32 / L) + lane / L; };
+    // The tokens of a lane are the same in every unit; where they are many, their factors would take its registers.  Two sets always have factors.
+    constexpr bool SCALED = std::is_same<E, __half>::value && std::is_same<W, __half>::value && G == 1, KEPT = SCALED && S == 2 && NV * V <= 4;
+    const auto factor = [&](int k) { return reciprocal(__ldg(a.scale + (int64_t)tile * (V * P) + j * V + k / V * (L * V) + k % V)); };
+    float kept[KEPT ? NV * V : 1];
+    if (KEPT)
+#pragma unroll
+        for (int k = 0; k < NV * V; ++k) kept[k] = factor(k);
     Quad<W, SETS, GLOBAL> cur, ahead;
     if (q0 < q1) cur.load(a, (size_t)q0 * 32 + in_slice(unit));
     if constexpr (!GLOBAL) copy_in(smem, image, (uint32_t)a.image_bytes);
@@ -816,6 +868,9 @@ __global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_
             }
             const int64_t t0 = (int64_t)tile * (V * P) + j * V;
             // token k of the lane is t0 + (k / V) L V + k % V
+            if (SCALED && (S == 2 || a.scale))
+#pragma unroll
+                for (int k = 0; k < NV * V; ++k) acc[0][k] *= KEPT ? kept[KEPT ? k : 0] : factor(k);
             const auto store = [&](auto *to, int64_t stride, const auto &value) {
                 to += t0 * stride + c;
                 const int left = (int)min((int64_t)(P * V), (int64_t)a.tokens - t0);
@@ -1137,6 +1192,7 @@ struct BlockArgs {
     int64_t y_stride, z_stride;
     int y_type, act;
     float clip;
+    const float *scale;          // of the image's tokens (PackArgs), or nullptr; fp16 only
     int whole_y, whole_z;        // rows of y, of z begin on 16 bytes: blocks of 16 neighbours are stored in whole sectors
 };
 
@@ -1298,6 +1354,15 @@ __global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_co
                     if (G == 2) acc[m][2 * G - 2 + half][i] += b1[i & 1];
                 }
         }
+        if (std::is_same<E, __half>::value && G == 1 && a.scale)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float f = reciprocal(__ldg(a.scale + tile0 + m * 16 + i * 8 + lane / 4));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) { acc[m][half][2 * i] *= f; acc[m][half][2 * i + 1] *= f; }
+                }
         const auto store = [&](auto *to, int64_t stride, bool whole, const auto &value) {
             using T = typename std::remove_pointer<decltype(to)>::type;
             to += tile0 * stride;

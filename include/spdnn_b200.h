@@ -283,7 +283,8 @@ int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *
 /* Gradients from dy = dL/dy and what the forward call read and saved; dy, x, w and dx have one float type.  dx
  * [tokens][inputs] or NULL; dw, dbias in fp32 ([outputs][slots] without gaps, [outputs]), overwritten, or NULL (dbias only with dw).
  * z may be NULL for SPDNN_ACT_NONE (linear).  The slope of RELU at 0 is 0, of CLIP at 0 and clip too.  On its way to
- * dx (not to dw and dbias) dL/dz is rounded to the operands' type.  Every sum has a fixed order: the same call gives the same bits. */
+ * dx (not to dw and dbias) dL/dz is rounded to the operands' type; in fp16 after a token's values were multiplied by the power of two that brings the
+ * largest into [2^14, 2^15) (the sums are divided by it), so that they keep half a step, or 2^-39 of the token's largest.  Every sum has a fixed order: the same call gives the same bits. */
 int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
                           const spdnn_operand_t *w, const spdnn_operand_t *z, int activation, float clip, const spdnn_operand_t *dx,
                           float *dw, float *dbias, void *workspace, int64_t workspace_bytes, void *cuda_stream, char *err,

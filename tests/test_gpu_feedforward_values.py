@@ -1,0 +1,95 @@
+"""GPU tests of the feed-forward operators where values leave the ordinary: gradients beyond fp16's range, infinities, activations far
+from zero.  References and the meaning of U and half_step: tests/feedforward_reference.py."""
+import numpy as np
+import pytest
+
+import feedforward_reference as ref
+from test_gpu_feedforward import BF16, F16, F32, Problem, Shared, check, torch
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- dL/dz on its way to dx in fp16 ---------------------------------------------------------------
+
+def scaled_dx(f, dy):
+    """dx and its bound where the gathered dL/dz of a token are held in fp16 at a power of two of their own: a value is off by half
+    a step, or by half the smallest subnormal at that scale, where the token's largest value lies in [2^14, 2^15): 2^-25 2^-14 of it (twice
+    that where the kernel's largest value is below a power of two and the exact one is not)."""
+    h, u = ref.half_step(F16), ref.U
+    dyd = dy.double()
+    off = [e + u * z.abs() for z, e in zip(f.z, f.dz)]
+    s, ds = ref.slope(f.z[0], f.kind, f.clip), 0.85 * off[0] + 32 * u * (1 + f.z[0].abs())
+    if f.kind in ("none", "relu", "clip"):
+        ds = ref.corners(f.z[0], f.dz[0], f.kind, f.clip)
+    if len(f.ws) == 1:
+        d, dd = [dyd * s], [dyd.abs() * ds]
+    else:
+        a, da = ref.act(f.z[0], f.kind, f.clip), 1.13 * off[0] + 16 * u * f.z[0].abs()
+        d = [dyd * s * f.z[1], dyd * a]
+        dd = [dyd.abs() * (ds * (f.z[1].abs() + off[1]) + s.abs() * off[1]), dyd.abs() * da]
+    top = torch.stack([v.abs() for v in d]).nan_to_num(0, 0, 0).amax((0, 2))
+    rows = torch.as_tensor(f.rows, device=dy.device).long()
+    fan = int(torch.bincount(rows[rows >= 0]).max())
+    dx, bound = torch.zeros(dy.shape[0], f.inputs, dtype=torch.float64, device=dy.device), 0
+    for v, e, w in zip(d, dd, f.ws):
+        W, A = ref.dense(f.rows, w, f.inputs), ref.dense(f.rows, w.double().abs(), f.inputs)
+        es = (e + 4 * u * v.abs()) * (1 + h) + h * v.abs() + 2.0 ** -38 * top[:, None]
+        dx = dx + v @ W.t()
+        bound = bound + es @ A.t() + (fan * len(f.ws) + 2) * u * ((v.abs() + es) @ A.t())
+    return dx, bound * (1 + h) + ref.stored(dx, F16), d
+
+
+@pytest.mark.parametrize("kind, sets", [("silu", 2), ("gelu", 2), ("relu", 2), ("none", 2), ("gelu_tanh", 1), ("clip", 1)])
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("tokens", [1, 6, 40, 200])
+def test_fp16_gradients_beyond_the_types_range(tokens, shared, kind, sets):
+    """dL/dz above 65504 and below 2^-24 where dx itself is well inside: both by the token."""
+    p = Shared(tokens, 256, 320, 32, F16, sets, 16, False) if shared else Problem(tokens, 256, 320, 16, F16, sets, "ragged")
+    # small weights and large activations: pre-activations of order 30, gradients of order 3000 of most tokens ...
+    p.w = [(0.01 * w.float()).to(F16) for w in p.w]
+    p.x = (3000 * p.x.float()).clamp(-6e4, 6e4).to(F16)
+    p.dy = (3000 * p.dy.float()).to(F16)
+    # ... and tiny ones of every third, whose dL/dz are subnormal or gone in fp16
+    p.dy[2::3] = (p.dy[2::3].float() * 2.0 ** -36).to(F16)
+    y, saved = p.forward(kind, save=True)
+    f = p.reference(kind)
+    dx, dw, db = p.backward(saved, kind)
+    want, bound, d = scaled_dx(f, p.dy)
+    assert want.abs().max() < 6e4
+    if sets == 2:
+        assert max(float(v.abs().max()) for v in d) > 65504
+    check(dx, want, bound, "dx")
+    assert all(torch.isfinite(t).all() for t in dw + db)
+    only = p.backward(saved, kind, need_dw=False)[0]
+    assert torch.equal(only, dx)
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("sets", [1, 2])
+def test_fp16_small_gradients_meet_large_weights(sets, shared):
+    """dL/dz around fp16's smallest numbers, weights of order 100: what dx loses is half a step of a term, not of the subnormals."""
+    p = Shared(70, 256, 320, 32, F16, sets, 16, True) if shared else Problem(70, 300, 200, 16, F16, sets)
+    p.w = [(100 * w.float()).to(F16) for w in p.w]
+    p.x = (0.01 * p.x.float()).to(F16)
+    p.dy = (2.0 ** -22 * p.dy.float()).to(F16)
+    y, saved = p.forward("silu", save=True)
+    want, bound, d = scaled_dx(p.reference("silu"), p.dy)
+    check(p.backward(saved, "silu")[0], want, bound, "dx")
+
+
+@pytest.mark.parametrize("tokens", [5, 90])
+def test_fp16_infinite_gradients_stay_with_their_connections(tokens):
+    p = Problem(tokens, 256, 320, 16, F16, 2)
+    y, saved = p.forward("silu", save=True)
+    f = p.reference("silu")
+    want, bound, _ = scaled_dx(f, p.dy)
+    clean = p.backward(saved, "silu")[0]
+    check(clean, want, bound, "dx")
+    p.dy[3, 11], p.dy[4, 200] = float("inf"), float("nan")
+    dx = p.backward(saved, "silu")[0]
+    touched = torch.zeros_like(dx, dtype=torch.bool)
+    touched[3, torch.as_tensor(p.rows[11]).cuda().long()] = True
+    touched[4, torch.as_tensor(p.rows[200]).cuda().long()] = True
+    assert not torch.isfinite(dx[touched]).any()
+    # what else these two tokens hold is scaled by their largest finite value, which may have been one of the two
+    check(dx[~touched], want[~touched], (2 * bound)[~touched], "the others")
