@@ -316,7 +316,7 @@ Workspace layout(const spdnn_topology &top, const GatherPlan &g, const DeviceTab
     w.image = at; at += aligned(g.tiles * g.image_bytes);
     if (backward) {
         const int64_t stride = (tokens + 63) / 64 * 64;
-        w.x_columns = at; at += aligned(stride * top.host.inputs * type_size(image));
+        w.x_columns = at; at += aligned(stride * top.host.inputs * type_size(image) + 16);
         w.d_columns = at; at += aligned(stride * top.host.outputs * sets * 4);
         w.scale = at; at += image == F16 ? aligned(stride * 4) : 0;
     }
@@ -508,7 +508,7 @@ cudaError_t launch_dw(const Call &c, const Gradients &d, int type, const void *x
     const Topology &h = c.top->host;
     DwArgs a{};
     a.x = x_columns; a.d = d_columns; a.rows = c.top->rows; a.token_stride = stride;
-    a.outputs = h.outputs; a.slots = h.slots; a.chunks = (h.slots + kDwSlots - 1) / kDwSlots;
+    a.inputs = h.inputs; a.outputs = h.outputs; a.slots = h.slots; a.chunks = (h.slots + kDwSlots - 1) / kDwSlots;
     a.dw0 = d.dw[0]; a.dw1 = d.dw[1]; a.db0 = d.db[0]; a.db1 = d.db[1];
     const int per_block = kDwThreads / 32;
     const unsigned grid = (unsigned)(((int64_t)a.outputs * a.chunks + per_block - 1) / per_block);

@@ -311,7 +311,7 @@ struct PackArgs {
     int64_t z_stride;
     void *image;           // tiles of image_bytes each, or nullptr
     int64_t image_bytes;
-    void *columns;         // [rows][sets][token_stride], or nullptr: what dw_kernel reads (gradients as float)
+    void *columns;         // [rows][sets][token_stride], or nullptr: what dw_kernel reads (gradients as float; x followed by 16 bytes of zeros)
     int64_t token_stride;
     const float *scale;    // [token_stride] what a token's values in the image are multiplied by, or nullptr: see token_scale_kernel
     int rows, tokens;
@@ -699,7 +699,11 @@ __global__ void __launch_bounds__(kPackThreads) prepare_kernel(const __grid_cons
         if (!a.by_blocks) order_block<W, SETS>(a.order, blockIdx.x);
         else if constexpr (sizeof(W) == 2) order_blocks_block<W, SETS, GRADIENT>(a.blocks, blockIdx.x);
     } else if (blockIdx.x - a.order_blocks < a.main_blocks) pack_block<E, GRADIENT ? SETS : 1, GRADIENT>(a.main, blockIdx.x - a.order_blocks, shared);
-    else if (GRADIENT) pack_block<E, 1, false>(a.x, blockIdx.x - a.order_blocks - a.main_blocks, shared);
+    else if (GRADIENT) {
+        const unsigned block = blockIdx.x - a.order_blocks - a.main_blocks;
+        pack_block<E, 1, false>(a.x, block, shared);
+        if (block == 0 && threadIdx.x == 0) *(uint4 *)((E *)a.x.columns + a.x.rows * a.x.token_stride) = make_uint4(0, 0, 0, 0);
+    }
 }
 
 // ---- the gather ----------------------------------------------------------------------------------
@@ -1425,11 +1429,11 @@ __global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_co
 // ---- gradients of the weights ----------------------------------------------------------------------
 
 struct DwArgs {
-    const void *x;            // [inputs][token_stride]
+    const void *x;            // [inputs][token_stride], and 16 bytes of zeros
     const float *d;           // [outputs][sets][token_stride]
     const int32_t *rows;      // [outputs][slots] canonical, -1 = none
     int64_t token_stride;
-    int outputs, slots, chunks;   // chunks of kDwSlots connections per output
+    int inputs, outputs, slots, chunks;   // chunks of kDwSlots connections per output
     float *dw0, *dw1;         // [outputs][slots]
     float *db0, *db1;         // or nullptr
 };
@@ -1455,10 +1459,11 @@ template <int COUNT> __device__ __forceinline__ float sum_lanes(float (&v)[COUNT
 
 // A warp owns kDwSlots connections of one output: every lane sums its tokens' products in registers, the lanes are joined at the
 // end.  Adjacent warps take adjacent outputs, whose inputs are often the same rows (blocks of a butterfly).  What bounds it is bringing
-// the rows from L2, so the loads of several are in flight before the first is used.  A connection that is not there reads row 0 (or, in the
-// lanes behind the last token, any row's first tokens with a gradient of zero) and its sum is dropped.
+// the rows from L2, so the loads of several are in flight before the first is used.  A connection that is not there reads row 0 and its sum is
+// dropped.  Lanes behind the last token read zeros for both factors: an infinity of any other token would make NaN of a gradient of zero.  (They read
+// them behind x's columns; a load under a condition took 155 us instead of 125 at 1024 tokens, 16384 -> 16384, and a last step of its own 159.)
 template <class E, int G>
-__global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
+__global__ void __launch_bounds__(kDwThreads, G == 1 ? 7 : 4) dw_kernel(const DwArgs a) {
     constexpr int V = 16 / sizeof(E);
     constexpr int PAIRS = V / 2;
     constexpr int BATCH = 4;
@@ -1481,6 +1486,7 @@ __global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
     for (int64_t t0 = 0; t0 < a.token_stride; t0 += 32 * V) {
         const bool inside = t0 + lane * V < a.token_stride;
         const int64_t t = inside ? t0 + lane * V : 0;
+        const int least = inside ? 0 : a.inputs;
         f32x2 dv[G][PAIRS];
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -1496,7 +1502,7 @@ __global__ void __launch_bounds__(kDwThreads) dw_kernel(const DwArgs a) {
             Raw<E, V> raw[BATCH];
 #pragma unroll
             for (int k = 0; k < BATCH; ++k) {
-                const int row = max(__shfl_sync(0xffffffffu, mine, j + k), 0);
+                const int row = max(__shfl_sync(0xffffffffu, mine, j + k), least);
                 raw[k].load(x + (int64_t)row * a.token_stride + t);
             }
 #pragma unroll

@@ -93,3 +93,37 @@ def test_fp16_infinite_gradients_stay_with_their_connections(tokens):
     assert not torch.isfinite(dx[touched]).any()
     # what else these two tokens hold is scaled by their largest finite value, which may have been one of the two
     check(dx[~touched], want[~touched], (2 * bound)[~touched], "the others")
+
+
+# ---- infinities in gradients of weights --------------------------------------------------------------
+
+def check_with_infinities(got, want, bound, what):
+    odd = ~torch.isfinite(want)
+    assert odd.any()
+    assert torch.equal(got[odd].double().nan_to_num(7.0, posinf=5.0, neginf=3.0), want[odd].nan_to_num(7.0, posinf=5.0, neginf=3.0)), what
+    check(got[~odd], want[~odd], bound[~odd], what)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shared", [False])
+@pytest.mark.parametrize("tokens", [20, 63, 64, 100, 129, 300])
+def test_infinities_in_gradients_of_weights(tokens, shared, dtype):
+    """An infinite activation or gradient of one token gives infinities of the definition's sign, and NaN only where the definition
+    has 0 times infinity or a difference of two."""
+    p = Shared(tokens, 256, 320, 32, dtype, 1, 16, False) if shared else Problem(tokens, 256, 320, 16, dtype, 1, "ragged")
+    p.dy = torch.where(p.dy.float().abs() < 0.1, torch.ones_like(p.dy), p.dy)
+    p.dy[1, ::5] = 1.0                                   # few bits, and gradients of zero
+    p.dy[1, 4::5] = 0.0
+    p.x[1, 7], p.x[tokens - 1, 30] = float("inf"), -float("inf")
+    p.dy[2, 9], p.dy[12, 21] = -float("inf"), float("inf")
+    p.x[2, ::3] = 0.0
+    y, saved = p.forward("none", save=True)
+    dx, dw, db = p.backward(saved, "none")
+    rows = torch.as_tensor(p.rows).cuda().long()
+    xd, v, at = p.x.double(), p.dy.double(), rows.clamp(min=0)
+    want = torch.gather((xd.t() @ v).t(), 1, at).masked_fill(rows < 0, 0.0)
+    size = torch.gather((xd.abs().t() @ v.abs()).t(), 1, at).masked_fill(rows < 0, 0.0)
+    bound = (tokens + 8 + 4) * ref.U * size + 2.0 ** -140
+    assert (want == float("inf")).any() and (want == -float("inf")).any() and torch.isnan(want).any()
+    check_with_infinities(dw[0], want, bound, "dw")
+    check_with_infinities(db[0], v.sum(0), (tokens + 8) * ref.U * v.abs().sum(0), "db")
