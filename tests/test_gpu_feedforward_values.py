@@ -105,7 +105,7 @@ def check_with_infinities(got, want, bound, what):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("shared", [False])
+@pytest.mark.parametrize("shared", [False, True])
 @pytest.mark.parametrize("tokens", [20, 63, 64, 100, 129, 300])
 def test_infinities_in_gradients_of_weights(tokens, shared, dtype):
     """An infinite activation or gradient of one token gives infinities of the definition's sign, and NaN only where the definition
