@@ -1,5 +1,7 @@
 """GPU tests of the feed-forward operators where values leave the ordinary: gradients beyond fp16's range, infinities, activations far
 from zero.  References and the meaning of U and half_step: tests/feedforward_reference.py."""
+import math
+
 import numpy as np
 import pytest
 
@@ -127,3 +129,32 @@ def test_infinities_in_gradients_of_weights(tokens, shared, dtype):
     assert (want == float("inf")).any() and (want == -float("inf")).any() and torch.isnan(want).any()
     check_with_infinities(dw[0], want, bound, "dw")
     check_with_infinities(db[0], v.sum(0), (tokens + 8) * ref.U * v.abs().sum(0), "db")
+
+
+# ---- activations far from zero -----------------------------------------------------------------------
+
+def activation_of(values, dtype, kind, tokens, shared, out_dtype):
+    """The activation of `values` [tokens], through a layer whose first connection has the weight one and the others zero."""
+    from graphchallenge21_b200 import SparseTopology
+    n = 32
+    rows = np.tile(np.arange(n), (n, 1)) if shared else np.arange(n)[:, None]
+    top = SparseTopology.from_rows(rows, n)
+    x = torch.zeros(tokens, n, dtype=dtype, device="cuda")
+    x[:, 0] = values
+    w = torch.zeros(n, rows.shape[1], dtype=dtype, device="cuda")
+    w[:, 0] = 1.0
+    y, saved = top.linear(x, w, activation=kind, save=True, out_dtype=out_dtype)
+    assert torch.equal(saved.z[0, :, 0], values.float())
+    return top, x, w, y, saved
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens, shared", [(3, False), (700, False), (700, True)])
+def test_gelu_keeps_its_digits_far_below_zero(tokens, shared, dtype):
+    """v Phi(v) for v down to -12: a relative bound.  In the tail Phi is e^(-v^2 / 2) times what changes slowly: three roundings of the exponent
+    put it off by 1.5 v^2 u; the exponential and the reciprocal (4 u each), the polynomial and the products by less than 20 u."""
+    v = torch.linspace(-12, 4, tokens, device="cuda").to(dtype)
+    y = activation_of(v, dtype, "gelu", tokens, shared, F32)[3][:, 0]
+    z = v.double()
+    want = 0.5 * z * torch.erfc(-z * math.sqrt(0.5))         # (torch.special.ndtr(-12.0) is 0)
+    check(y, want, (2 * z * z + 4 * z.abs() + 20) * ref.U * want.abs() + 2.0 ** -140, "gelu")
