@@ -161,7 +161,8 @@ template <bool FAST> __device__ __forceinline__ void activate_both(float v, int 
         }
         case GELU_TANH: {
             const float s = sigmoid<FAST>(2.0f * kGeluA * (v + kGeluB * v * v * v));
-            value = v * s; slope = s + v * s * (1.0f - s) * 2.0f * kGeluA * (1.0f + 3.0f * kGeluB * v * v);
+            // where v^2 is infinite the factor before it is zero
+            value = v * s; slope = s + v * s * (1.0f - s) * 2.0f * kGeluA * (1.0f + 3.0f * kGeluB * fminf(v * v, 1e30f));
             return;
         }
         default: value = v; slope = 1.0f;

@@ -158,3 +158,18 @@ def test_gelu_keeps_its_digits_far_below_zero(tokens, shared, dtype):
     z = v.double()
     want = 0.5 * z * torch.erfc(-z * math.sqrt(0.5))         # (torch.special.ndtr(-12.0) is 0)
     check(y, want, (2 * z * z + 4 * z.abs() + 20) * ref.U * want.abs() + 2.0 ** -140, "gelu")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("shared", [False, True])
+def test_slopes_of_huge_pre_activations(kind, dtype, shared):
+    """1 above zero and 0 below, to the largest numbers there are."""
+    v = torch.tensor([1e5, 1e13, 1e18, 1.8e19, 2e19, 1e25, 1e30, 3e38], device="cuda").repeat(4)
+    v = torch.cat([v, -v]).to(dtype)
+    top, x, w, y, saved = activation_of(v, dtype, kind, 64, shared, None)
+    assert torch.equal(y[:, 0], v.clamp(min=0))
+    dx, dw, db = top.linear_backward(torch.ones_like(y), x, w, saved, activation=kind)
+    assert torch.isfinite(dx).all() and torch.isfinite(db).all()
+    reads = top.outputs if shared else 1
+    assert torch.equal(dx[:, 0], (v > 0).to(dtype) * reads)
