@@ -153,6 +153,28 @@ class Saved:
         return iter(self.z)
 
 
+def _whole(a, name):
+    """``a`` as an array of integers; floats only where they are whole numbers."""
+    a = np.asarray(a)
+    if a.dtype.kind not in "iufb":
+        raise SpDNNError(-1, f"{name} must hold integers")
+    if a.dtype.kind == "f":
+        with np.errstate(invalid="ignore"):
+            whole = a.astype(np.int64)
+        if not np.array_equal(whole, a):
+            raise SpDNNError(-1, f"{name} must hold integers")
+        return whole
+    return a
+
+
+def _int32(a, name):
+    """``a`` as contiguous int32, refused where a value does not fit (a cast would wrap around to another index)."""
+    a = _whole(a, name)
+    if a.dtype != np.int32 and a.size and not (a.min() >= -(1 << 31) and a.max() < 1 << 31):
+        raise SpDNNError(-1, f"{name} holds values beyond 32 bits")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 class SparseTopology:
     """The connections between ``inputs`` and ``outputs`` neurons, as CSC: output c is connected to inputs
     ``row_idx[col_ptr[c]:col_ptr[c + 1]]``.  ``slots``: columns of a weight matrix (0: as many as the output with most
@@ -162,8 +184,7 @@ class SparseTopology:
         self._top = C.c_void_p()
         self._lib = _lib.load()
         self._sizes = {}                 # workspaces: a function of these arguments and the topology
-        col_ptr = np.ascontiguousarray(col_ptr, dtype=np.int32)
-        row_idx = np.ascontiguousarray(row_idx, dtype=np.int32)
+        col_ptr, row_idx = _int32(col_ptr, "col_ptr"), _int32(row_idx, "row_idx")
         if col_ptr.shape != (outputs + 1,):
             raise SpDNNError(-1, f"col_ptr must have {outputs + 1} entries")
         if row_idx.ndim != 1 or row_idx.size != int(col_ptr[-1]):
@@ -181,7 +202,9 @@ class SparseTopology:
     def from_rows(cls, rows, inputs: int, device: int | None = 0):
         """``rows`` int [outputs, K]: the inputs of every output (entries < 0 are skipped), as ``SpDNN.set_layer_rows``; weight
         matrices are [outputs, K]."""
-        rows = np.asarray(rows)
+        rows = _whole(rows, "rows")
+        if rows.ndim != 2:
+            raise SpDNNError(-1, "rows must be a matrix [outputs, connections]")
         if rows.size and rows.min() >= 0:
             return cls(inputs, rows.shape[0], np.arange(rows.shape[0] + 1, dtype=np.int64) * rows.shape[1], rows.reshape(-1), device,
                        rows.shape[1])

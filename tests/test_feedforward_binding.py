@@ -2,6 +2,7 @@
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 from graphchallenge21_b200 import Saved, SparseTopology, SpDNNError
@@ -59,3 +60,24 @@ def test_a_topology_that_cannot_be_created_leaves_no_device_memory(harness):
     for where, times in (("device", device), ("host", host)):
         for n in range(1, times + 1):
             assert harness(where, n) == ["1", "0"], (where, n)
+
+
+@pytest.mark.parametrize("rows", [[2 ** 32 + 3], [2 ** 31], [-2 ** 32 + 1], [3.9], [float("nan")], [float("inf")], [2.0 ** 40], [2 ** 64], [1j],
+                                  np.array([2 ** 63 + 1], dtype=np.uint64)])
+def test_indices_that_are_not_32_bit_integers_are_refused(rows):
+    """A cast would make another index of them that the library cannot tell from the one that was meant."""
+    with pytest.raises(SpDNNError, match="row_idx"):
+        SparseTopology(8, 1, [0, 1], rows, device=None)
+    with pytest.raises(SpDNNError, match="col_ptr"):
+        SparseTopology(8, 1, [0, rows[0]], [0], device=None)
+
+
+def test_rows_that_are_not_a_matrix_of_indices_are_refused():
+    for rows, says in (([[2 ** 32 + 3]], "beyond 32 bits"), ([[3.9]], "integers"), ([[float("nan"), 1]], "integers"), ([[-0.5, 1]], "integers"),
+                       ([3, 4], "matrix"), (3, "matrix")):
+        with pytest.raises(SpDNNError, match=says):
+            SparseTopology.from_rows(rows, 8, device=None)
+    # whole numbers of other types, and any negative number for a connection that is not there, are what they were
+    for t in (np.int8, np.uint16, np.int64, np.float32):
+        assert SparseTopology.from_rows(np.array([[3, 1]], dtype=t), 8, device=None).rows().tolist() == [[1, 3]]
+    assert SparseTopology.from_rows([[3, -2 ** 40], [1, -1]], 8, device=None).rows().tolist() == [[3, -1], [1, -1]]
