@@ -38,6 +38,7 @@ def _torch():
     return torch
 
 
+MAX_TOKENS, MAX_COLUMNS = 1 << 26, 1 << 30      # of one call; of a microscaled matrix: checked here, where they are not yet C ints
 _Error = C.c_char * _ERR_LEN
 
 
@@ -63,6 +64,8 @@ class MX4:
         if not _TYPES:
             _torch()
         cols = int(cols)
+        if cols > MAX_COLUMNS:
+            raise SpDNNError(-1, f"a matrix has at most {MAX_COLUMNS} columns")
         blocks = (cols + 31) // 32
         shape = codes.shape
         if len(shape) != 3 or shape[1] != blocks or shape[2] != 16 or scales.shape != shape[:2] or cols < 1 or not (
@@ -128,6 +131,8 @@ def mx4_quantize(x) -> MX4:
     if not hasattr(x, "is_cuda") or x.dim() != 2 or x.shape[1] < 1:
         raise SpDNNError(-1, "x must be a matrix with at least one column")
     rows, cols = x.shape
+    if cols > MAX_COLUMNS:
+        raise SpDNNError(-1, f"a matrix has at most {MAX_COLUMNS} columns")
     operand = _operand(x, rows, cols, None, "x")
     blocks = (cols + 31) // 32
     codes = x.new_empty((rows, blocks, 16), dtype=torch.uint8)
@@ -189,6 +194,9 @@ class SparseTopology:
             raise SpDNNError(-1, f"col_ptr must have {outputs + 1} entries")
         if row_idx.ndim != 1 or row_idx.size != int(col_ptr[-1]):
             raise SpDNNError(-1, "row_idx size must equal col_ptr[-1]")
+        for v, name in ((inputs, "inputs"), (outputs, "outputs"), (slots, "slots"), (-1 if device is None else device, "device")):
+            if not -(1 << 31) <= v < 1 << 31:
+                raise SpDNNError(-1, f"{name} is out of range")
         self._col_ptr, self._row_idx = col_ptr, row_idx
         self.device = None if device is None else int(device)
         _call(self._lib.spdnn_topology_create, C.byref(self._top), -1 if device is None else self.device, inputs, outputs, slots,
@@ -262,6 +270,8 @@ class SparseTopology:
         if len(x.shape) != 2:
             raise SpDNNError(-1, f"x must be [tokens, {self.inputs}]")
         tokens, device = x.shape[0], self.device
+        if tokens > MAX_TOKENS:
+            raise SpDNNError(-1, f"at most {MAX_TOKENS} tokens a call")
         xo = _operand(x, tokens, self.inputs, device, "x")
         ops = [xo]
         for w in weights:

@@ -5,7 +5,7 @@ import subprocess
 import numpy as np
 import pytest
 
-from graphchallenge21_b200 import Saved, SparseTopology, SpDNNError
+from graphchallenge21_b200 import MX4, Saved, SparseTopology, SpDNNError, mx4_quantize
 from graphchallenge21_b200 import build, feedforward
 
 torch = pytest.importorskip("torch")
@@ -81,3 +81,36 @@ def test_rows_that_are_not_a_matrix_of_indices_are_refused():
     for t in (np.int8, np.uint16, np.int64, np.float32):
         assert SparseTopology.from_rows(np.array([[3, 1]], dtype=t), 8, device=None).rows().tolist() == [[1, 3]]
     assert SparseTopology.from_rows([[3, -2 ** 40], [1, -1]], 8, device=None).rows().tolist() == [[3, -1], [1, -1]]
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """They would reach the library modulo 2^32."""
+    for sizes in (dict(inputs=2 ** 32 + 4), dict(inputs=4 - 2 ** 32), dict(inputs=4, slots=2 ** 32 + 2), dict(inputs=4, device=2 ** 32)):
+        with pytest.raises(SpDNNError, match="out of range"):
+            SparseTopology(outputs=1, col_ptr=[0, 1], row_idx=[0], **{"device": None, **sizes})
+    with pytest.raises(SpDNNError, match="inputs and outputs"):
+        SparseTopology(2 ** 31 - 1, 1, [0, 1], [0], device=None)
+
+
+class Shape:
+    """What the binding looks at of a tensor that is too large for this test."""
+    is_cuda, dtype = True, torch.float16
+
+    def __init__(self, *shape):
+        self.shape = shape
+
+    def dim(self):
+        return len(self.shape)
+
+
+def test_matrices_of_more_rows_or_columns_than_a_call_takes_are_refused():
+    top = on_the_host()
+    top.inputs, top.slots, top._top = 1, 1, True
+    for tokens in (2 ** 26 + 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5):
+        with pytest.raises(SpDNNError, match="tokens a call"):
+            top._begin(Shape(tokens, 1), (), "none")
+    for cols in (2 ** 30 + 1, 2 ** 32 + 32):
+        with pytest.raises(SpDNNError, match="columns"):
+            mx4_quantize(Shape(1, cols))
+        with pytest.raises(SpDNNError, match="columns"):
+            MX4(Shape(1, cols // 32, 16), Shape(1, cols // 32), cols)
