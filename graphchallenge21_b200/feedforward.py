@@ -6,7 +6,8 @@ weights given to each call, and their gradients.  ``mx4_quantize`` makes microsc
 activations, which the forward calls take in place of tensors.
 
 Calls enqueue on torch's current stream of the tensors' device and return at once; they may be captured into CUDA graphs.
-Nothing here is differentiated by autograd: the gradients are the ``*_backward`` calls.
+Nothing here is differentiated by autograd: the gradients are the ``*_backward`` calls, and tensors that require grad are refused
+unless grad mode is off (``torch.no_grad()``, the forward and backward of an ``autograd.Function``), as torch's own ``out=`` does.
 """
 from __future__ import annotations
 
@@ -23,15 +24,15 @@ _ERR_LEN = 256
 
 
 _TYPES = {}          # torch type -> SPDNN_F32 ..., filled with what follows when torch is first needed
-_F32 = _U8 = _raw_stream = None
+_F32 = _U8 = _raw_stream = _grad_enabled = None
 _byref, _Operand = C.byref, _lib.Operand
 
 
 def _torch():
     import torch
-    global _F32, _U8, _raw_stream
+    global _F32, _U8, _raw_stream, _grad_enabled
     if not _TYPES:
-        _F32, _U8 = torch.float32, torch.uint8
+        _F32, _U8, _grad_enabled = torch.float32, torch.uint8, torch.is_grad_enabled
         # torch.cuda.current_stream makes an object for the handle, in twenty times the time
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
@@ -102,6 +103,13 @@ def _on(device, fn, *args):
             _call(fn, *args)
 
 
+def _refuse_grad(name):
+    """For a tensor that requires grad: its result would have no graph, and the gradient would be lost without a word."""
+    if _grad_enabled():
+        raise SpDNNError(-1, f"{name} requires grad, which these calls do not record: pass it detached, or call under torch.no_grad() and "
+                             "use the backward call")
+
+
 def _operand(t, rows, cols, device, name):
     """The C operand of a matrix [rows, cols] on GPU ``device`` (None: any)."""
     if isinstance(t, MX4):
@@ -113,6 +121,8 @@ def _operand(t, rows, cols, device, name):
             raise SpDNNError(-1, f"{name} must be a CUDA tensor")
         if t.shape != (rows, cols):
             raise SpDNNError(-1, f"{name} must be {(rows, cols)}, not {tuple(t.shape)}")
+        if t.requires_grad:
+            _refuse_grad(name)
         stride, step = t.stride()
         if step != 1 and cols > 1:
             raise SpDNNError(-1, f"{name} must have adjacent elements in a row (stride 1)")
@@ -283,6 +293,8 @@ class SparseTopology:
             return None
         if b.dtype is not _F32 or b.get_device() != self.device or b.shape != (self.outputs,) or not b.is_contiguous():
             raise SpDNNError(-1, f"a bias must be contiguous float32 [{self.outputs}] on the topology's device")
+        if b.requires_grad:
+            _refuse_grad("a bias")
         return b.data_ptr()
 
     def _workspace(self, x, *key):

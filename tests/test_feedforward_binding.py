@@ -114,3 +114,22 @@ def test_matrices_of_more_rows_or_columns_than_a_call_takes_are_refused():
             mx4_quantize(Shape(1, cols))
         with pytest.raises(SpDNNError, match="columns"):
             MX4(Shape(1, cols // 32, 16), Shape(1, cols // 32), cols)
+
+
+def test_tensors_that_require_grad_are_refused_in_grad_mode():
+    top = on_the_host()
+    bias = torch.zeros(6, requires_grad=True)
+
+    class Parameter:
+        """A matrix on the GPU as far as the binding looks."""
+        is_cuda, dtype, requires_grad, shape = True, torch.float32, True, (3, 4)
+        stride, data_ptr, get_device = (lambda self: (4, 1)), (lambda self: 0), (lambda self: 0)
+
+    with pytest.raises(SpDNNError, match="weights requires grad"):
+        feedforward._operand(Parameter(), 3, 4, 0, "weights")
+    with pytest.raises(SpDNNError, match="a bias requires grad"):
+        top._bias(bias)
+    with torch.no_grad():
+        feedforward._operand(Parameter(), 3, 4, 0, "weights")
+        assert top._bias(bias) == bias.data_ptr()
+    assert top._bias(bias.detach()) == bias.data_ptr()

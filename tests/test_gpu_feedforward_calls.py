@@ -1,7 +1,7 @@
 """GPU tests of how the feed-forward operators are called: what they refuse, and first calls."""
 import pytest
 
-from test_gpu_feedforward import BF16, Problem, torch
+from test_gpu_feedforward import BF16, F32, Problem, torch
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,45 @@ def test_the_first_call_comes_from_another_stream_at_once(tokens):
             torch.cuda.current_stream().synchronize()
         assert torch.equal(y, want)
         top.close()
+
+
+def test_tensors_that_require_grad_are_refused_in_grad_mode():
+    from graphchallenge21_b200 import SpDNNError, mx4_quantize
+    p = Problem(7, 40, 30, 4, F32, 2)
+    y, saved = p.forward("silu", save=True)
+    grads = p.backward(saved, "silu")
+    out = torch.empty_like(y)
+    for t in (p.x, *p.w, *p.b, p.dy, out):
+        t.requires_grad_()
+        with pytest.raises(SpDNNError, match="requires grad"):
+            p.backward(saved, "silu") if t is p.dy else p.forward("silu", out=out)
+        if t is p.x:
+            with pytest.raises(SpDNNError, match="requires grad"):
+                mx4_quantize(t)
+        with torch.no_grad():
+            assert torch.equal(p.forward("silu", out=out), y) and torch.equal(p.backward(saved, "silu")[0], grads[0])
+        t.requires_grad_(False)
+
+
+def test_inside_an_autograd_function():
+    """As a training program uses the calls: grad mode is off in both directions."""
+    p = Problem(20, 40, 30, 4, F32, 2)
+
+    class Block(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, wg, wu, bg, bu):
+            y, ctx.saved = p.top.gated(x, wg, wu, bg, bu, save=True)
+            ctx.save_for_backward(x, wg, wu)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            dx, dwg, dwu, dbg, dbu = p.top.gated_backward(dy.contiguous(), *ctx.saved_tensors, ctx.saved)
+            return dx, dwg, dwu, dbg, dbu
+
+    leaves = [t.requires_grad_() for t in (p.x, *p.w, *p.b)]
+    got = torch.autograd.grad((Block.apply(*leaves) * p.dy).sum(), leaves)
+    for t in leaves:
+        t.requires_grad_(False)
+    dx, dw, db = p.backward(p.forward("silu", save=True)[1], "silu")
+    assert all(torch.equal(a, b) for a, b in zip(got, [dx, *dw, *db]))
