@@ -85,11 +85,14 @@ class MX4:
         """The values as a tensor (float32 unless ``dtype`` or ``out`` says otherwise)."""
         torch = _torch()
         device = self.codes.get_device()
+        given = out
         if out is None:
             out = self.codes.new_empty(self.shape, dtype=dtype or torch.float32)
         operand = _operand(out, *self.shape, device, "out")
         _on(device, _lib.load().spdnn_mx4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
             _byref(operand), _stream(device))
+        if given is not None:
+            _written(given)
         return out
 
 
@@ -101,6 +104,11 @@ def _on(device, fn, *args):
     else:
         with cuda.device(device):
             _call(fn, *args)
+
+
+def _written(t):
+    """A tensor of the caller has new values: autograd must notice if it was kept for a gradient."""
+    _torch().autograd.graph.increment_version(t)
 
 
 def _refuse_grad(name):
@@ -330,6 +338,7 @@ class SparseTopology:
         tokens, kind, refs, x_type, w_type = self._begin(x, weights, activation)
         refs += [self._bias(b) for b in biases]
         like = x.codes if x_type == MX4_TYPE else x
+        given = out
         if out is None:
             if out_dtype is None and like is not x:
                 raise SpDNNError(-1, "out_dtype is needed for microscaled activations")
@@ -344,6 +353,8 @@ class SparseTopology:
             z = (None,) * len(weights)
         ws, size, keep = self._workspace(like, tokens, len(weights), x_type, w_type, 0)
         _call(fn, self._top, tokens, *refs, kind, clip, _byref(y), *z, ws, size, _stream(self.device))
+        if given is not None:
+            _written(given)
         return (out, saved) if save else out
 
     def linear(self, x, w, bias=None, activation: str = "none", clip: float = 32.0, save: bool = False, out_dtype=None, out=None):

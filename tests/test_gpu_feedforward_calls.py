@@ -74,3 +74,23 @@ def test_inside_an_autograd_function():
         t.requires_grad_(False)
     dx, dw, db = p.backward(p.forward("silu", save=True)[1], "silu")
     assert all(torch.equal(a, b) for a, b in zip(got, [dx, *dw, *db]))
+
+
+def test_results_in_tensors_of_the_caller_count_as_changes_of_them():
+    """A tensor that autograd has kept for a gradient and that a call writes to is found out, as with torch's own operations."""
+    from graphchallenge21_b200 import mx4_quantize
+    p = Problem(7, 40, 30, 4, F32, 1)
+    q = mx4_quantize(p.w[0])
+    for write, shape in ((lambda t: p.forward("silu", out=t), (7, 30)), (lambda t: q.dequantize(out=t), (30, 4))):
+        out = torch.ones(shape, device="cuda")
+        w = torch.ones(shape, device="cuda", requires_grad=True)
+        loss = (w * out).sum()
+        before = out._version
+        write(out)
+        assert out._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            kept = torch.ones(shape, device="cuda")
+            write(kept)                                    # has no version to count
+        assert torch.equal(kept, out)
