@@ -62,6 +62,7 @@ SYMBOLS = {
     "spdnn_topology_destroy": (None, [C.c_void_p]),
     "spdnn_topology_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int),
                                       C.POINTER(C.c_int64)]),
+    "spdnn_topology_blocks": (C.c_int, [C.c_void_p, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "spdnn_topology_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64]),
     "spdnn_layer_workspace": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int64)]),
     "spdnn_linear": (C.c_int, [C.c_void_p, C.c_int, _OP, _OP, C.c_void_p, C.c_int, C.c_float, _OP, _OP, *_TAIL]),

@@ -42,6 +42,7 @@ struct spdnn_topology : DeviceTopology {
     Topology host;
     int device = -1;                // -1: analysis only
     int sm_count = 0;
+    int block_count[2] = {0, 0};    // forward, backward
     // plans made so far: functions of the topology and the key, kept because a call may come every few microseconds
     mutable std::mutex plans_lock;
     mutable std::map<std::array<int, 5>, GatherPlan> plans;
@@ -623,6 +624,8 @@ extern "C" int spdnn_topology_create(spdnn_topology_t **out, int device, int inp
             delete t;
             return fail(err, err_len, SPDNN_ERR_ARG, why);
         }
+        t->block_count[0] = t->host.forward_blocks.blocks;
+        t->block_count[1] = t->host.backward_blocks.blocks;
         if (device < 0) {
             *out = t;
             return SPDNN_OK;
@@ -668,6 +671,13 @@ extern "C" int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int
     if (slots) *slots = top->host.slots;
     if (fan_out) *fan_out = top->host.fan_out;
     if (connections) *connections = top->host.connections;
+    return SPDNN_OK;
+}
+
+extern "C" int spdnn_topology_blocks(const spdnn_topology_t *top, int *forward, int *backward) {
+    if (!top) return SPDNN_ERR_ARG;
+    if (forward) *forward = top->block_count[0];
+    if (backward) *backward = top->block_count[1];
     return SPDNN_OK;
 }
 

@@ -201,7 +201,8 @@ def _int32(a, name):
 class SparseTopology:
     """The connections between ``inputs`` and ``outputs`` neurons, as CSC: output c is connected to inputs
     ``row_idx[col_ptr[c]:col_ptr[c + 1]]``.  ``slots``: columns of a weight matrix (0: as many as the output with most
-    connections has).  ``device=None``: analysis only (``rows``, ``pack``), no GPU needed."""
+    connections has).  ``device=None``: analysis only (``rows``, ``pack``), no GPU needed.  ``blocks``: how many groups of up to 16
+    neurons with equal connections the tensor cores take, forward and backward (0: none, too few neurons share theirs)."""
 
     def __init__(self, inputs: int, outputs: int, col_ptr, row_idx, device: int | None = 0, slots: int = 0):
         self._top = C.c_void_p()
@@ -221,6 +222,9 @@ class SparseTopology:
               C.c_void_p(col_ptr.ctypes.data), C.c_void_p(row_idx.ctypes.data))
         slots, fan_out, connections = C.c_int(), C.c_int(), C.c_int64()
         self._lib.spdnn_topology_info(self._top, None, None, C.byref(slots), C.byref(fan_out), C.byref(connections))
+        forward, backward = C.c_int(), C.c_int()
+        self._lib.spdnn_topology_blocks(self._top, C.byref(forward), C.byref(backward))
+        self.blocks = forward.value, backward.value
         self.inputs, self.outputs = int(inputs), int(outputs)
         self.slots, self.fan_out, self.connections = slots.value, fan_out.value, connections.value
 

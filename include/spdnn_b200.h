@@ -259,6 +259,11 @@ void spdnn_topology_destroy(spdnn_topology_t *top);
 /* slots: columns of a weight matrix; fan_out: most outputs that one input feeds.  Pointers may be NULL. */
 int spdnn_topology_info(const spdnn_topology_t *top, int *inputs, int *outputs, int *slots, int *fan_out, int64_t *connections);
 
+/* Blocks of up to 16 neurons with equal lists of connections (outputs over the same inputs; inputs read by the same outputs), which 16-bit calls of
+ * 17 tokens or more take to the tensor cores.  0: too few neurons share their list, and connections are gathered one by one.  It does not
+ * depend on how the neurons are numbered.  Pointers may be NULL. */
+int spdnn_topology_blocks(const spdnn_topology_t *top, int *forward, int *backward);
+
 /* The canonical order, to host memory: rows[outputs][slots] = inputs of every output ascending, -1 behind the last one. */
 int spdnn_topology_rows(const spdnn_topology_t *top, int32_t *rows, int64_t capacity);
 
