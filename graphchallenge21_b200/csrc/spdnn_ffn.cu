@@ -470,7 +470,7 @@ int run_forward(const Call &c, const float *b0, const float *b1) {
     }
     const DeviceTable &t = c.top->forward;
     const int it = image_type(c.x->type), wt = ordered_type(c.x->type, c.w[0]->type);
-    const GatherPlan g = plan_gather(*c.top, true, std::max(c.tokens, 1), c.sets, it, wt);
+    const GatherPlan g = plan_gather(*c.top, true, c.tokens, c.sets, it, wt);
     const Workspace ws = layout(*c.top, g, t, c.tokens, c.sets, it, wt, false);
     if ((rc = check_run(c, ws.total)) || (rc = check_blocks(c, g))) return rc;
     OnDevice guard(c.top->device);
@@ -600,8 +600,10 @@ int run_backward(const Call &c, const Gradients &d) {
     }
     if (d.dw[0] && e == cudaSuccess) {
         const DeviceBlocks &b = c.top->forward_blocks;
-        if (e == cudaSuccess && go_by_blocks(b, c.tokens, type, type)) e = launch_dw_blocks(c, d, b, type, base + ws.x_columns, (const float *)(base + ws.d_columns), stride);
-        else if (e == cudaSuccess) e = launch_dw(c, d, type, base + ws.x_columns, (const float *)(base + ws.d_columns), stride);
+        const char *x_columns = base + ws.x_columns;
+        const float *d_columns = (const float *)(base + ws.d_columns);
+        e = go_by_blocks(b, c.tokens, type, type) ? launch_dw_blocks(c, d, b, type, x_columns, d_columns, stride)
+                                                  : launch_dw(c, d, type, x_columns, d_columns, stride);
     }
     if (e != cudaSuccess) return fail_cuda(c.err, c.err_len, e);
     return SPDNN_OK;

@@ -211,39 +211,6 @@ template <class E> __device__ __forceinline__ f32x2 widen_word(uint32_t w) {
     else return widen<E>(w);
 }
 
-// V consecutive values of one neuron as pairs of floats (V = 1: one pair with a zero).
-template <class E, int V> struct Values {
-    static constexpr int kPairs = (V + 1) / 2;
-    f32x2 v[kPairs];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) v[i] = 0;
-    }
-    __device__ __forceinline__ void load(const void *p) {
-        constexpr int bytes = V * (int)sizeof(E);
-        if constexpr (sizeof(E) == 4) {
-            if constexpr (bytes == 16) {
-                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(p);
-                v[0] = w.x; v[1] = w.y;
-            } else if constexpr (bytes == 8) {
-                v[0] = *reinterpret_cast<const f32x2 *>(p);
-            } else {
-                v[0] = pack2(*reinterpret_cast<const float *>(p), 0.0f);
-            }
-        } else if constexpr (bytes == 16) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(p);
-            v[0] = widen<E>(w.x); v[1] = widen<E>(w.y); v[2] = widen<E>(w.z); v[3] = widen<E>(w.w);
-        } else if constexpr (bytes == 8) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p);
-            v[0] = widen<E>(w.x); v[1] = widen<E>(w.y);
-        } else if constexpr (bytes == 4) {
-            v[0] = widen<E>(*reinterpret_cast<const uint32_t *>(p));
-        } else {
-            v[0] = pack2(to_float(*reinterpret_cast<const E *>(p)), 0.0f);
-        }
-    }
-};
-
 // V consecutive 16- or 32-bit values as they are in memory.
 template <class E, int V> struct Raw {
     static constexpr int kBytes = V * (int)sizeof(E);
@@ -1271,14 +1238,12 @@ __global__ void __launch_bounds__(kBlockWarps * 32) block_kernel(const __grid_co
     // where the copies are: unit, chunk of its list, which begins at chunk `begin` and has `count`; S sets one after another
     int64_t ahead = first;
     uint32_t begin = 0, count = 0, at = 0;
-    const auto open = [&] {                            // skips blocks without connections
-        for (; ahead < last; ++ahead) {
-            const int b = (int)(ahead / tiles);
-            begin = __ldg(a.chunk_ptr + b);
-            count = __ldg(a.chunk_ptr + b + 1) - begin;
-            at = 0;
-            if (count) return;
-        }
+    const auto open = [&] {
+        if (ahead >= last) return;
+        const int b = (int)(ahead / tiles);
+        begin = __ldg(a.chunk_ptr + b);
+        count = __ldg(a.chunk_ptr + b + 1) - begin;    // at least one
+        at = 0;
     };
     open();
     uint32_t row = ahead < last ? __ldg(a.rows + (size_t)begin * 32 + lane) : 0u;
@@ -1503,10 +1468,9 @@ __global__ void __launch_bounds__(kDwThreads, G == 1 ? 7 : 4) dw_kernel(const Dw
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int i = 0; i < PAIRS; i += 2) {
-                Values<float, 4> part;
-                part.zero();
-                if (inside) part.load(d + g * a.token_stride + t + 2 * i);
-                dv[g][i] = part.v[0]; dv[g][i + 1] = part.v[1];
+                ulonglong2 part = make_ulonglong2(0, 0);
+                if (inside) part = *(const ulonglong2 *)(d + g * a.token_stride + t + 2 * i);
+                dv[g][i] = part.x; dv[g][i + 1] = part.y;
             }
 #pragma unroll
         for (int j = 0; j < kDwSlots; j += BATCH) {
