@@ -657,7 +657,7 @@ __device__ __forceinline__ void order_blocks_block(const OrderBlocksArgs &a, uns
 
 // Everything that a call lays out, in one launch (a launch takes longer than most of these blocks): the table, then image and columns
 // of the gathered values, then (backward) the columns of x.  Measured: 4096 tokens x 4096, bf16, and a table of 524288 connections 21 us (34 MB in, 37
-// out); dL/dz of 4096 x 4096, both sets, with 4096 x 1024 of x 81 us (177 MB in, 201 out: 4.7 TB/s).
+// out); dL/dz of 4096 x 4096, both sets, with 4096 x 1024 of x 75 us (176 MB in, 210 out: 5.1 TB/s).
 struct PrepareArgs {
     OrderArgs order;
     OrderBlocksArgs blocks;
@@ -666,8 +666,10 @@ struct PrepareArgs {
     unsigned order_blocks, main_blocks;     // the rest are x's
 };
 
+// Of gradients five blocks an SM (six of fp32) need no spills: left to itself the compiler took 60 registers for four blocks and 79 and 97 us where these
+// take 75 and 88 (4096 tokens x 4096, bf16; 1024 x 16384, fp16; both sets).
 template <class E, class W, int SETS, bool GRADIENT>
-__global__ void __launch_bounds__(kPackThreads) prepare_kernel(const __grid_constant__ PrepareArgs a) {
+__global__ void __launch_bounds__(kPackThreads, GRADIENT ? (sizeof(E) == 2 ? 5 : 6) : 0) prepare_kernel(const __grid_constant__ PrepareArgs a) {
     constexpr int MAIN = pack_tile_bytes<E, GRADIENT ? SETS : 1, GRADIENT>(), X = pack_tile_bytes<E, 1, false>();
     __shared__ __align__(16) unsigned char shared[MAIN > X ? MAIN : X];
     if (blockIdx.x < a.order_blocks) {
