@@ -13,7 +13,6 @@
 #include <string>
 #include <thread>
 #include <unordered_map>
-#include <utility>
 #include <vector>
 
 namespace spdnn_impl {
@@ -162,7 +161,7 @@ private:
     bool seen_[16];
 };
 
-// Runs f(begin, end) over [0, n) in a few host threads (large topologies: 16384 neurons of 32 connections take 15 ms in one).
+// Runs f(begin, end) over [0, n) in a few host threads (large topologies: 16384 neurons of 32 connections take 86 ms in one, 20 in eight, with all else).
 template <class F>
 inline void in_threads(int n, int64_t work, const F &f) {
     const int threads = (int)std::min<int64_t>(std::min<int64_t>(std::max(1u, std::thread::hardware_concurrency()), 8), work / 32768 + 1);
@@ -219,27 +218,6 @@ inline std::string build_gather_table(int outs, int rows, const std::vector<uint
 // The blocks of a gather: neuron i gathers row(i, k) for k < length(i), with the weight at source(i, k).
 template <class Length, class Row, class Source>
 inline void build_block_table(int outs, int rows, int64_t entries, const Length &length, const Row &row, const Source &source, BlockTable &t) {
-    std::vector<uint64_t> hash(outs);
-    in_threads(outs, entries, [&](int begin, int end) {
-        for (int i = begin; i < end; ++i) {
-            uint64_t h = 0x9E3779B97F4A7C15ull ^ length(i);
-            for (size_t k = 0; k < length(i); ++k) h = (h ^ row(i, k)) * 0xBF58476D1CE4E5B9ull, h ^= h >> 29;
-            hash[i] = h;
-        }
-    });
-    // Whether blocks are worth it, from equal hashes, whatever the neurons' order: a random topology is given up here, before its lists are compared.
-    // (Different lists of one hash would count as too few chunks; the lists decide then.)
-    {
-        std::vector<std::pair<uint64_t, uint32_t>> sorted(outs);
-        for (int i = 0; i < outs; ++i) sorted[i] = {hash[i], (uint32_t)length(i)};
-        std::sort(sorted.begin(), sorted.end());
-        int64_t chunks = 0;
-        for (size_t i = 0, j; i < sorted.size(); i = j) {
-            for (j = i + 1; j < sorted.size() && sorted[j] == sorted[i]; ++j) {}
-            chunks += (int64_t)((j - i + 15) / 16) * std::max<int64_t>(1, ((int64_t)sorted[i].second + 31) / 32);
-        }
-        if (!entries || chunks * 512 > entries * kBlockWaste) return;
-    }
     std::unordered_map<uint64_t, int> newest;          // hash of a list -> the class that was opened last for it
     std::vector<int> first, older;                     // of a class: its first neuron; the class before it with the same hash
     std::vector<std::vector<int32_t>> members;
@@ -249,8 +227,11 @@ inline void build_block_table(int outs, int rows, int64_t entries, const Length 
             if (row(i, k) != row(j, k)) return false;
         return true;
     };
+    int64_t chunks = 0, blocks = 0;
     for (int i = 0; i < outs; ++i) {
-        const auto found = newest.find(hash[i]);
+        uint64_t h = 0x9E3779B97F4A7C15ull ^ length(i);
+        for (size_t k = 0; k < length(i); ++k) h = (h ^ row(i, k)) * 0xBF58476D1CE4E5B9ull, h ^= h >> 29;
+        const auto found = newest.find(h);
         int c = found == newest.end() ? -1 : found->second;
         while (c >= 0 && !same(first[c], i)) c = older[c];
         if (c < 0) {
@@ -258,17 +239,16 @@ inline void build_block_table(int outs, int rows, int64_t entries, const Length 
             first.push_back(i);
             older.push_back(found == newest.end() ? -1 : found->second);
             members.emplace_back();
-            newest[hash[i]] = c;
+            newest[h] = c;
+        }
+        // They only grow, so it does not matter in which order the neurons come; of a random topology an eighth of them is read.
+        if (members[c].size() % 16 == 0) {
+            ++blocks;
+            chunks += (int64_t)std::max<size_t>(1, (length(i) + 31) / 32);
+            if (chunks * 512 > entries * kBlockWaste) return;
         }
         members[c].push_back(i);
     }
-    int64_t chunks = 0, blocks = 0;
-    for (size_t c = 0; c < first.size(); ++c) {
-        const int64_t b = ((int64_t)members[c].size() + 15) / 16;
-        blocks += b;
-        chunks += b * (int64_t)std::max<size_t>(1, (length(first[c]) + 31) / 32);
-    }
-    if (chunks * 512 > entries * kBlockWaste) return;
     t.blocks = (int)blocks;
     t.chunk_ptr.assign(1, 0);
     t.chunk_ptr.reserve(blocks + 1);
