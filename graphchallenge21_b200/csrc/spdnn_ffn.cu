@@ -148,7 +148,7 @@ GatherPlan make_plan(const spdnn_topology &top, bool forward, int tokens, int se
         const int v = std::min(T, full), p = T / v, nv = lane_units(p), lanes = p / nv;
         const int64_t bytes = image_size(t.rows, s_values, v, p, size), tiles = ((int64_t)tokens + T - 1) / T, units = (int64_t)slices * lanes;
         const int warps = gather_threads(v * nv * sums) / 32;
-        // Clocks, fitted to a sweep of T and splits over 15 sizes (33 to 4096 tokens, 300 to 16384 neurons; the choice is 1 % off the best of the
+        // Clocks, fitted to a sweep of T and splits over 15 sizes (33 to 4096 tokens, 300 to 16384 neurons; the choice is 0.4 % off the best of the
         // sweep in the mean).  A connection of a warp takes the shared memory's wavefronts (1.3 per 128 bytes in the order of topology.h,
         // more where more neurons are read at a time than it was made for) with those of the table, or its instructions on four
         // schedulers; a quad that a warp works on alone, the latency of its loads and instructions.

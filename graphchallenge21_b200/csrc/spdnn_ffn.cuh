@@ -7,13 +7,16 @@
 //              dx[t,i]  = sum over connections (c,j) with r(c,j) = i of  sum_s w_s[c,j] d_s[t,c]
 //              dw_s[c,j] = sum_t d_s[t,c] x[t,r(c,j)],   db_s[c] = sum_t d_s[t,c]
 //
-// There is no dense contraction in this: what a multiply-add costs is fetching its activation.  So activations are gathered in
-// vectors over TOKENS: an IMAGE holds the values of T tokens of every neuron side by side, one load brings a connection's
-// activation for up to eight tokens, and its index and weights are fetched once for all of them.  pack_kernel writes the
+// Of a pattern in general there is no dense contraction in this: what a multiply-add costs is fetching its activation.  So activations are gathered
+// in vectors over TOKENS: an IMAGE holds the values of T tokens of every neuron side by side, one load brings a connection's
+// activation for up to eight tokens, and its index and weights are fetched once for all of them.  prepare_kernel writes the
 // images (and takes in whatever is irregular: strides, types, 4-bit blocks, the last tokens), gather_kernel brings one into
-// shared memory and runs a range of neurons on it.
+// shared memory and runs a range of neurons on it.  Where neurons share their connections, 16 of them over the same rows are a small dense
+// contraction, and block_kernel and dw_block_kernel take it to the tensor cores.
 //
-// Roundings: all sums, the pre-activations kept for the backward pass and the d that the weights' gradients are made of are in 32 bits.  The
+// Roundings.  Sums and the pre-activations kept for the backward pass are float32.  Inside a tensor-core instruction products are added without
+// rounding and cut off to float32 (16 products at a time in block_kernel, 32 tokens in dw_block_kernel).  The d that the weights' gradients are made of
+// are float32 too; dw_block_kernel multiplies with their upper 22 bits.  The
 // d that dx gathers is rounded to the activations' type: a gathered value costs what it is wide, in shared memory and in tokens per
 // image, and the error is half a step of every term.  fp16 does not hold d's range (a product of two or three factors of the operands' order), so a
 // token's d are gathered at a power of two of their own (token_scale_kernel), which the sums are divided by again.
@@ -87,7 +90,8 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluA = 0.79788456080286536f, kGeluB = 0.044715f;
 
 // v / (1 + e^-w), the shape of SILU (w = v) and of GELU_TANH (w = 2 a (v + b v^3): (1 + tanh(w / 2)) / 2 = 1 / (1 + e^-w)).  FAST:
-// the hardware's exponential and reciprocal, a few 2^-22 off: for results that are rounded to 16 bits, or made of 16-bit operands.
+// the hardware's exponential and reciprocal, for operands of 16 bits: off by (8 + 2 |w|) 2^-24 of the result, the part that grows with w being of the
+// size of what the rounding of w itself does to the exponential.
 template <bool FAST> __device__ __forceinline__ float sigmoid_times(float v, float w) {
     if (!FAST) return v / (1.0f + expf(-w));
     float e, r;
@@ -1071,7 +1075,7 @@ __device__ __forceinline__ void four_weights(const Matrix &m, bool vector, int c
 }
 
 // Forward pass of up to T tokens in one launch that reads the caller's operands as they are: with few tokens the latency of a call is what
-// counts, and laying out image and weights first would take longer than the sums (one token, 4096 -> 16384, gated, bf16: 3.7 us for 5.3 MB of
+// counts, and laying out image and weights first would take longer than the sums (one token, 4096 -> 16384, gated, bf16: 3.7 us for 3.1 MB of
 // weights and rows; 11.7 in the launches of the images' way when this was written).  Eight lanes share a neuron, four connections
 // of 32 each; the tokens' activations lie in shared memory [inputs + 1][T] (the last row zeros, where missing connections point).
 template <class E, class W, bool MX, int T, int G>

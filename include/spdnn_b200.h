@@ -226,7 +226,9 @@ int spdnn_layer_static(const float *yin, float *yout, int neurons, int live_in, 
  *
  * A set of weights is a matrix [outputs][slots] in CANONICAL order: connection j of a neuron is its j-th smallest input
  * (spdnn_topology_rows).  What a matrix holds where a neuron has no j-th connection is never read; gradients are zero there.
- * Sums run in 32 bits, in no order that callers may rely on; results are rounded once. */
+ * Sums are held in float32, in no order that callers may rely on (the tensor cores, which take 16-bit neurons that share their connections, cut
+ * off what they add at a time instead of rounding it); results are rounded once.  Activations are computed in float32 (of 16-bit operands with the
+ * hardware's exponential, also where the result is float32), within (20 + 12 |z| + 2 z^2 + |z|^3) 2^-24 of the value, or 2^-120. */
 typedef struct spdnn_topology spdnn_topology_t;
 
 enum { SPDNN_F32 = 0, SPDNN_F16 = 1, SPDNN_BF16 = 2, SPDNN_MX4 = 3 };
@@ -287,9 +289,10 @@ int spdnn_gated(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *
 
 /* Gradients from dy = dL/dy and what the forward call read and saved; dy, x, w and dx have one float type.  dx
  * [tokens][inputs] or NULL; dw, dbias in fp32 ([outputs][slots] without gaps, [outputs]), overwritten, or NULL (dbias only with dw).
- * z may be NULL for SPDNN_ACT_NONE (linear).  The slope of RELU at 0 is 0, of CLIP at 0 and clip too.  On its way to
- * dx (not to dw and dbias) dL/dz is rounded to the operands' type; in fp16 after a token's values were multiplied by the power of two that brings the
- * largest into [2^14, 2^15) (the sums are divided by it), so that they keep half a step, or 2^-39 of the token's largest.  Every sum has a fixed order: the same call gives the same bits. */
+ * z may be NULL for SPDNN_ACT_NONE (linear).  The slope of RELU at 0 is 0, of CLIP at 0 and clip too.  Every sum has a fixed order: the same call
+ * gives the same bits.  On its way to dx dL/dz is rounded to the operands' type; in fp16 after a token's values were multiplied by the power of two
+ * that brings the largest into [2^14, 2^15) (the sums are divided by it), so that they keep half a step, or 2^-39 of the token's largest.  On its way to dw it is
+ * not rounded, but of 16-bit neurons that share their connections 22 bits of it are multiplied. */
 int spdnn_linear_backward(const spdnn_topology_t *top, int tokens, const spdnn_operand_t *dy, const spdnn_operand_t *x,
                           const spdnn_operand_t *w, const spdnn_operand_t *z, int activation, float clip, const spdnn_operand_t *dx,
                           float *dw, float *dbias, void *workspace, int64_t workspace_bytes, void *cuda_stream, char *err,

@@ -173,3 +173,17 @@ def test_slopes_of_huge_pre_activations(kind, dtype, shared):
     assert torch.isfinite(dx).all() and torch.isfinite(db).all()
     reads = top.outputs if shared else 1
     assert torch.equal(dx[:, 0], (v > 0).to(dtype) * reads)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("tokens, shared", [(4, False), (999, False), (999, True)])
+def test_activations_to_a_relative_bound(tokens, shared, kind, dtype):
+    """(20 + 12 |z| + 2 z^2 + |z|^3) u of the value: the exponent w of SILU is z, of the tanh form 1.6 z + 0.072 z^3; five roundings of w and two of
+    the exponential's argument make 7 u |w| of the exponential at most, GELU's v^2 / 2 less than 2 z^2 u; the rest is below 20 u."""
+    v = torch.linspace(-20, 20, tokens, device="cuda").to(dtype)
+    y = activation_of(v, dtype, kind, tokens, shared, F32)[3][:, 0]
+    z = v.double()
+    w = z if kind == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    want = 0.5 * z * torch.erfc(-z * math.sqrt(0.5)) if kind == "gelu" else z / (1 + torch.exp(-w))
+    check(y, want, (20 + 12 * z.abs() + 2 * z * z + z.abs() ** 3) * ref.U * want.abs() + 2.0 ** -120, kind)
