@@ -347,7 +347,12 @@ class SparseTopology:
             if out_dtype is None and like is not x:
                 raise SpDNNError(-1, "out_dtype is needed for microscaled activations")
             out = like.new_empty((tokens, self.outputs), dtype=out_dtype)
-        y = _operand(out, tokens, self.outputs, self.device, "out")
+            y_type = x_type if out_dtype is None else _TYPES.get(out_dtype)
+            if y_type is None:
+                raise SpDNNError(-1, f"out is {out_dtype}, not float32, float16 or bfloat16")
+            y = _Operand(out.data_ptr(), None, self.outputs, y_type, 0)
+        else:
+            y = _operand(out, tokens, self.outputs, self.device, "out")
         if save:
             if like is not x:
                 raise SpDNNError(-1, "microscaled activations have no backward pass: nothing to save")

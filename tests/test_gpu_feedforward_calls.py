@@ -153,3 +153,13 @@ def test_fp16_gradients_leave_what_is_behind_them_alone(tokens):
     for got, w, size in ((dw[0], want[1][0], 75 * p.top.slots), (dw[1], want[1][1], 75 * p.top.slots), (db[0], want[2][0], 75), (db[1], want[2][1], 75)):
         assert torch.equal(got[:size], w.reshape(-1)) and (got[size:] == 7).all()
     assert (ws[n.value:] == 0xA5).all()
+
+
+def test_result_types_that_do_not_exist_are_refused():
+    from graphchallenge21_b200 import SpDNNError
+    p = Problem(7, 40, 30, 4, BF16, 1)
+    for t in (torch.float64, torch.int32, torch.uint8):
+        with pytest.raises(SpDNNError, match="not float32"):
+            p.forward("silu", out_dtype=t)
+        with pytest.raises(SpDNNError, match="not float32"):
+            p.forward("silu", out=torch.empty(7, 30, dtype=t, device="cuda"))
