@@ -761,7 +761,8 @@ template <class W, int SETS, bool WIDE> struct Quad {
 // quad: each is requested while the one before it is worked on, the first of a unit before the last of the one before it.
 //
 // Measured: 4096 tokens, 4096 -> 16384, gated, bf16 (T = 16) 265 us = 16.2 T fma/s, 0.43 of the FP32 pipe; issue slots 76 % busy, LSU pipe 73 %.  1024
-// tokens, 16384 -> 16384, fp16 (T = 4) 114 us without and 124 with pre-activations; its dx (T = 2, two values a connection) 222 us, LSU pipe 82 %.
+// tokens, 16384 -> 16384, fp16 (T = 4) 114 us without and 124 with pre-activations; its dx (T = 2, two values a connection) 234 us (222 without the
+// factors of the tokens), LSU pipe 79 %.
 template <class E, class W, int V, int P, int S, int G, bool GLOBAL>
 __global__ void __launch_bounds__(gather_threads(V * lane_units(P) * G)) gather_kernel(const __grid_constant__ GatherArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -920,7 +921,7 @@ __device__ __forceinline__ void mma_16x8x8_tf32(float (&c)[4], const uint32_t (&
 // bits) is exact in tf32; d is the sum of two tf32 numbers, 22 bits, and takes two products.  The
 // second has d's sign and is zero for a d of zero only (where nothing is left it is 2^-30 of d; below 2^-96 it may vanish), and an infinite d itself:
 // so an infinity of x or of d goes through both products as it goes through one.  The tensor cores cut sums off instead
-// of rounding them: they add up 32 tokens only, the rest is added in float32.  Measured: 4096 tokens, 1024 -> 4096, both sets, bf16: 50 us (dw_kernel:
+// of rounding them: they add up 32 tokens only, the rest is added in float32.  Measured: 4096 tokens, 1024 -> 4096, both sets, bf16: 53 us (dw_kernel:
 // 119) for 143 MB from HBM; what bounds it is the latency of those loads (128 registers a thread leave 16 warps an SM).
 template <class E, int G>
 __global__ void __launch_bounds__(kDwBlockThreads, 2) dw_block_kernel(const __grid_constant__ DwBlockArgs a) {
